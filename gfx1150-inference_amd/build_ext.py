@@ -26,7 +26,7 @@ LIB_NAME = "libqmm_gfx950.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 
 HIP_SOURCES = ["qmm_api.hip", "qmm_gemv.hip", "qmm_gemv_mfma.hip", "qmm_dequant.hip", "qmm_prefill.hip", "qmm_embed.hip", "qmm_upload.hip", "qmm_layer.hip",
-               "qmm_host.hip"]
+               "qmm_host.hip", "qmm_paged.hip", "qmm_paged_attention.hip", "qmm_beam.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 HIP_FLAGS = [

@@ -1,0 +1,442 @@
+// One step of beam search's selection: the best `beams` of beams x vocab totals
+//   total(w, j) = score_w + x_wj - log sum_i exp(x_wi),
+// without storing any of them.  Bound by reading the logits once.
+//   Pass 1: a block holds one chunk of one beam's logits in registers.  Within a beam the totals are ordered
+//           as the logits, so the chunk's best `beams` logits are found there, beside its maximum and its sum
+//           of exp(x - max).
+//   Pass 2: one block per sentence joins the chunks' sums into each beam's logarithm, in 64 bits, and
+//           ranks the chunks' candidates by (total in 64 bits, beam, token).
+// The order of equal totals and every sum are fixed by the sizes alone, so equal beams give equal totals.
+#include "qmm_paged.h"
+
+#include <algorithm>
+#include <mutex>
+#include <type_traits>
+
+namespace qmm {
+namespace paged {
+namespace {
+
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kMaxBeams = 64;
+constexpr int kWaveList = 128;     // candidates that a wave may list before it narrows them down exactly
+constexpr int kMergeThreads = 1024, kMergeList = 1024;
+
+struct Sum {  // sum of exp(x - m) over a wave's logits
+    double m, s;
+};
+
+struct Candidate {
+    float x;
+    int32_t token;  // -1: none
+};
+
+// A monotone image of the float order; NaN (of either sign) as -inf.
+__device__ __forceinline__ uint32_t order_key(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const uint32_t k = u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+    return x != x ? 0x007FFFFFu : k;
+}
+
+__device__ __forceinline__ double wave_add(double x) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
+    return x;
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
+    return x;
+}
+
+// The largest t that at least n of the wave's keys reach (n <= 64), one bit at a time.
+__device__ __forceinline__ uint32_t wave_threshold(uint32_t key, int n) {
+    uint32_t t = 0;
+#pragma unroll 1
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t c = t | (1u << bit);
+        if (__popcll(__ballot(key >= c)) >= n) t = c;
+    }
+    return t;
+}
+
+__device__ __forceinline__ int lanes_below(uint64_t mask) {
+    return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+}
+
+// exp(d), d <= 0: 2^(d log2 e) with the product's rounding put back, since the terms' errors would otherwise
+// share a sign and move a beam against the others.
+__device__ __forceinline__ float exp_of(float d) {
+    constexpr float kLog2e = 1.44269502162933349609f, kLog2eLow = 1.92596299112661746887e-8f, kLn2 = 0.693147182f;
+    d = d < -200.0f ? -200.0f : d;  // exp is 0 there; -inf would leave a NaN in `rest`
+    const float t = d * kLog2e;
+    const float rest = __fmaf_rn(d, kLog2eLow, __fmaf_rn(d, kLog2e, -t));
+    const float p = __builtin_amdgcn_exp2f(t);
+    return __fmaf_rn(p, rest * kLn2, p);
+}
+
+template <class T>
+struct Piece;  // 16 bytes of logits
+template <>
+struct Piece<float> {
+    using type = f32x4;
+};
+template <>
+struct Piece<_Float16> {
+    using type = f16x8;
+};
+template <>
+struct Piece<__bf16> {
+    using type = bf16x8;
+};
+
+// Chunk blockIdx.x of beam blockIdx.y: E logits a thread, in pieces of 16 bytes.  Which thread takes a token does not
+// depend on the row's address (rows of an odd vocabulary start anywhere), so that equal beams have equal sums to the
+// last bit and their ties stay ties; the pieces are loaded at whatever alignment they have.
+template <class T, int E>
+__global__ __launch_bounds__(kThreads) void select_chunk_kernel(const T* __restrict__ logits, int64_t sentence_stride, int64_t beam_stride,
+                                                                const float* __restrict__ scores, int beams, int vocab,
+                                                                Sum* __restrict__ sums, Candidate* __restrict__ cands) {
+    constexpr int kP = 16 / sizeof(T), kN = E / kP;
+    __shared__ uint64_t list[kWaves * kWaveList];
+    __shared__ int counts[kWaves];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int row = blockIdx.y, chunk = blockIdx.x;
+    const T* base = logits + (row / beams) * sentence_stride + (row % beams) * beam_stride;
+    const int first = chunk * (E * kThreads);  // token of the chunk's first element
+    float x[E];
+#pragma unroll
+    for (int j = 0; j < kN; ++j) {
+        const int at = first + (j * kThreads + tid) * kP;
+        if (at + kP <= vocab) {
+            typename Piece<T>::type p;
+            __builtin_memcpy(&p, base + at, 16);
+#pragma unroll
+            for (int e = 0; e < kP; ++e) x[j * kP + e] = static_cast<float>(p[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kP; ++e) x[j * kP + e] = at + e < vocab ? static_cast<float>(base[at + e]) : -INFINITY;
+        }
+    }
+    // the chunk's maximum and sum
+    float m = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < E; ++e) m = fmaxf(m, x[e]);
+    const float lane_best = m;
+    m = wave_max(m);
+    const float ref = m == -INFINITY ? 0.0f : m;  // nothing but -inf: every term is 0
+    float s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) s += exp_of(x[e] - ref);
+    const double ws = wave_add(static_cast<double>(s));
+    if (lane == 0) sums[(static_cast<int64_t>(row) * gridDim.x + chunk) * kWaves + w] = Sum{static_cast<double>(m), ws};
+
+    // the wave's best `beams`: a lower bound from the lanes' maxima, then every logit that reaches it
+    auto token_of = [&](int e) { return first + ((e / kP) * kThreads + tid) * kP + e % kP; };
+    auto inside = [&](int token) { return token < vocab; };
+    uint64_t* mine = list + w * kWaveList;
+    auto put = [&](bool take, int e, int n) {
+        const uint64_t mask = __ballot(take);
+        if (mask == 0) return n;
+        const int at = n + lanes_below(mask);
+        if (take && at < kWaveList) mine[at] = (static_cast<uint64_t>(order_key(x[e])) << 32) | static_cast<uint32_t>(~token_of(e));
+        return n + static_cast<int>(__popcll(mask));
+    };
+    int n = 0;
+    const bool dead = !(scores[row] > -INFINITY);  // every total is -inf: the lowest tokens stand for the rest
+    if (dead) {
+        if (w == 0) {
+            n = min(beams, vocab - first);  // a chunk holds at least 2048
+            if (lane < n) mine[lane] = static_cast<uint32_t>(~(first + lane));
+        }
+    } else {
+        uint32_t t = wave_threshold(order_key(lane_best), beams);
+#pragma unroll
+        for (int e = 0; e < E; ++e) n = put(order_key(x[e]) >= t && inside(token_of(e)), e, n);
+        if (n > kWaveList) {
+            // many equal logits: the exact bound, then the lowest tokens of those that equal it
+            t = 0;
+#pragma unroll 1
+            for (int bit = 31; bit >= 0; --bit) {
+                const uint32_t c = t | (1u << bit);
+                int count = 0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) count += static_cast<int>(__popcll(__ballot(order_key(x[e]) >= c && inside(token_of(e)))));
+                if (count >= beams) t = c;
+            }
+            int above = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) above += static_cast<int>(__popcll(__ballot(order_key(x[e]) > t && inside(token_of(e)))));
+            uint32_t last = 0x7FFFFFFFu;  // the lowest bound on the token that keeps beams - above of the equal ones
+#pragma unroll 1
+            for (int bit = 30; bit >= 0; --bit) {
+                const uint32_t c = last & ~(1u << bit);
+                int count = 0;
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    count += static_cast<int>(__popcll(__ballot(order_key(x[e]) == t && inside(token_of(e)) && static_cast<uint32_t>(token_of(e)) <= c)));
+                if (above + count >= beams) last = c;
+            }
+            n = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const uint32_t k = order_key(x[e]);
+                n = put(inside(token_of(e)) && (k > t || (k == t && static_cast<uint32_t>(token_of(e)) <= last)), e, n);
+            }
+        }
+    }
+    if (lane == 0) counts[w] = n;
+    __syncthreads();
+
+    const int64_t out = static_cast<int64_t>(row) * gridDim.x + chunk;
+    // rank the waves' lists against each other
+    int start[kWaves], total = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        start[i] = total;
+        total += counts[i];
+    }
+    auto nth = [&](int i) {
+        int from = 0;
+#pragma unroll
+        for (int k = 1; k < kWaves; ++k)
+            if (i >= start[k]) from = k;
+        return list[from * kWaveList + i - start[from]];
+    };
+    Candidate* dst = cands + out * beams;
+    for (int i = tid; i < total; i += kThreads) {
+        const uint64_t own = nth(i);
+        int rank = 0;
+        for (int k = 0; k < kWaves; ++k)
+            for (int c = 0; c < counts[k]; ++c) rank += list[k * kWaveList + c] > own;
+        if (rank < beams) {
+            const int token = static_cast<int>(~static_cast<uint32_t>(own));
+            dst[rank] = Candidate{static_cast<float>(base[token]), token};
+        }
+    }
+    for (int i = total + tid; i < beams; i += kThreads) dst[i] = Candidate{0.0f, -1};
+}
+
+__device__ __forceinline__ bool better(double ta, int ba, int ja, double tb, int bb, int jb) {
+    return ta > tb || (ta == tb && (ba < bb || (ba == bb && ja < jb)));
+}
+
+__global__ __launch_bounds__(kMergeThreads) void select_merge_kernel(const float* __restrict__ scores, const Sum* __restrict__ sums,
+                                                                     const Candidate* __restrict__ cands, int beams, int chunks,
+                                                                     float* __restrict__ out_scores, int32_t* __restrict__ out_parents,
+                                                                     int32_t* __restrict__ out_tokens) {
+    constexpr int kW = kMergeThreads / 64;
+    __shared__ double offset[kMaxBeams];  // score - logarithm; -inf: the beam is out
+    __shared__ uint32_t bounds[kW];
+    __shared__ double l_total[kMergeList];
+    __shared__ int2 l_at[kMergeList];
+    __shared__ int l_n;
+    __shared__ double r_total[kW];
+    __shared__ int2 r_at[kW];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t first_row = static_cast<int64_t>(blockIdx.x) * beams;
+    for (int b = w; b < beams; b += kW) {
+        const int parts = chunks * kWaves;
+        const Sum* sm = sums + (first_row + b) * parts;
+        double m = -INFINITY;
+        for (int i = lane; i < parts; i += 64) m = fmax(m, sm[i].m);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) m = fmax(m, __shfl_xor(m, o, 64));
+        double s = 0.0;
+        for (int i = lane; i < parts; i += 64) {
+            const Sum p = sm[i];
+            if (p.m > -INFINITY || p.s != p.s) s += p.s * exp(p.m - m);
+        }
+        s = wave_add(s);
+        const double at = static_cast<double>(scores[first_row + b]) - (m + log(s));
+        if (lane == 0) offset[b] = at == at ? at : -INFINITY;
+    }
+    if (tid == 0) l_n = 0;
+    __syncthreads();
+    const int per_beam = chunks * beams, n = beams * per_beam;
+    const Candidate* cs = cands + first_row * per_beam;
+    auto total_of = [&](int i, int& b, int& token) {
+        const Candidate c = cs[i];
+        b = i / per_beam;
+        token = c.token;
+        const double t = static_cast<double>(c.x) + offset[b];
+        return t == t ? t : -INFINITY;
+    };
+    // a bound that at least `beams` candidates of some wave reach: totals rounded to fp32 keep their order
+    uint32_t best = 0;
+    for (int i = tid; i < n; i += kMergeThreads) {
+        int b, token;
+        const double t = total_of(i, b, token);
+        if (token >= 0) best = max(best, order_key(static_cast<float>(t)));
+    }
+    const uint32_t t_wave = wave_threshold(best, beams);
+    if (lane == 0) bounds[w] = t_wave;
+    __syncthreads();
+    uint32_t bound = 0;
+    for (int i = 0; i < kW; ++i) bound = max(bound, bounds[i]);
+    for (int i = tid; i < n; i += kMergeThreads) {
+        int b, token;
+        const double t = total_of(i, b, token);
+        if (token >= 0 && order_key(static_cast<float>(t)) >= bound) {
+            const int at = atomicAdd(&l_n, 1);
+            if (at < kMergeList) {
+                l_total[at] = t;
+                l_at[at] = int2{b, token};
+            }
+        }
+    }
+    __syncthreads();
+    auto write = [&](int rank, double t, int2 at) {
+        out_scores[first_row + rank] = static_cast<float>(t);
+        out_parents[first_row + rank] = at.x;
+        out_tokens[first_row + rank] = at.y;
+    };
+    const int listed = l_n;
+    if (listed <= kMergeList) {
+        if (tid < listed) {
+            const double t = l_total[tid];
+            const int2 at = l_at[tid];
+            int rank = 0;
+            for (int i = 0; i < listed; ++i) rank += better(l_total[i], l_at[i].x, l_at[i].y, t, at.x, at.y);
+            if (rank < beams) write(rank, t, at);
+        }
+        return;
+    }
+    // Many equal totals: one after the other, each the best of those after the last one in order.
+    double last_t = INFINITY;
+    int2 last{-1, -1};
+    for (int r = 0; r < beams; ++r) {
+        double bt = -INFINITY;
+        int2 ba{INT32_MAX, INT32_MAX};
+        for (int i = tid; i < n; i += kMergeThreads) {
+            int b, token;
+            const double t = total_of(i, b, token);
+            if (token >= 0 && better(last_t, last.x, last.y, t, b, token) && better(t, b, token, bt, ba.x, ba.y)) {
+                bt = t;
+                ba = int2{b, token};
+            }
+        }
+        for (int o = 32; o > 0; o >>= 1) {
+            const double ot = __shfl_xor(bt, o, 64);
+            const int2 oa{__shfl_xor(ba.x, o, 64), __shfl_xor(ba.y, o, 64)};
+            if (better(ot, oa.x, oa.y, bt, ba.x, ba.y)) {
+                bt = ot;
+                ba = oa;
+            }
+        }
+        if (lane == 0) {
+            r_total[w] = bt;
+            r_at[w] = ba;
+        }
+        __syncthreads();
+        bt = r_total[0];
+        ba = r_at[0];
+        for (int i = 1; i < kW; ++i)
+            if (better(r_total[i], r_at[i].x, r_at[i].y, bt, ba.x, ba.y)) {
+                bt = r_total[i];
+                ba = r_at[i];
+            }
+        last_t = bt;
+        last = ba;
+        if (tid == 0) write(r, bt, ba);
+        __syncthreads();
+    }
+}
+
+// ---- host side -------------------------------------------------------------------------------
+// Logits a thread: as few as leave 512 chunks, so that small calls use the chip's width and large ones read
+// up to 64 logits a thread at once and leave few candidates.
+int per_thread(int64_t rows, int vocab) {
+    int e = 8;
+    while (e < 64 && rows * ((vocab + 2 * e * kThreads - 1) / (2 * e * kThreads)) >= 512) e *= 2;
+    return e;
+}
+
+struct SelectPlan {
+    int e, chunks;
+    size_t cands, bytes;
+};
+
+SelectPlan select_plan(int sentences, int beams, int vocab) {
+    SelectPlan p{};
+    const int64_t rows = static_cast<int64_t>(sentences) * beams;
+    p.e = per_thread(rows, vocab);
+    p.chunks = (vocab + p.e * kThreads - 1) / (p.e * kThreads);
+    p.cands = static_cast<size_t>(rows) * p.chunks * kWaves * sizeof(Sum);
+    p.bytes = p.cands + static_cast<size_t>(rows) * p.chunks * beams * sizeof(Candidate);
+    return p;
+}
+
+int check_select(int dtype, int sentences, int beams, int vocab) {
+    if (dtype != QMM_DTYPE_F32 && dtype != QMM_DTYPE_F16 && dtype != QMM_DTYPE_BF16) return bad("logits must be F32, F16 or BF16.");
+    if (sentences < 0 || vocab <= 0) return bad("sentences must be non-negative and vocab positive.");
+    if (beams <= 0 || beams > kMaxBeams) return bad("beams must be between 1 and 64.");
+    if (vocab > (1 << 30) || static_cast<int64_t>(sentences) * beams > 65535) return bad("vocab must be at most 2^30 and sentences * beams at most 65535.");
+    return QMM_OK;
+}
+
+int select(const void* logits, int dtype, int64_t sentence_stride, int64_t beam_stride, const float* scores, int sentences, int beams,
+           int vocab, float* out_scores, int32_t* out_parents, int32_t* out_tokens, void* workspace, size_t workspace_bytes,
+           hipStream_t stream) {
+    const int rc = check_select(dtype, sentences, beams, vocab);
+    if (rc != QMM_OK) return rc;
+    if (sentences == 0) return QMM_OK;
+    if (!logits || !scores || !out_scores || !out_parents || !out_tokens) return bad("logits, scores and the outputs must be non-null.");
+    if (reinterpret_cast<uintptr_t>(logits) % elem_bytes(dtype) != 0) return bad("logits must be aligned to their elements.");
+    const SelectPlan p = select_plan(sentences, beams, vocab);
+    std::unique_lock<std::mutex> held;
+    if (workspace) {
+        if (workspace_bytes < p.bytes || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+            return bad("the workspace must be 16-byte aligned and hold qmm_beam_select_workspace() bytes.");
+    } else {
+        const hipError_t e = take_workspace(WorkspaceKind::kAttention, stream, p.bytes, held, &workspace);
+        if (e != hipSuccess) return launched(e, "beam select workspace");
+    }
+    Sum* sums = static_cast<Sum*>(workspace);
+    Candidate* cands = reinterpret_cast<Candidate*>(static_cast<char*>(workspace) + p.cands);
+    const dim3 grid(static_cast<unsigned>(p.chunks), static_cast<unsigned>(sentences * beams));
+    auto go = [&](auto tc, auto ec) {
+        using T = decltype(tc);
+        hipLaunchKernelGGL((select_chunk_kernel<T, decltype(ec)::value>), grid, dim3(kThreads), 0, stream, static_cast<const T*>(logits),
+                           sentence_stride, beam_stride, scores, beams, vocab, sums, cands);
+    };
+    auto pick = [&](auto tc) {
+        switch (p.e) {
+            case 8: go(tc, std::integral_constant<int, 8>{}); break;
+            case 16: go(tc, std::integral_constant<int, 16>{}); break;
+            case 32: go(tc, std::integral_constant<int, 32>{}); break;
+            default: go(tc, std::integral_constant<int, 64>{}); break;
+        }
+    };
+    if (dtype == QMM_DTYPE_F32) pick(float{});
+    else if (dtype == QMM_DTYPE_F16) pick(_Float16{});
+    else pick(__bf16{});
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return launched(e, "beam select kernel launch");
+    hipLaunchKernelGGL(select_merge_kernel, dim3(static_cast<unsigned>(sentences)), dim3(kMergeThreads), 0, stream, scores, sums, cands,
+                       beams, p.chunks, out_scores, out_parents, out_tokens);
+    return launched(hipGetLastError(), "beam select merge kernel launch");
+}
+
+}  // namespace
+}  // namespace paged
+}  // namespace qmm
+
+extern "C" {
+
+size_t qmm_beam_select_workspace(int dtype, int sentences, int beams, int vocab) {
+    if (qmm::paged::entry([&] { return qmm::paged::check_select(dtype, sentences, beams, vocab); }) != QMM_OK) return 0;
+    return qmm::paged::select_plan(sentences, beams, vocab).bytes;
+}
+
+int qmm_beam_select(const void* logits, int dtype, int64_t sentence_stride, int64_t beam_stride, const float* scores, int sentences,
+                    int beams, int vocab, float* out_scores, int32_t* out_parents, int32_t* out_tokens, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+    return qmm::paged::entry([&] {
+        return qmm::paged::select(logits, dtype, sentence_stride, beam_stride, scores, sentences, beams, vocab, out_scores, out_parents,
+                                  out_tokens, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+    });
+}
+
+}  // extern "C"

@@ -44,6 +44,7 @@ QMM_ERR_OUT_OF_RANGE = 5
 DTYPE_F32 = 0
 DTYPE_F16 = 1
 DTYPE_BF16 = 2
+DTYPE_E4M3 = 3  # paged caches only
 
 if not os.path.exists(LIB_PATH):
     raise ImportError(
@@ -94,6 +95,34 @@ class GemmDesc(ctypes.Structure):
     _fields_ = [("ggml_type", _i), ("A", _vp), ("a_dtype", _i), ("W", _vp), ("C", _vp), ("c_dtype", _i),
                 ("M", _i), ("N", _i), ("K", _i), ("ev_before", _vp), ("ev_after", _vp)]
 
+
+class PagedKV(ctypes.Structure):
+    """Mirror of qmm_paged_kv (include/qmm.h)."""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("table", _vp), ("cu", _vp), ("ctx", _vp), ("table_stride", _i64),
+                ("k_layer", _i64), ("k_page", _i64), ("k_head", _i64), ("k_slot", _i64),
+                ("v_layer", _i64), ("v_page", _i64), ("v_head", _i64), ("v_slot", _i64),
+                ("table_width", _i), ("batch", _i), ("dtype", _i), ("num_layers", _i), ("num_pages", _i), ("kv_heads", _i),
+                ("page_size", _i), ("head_dim", _i), ("k_scale", ctypes.c_float), ("v_scale", ctypes.c_float)]
+
+
+class PagedNew(ctypes.Structure):
+    """Mirror of qmm_paged_new (include/qmm.h)."""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("q", _vp), ("q_out", _vp), ("positions", _vp),
+                ("k_token", _i64), ("k_head", _i64), ("v_token", _i64), ("v_head", _i64),
+                ("q_token", _i64), ("q_head", _i64), ("qo_token", _i64), ("qo_head", _i64),
+                ("tokens", _i), ("heads", _i), ("dtype", _i), ("rotary_dim", _i), ("neox", _i), ("freq_base", ctypes.c_float)]
+
+
+class PagedQuery(ctypes.Structure):
+    """Mirror of qmm_paged_query (include/qmm.h)."""
+
+    _fields_ = [("q", _vp), ("out", _vp), ("mask", _vp), ("q_token", _i64), ("q_head", _i64), ("out_token", _i64),
+                ("out_head", _i64), ("mask_stride", _i64), ("tokens", _i), ("max_new", _i), ("heads", _i), ("dtype", _i),
+                ("mask_words", _i), ("scale", ctypes.c_float)]
+
+
 _SIGNATURES = {
     "qmm_last_error": (ctypes.c_char_p, []),
     "qmm_version": (_i, []),
@@ -121,6 +150,13 @@ _SIGNATURES = {
     "qmm_kv_cache_init": (_i, [_i, _i, _i, _i]),
     "qmm_kv_cache_free": (_i, []),
     "qmm_gqa_attention_cached": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, ctypes.c_float, _i, _vp]),
+    "qmm_paged_append": (_i, [_vp, _vp, _vp]),
+    "qmm_paged_attention_workspace": (ctypes.c_size_t, [_vp, _vp]),
+    "qmm_paged_tree_attention": (_i, [_vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "qmm_paged_commit_path": (_i, [_vp, _vp, _i64, _i, _vp, _vp]),
+    "qmm_beam_select_workspace": (ctypes.c_size_t, [_i, _i, _i, _i]),
+    "qmm_beam_select": (_i, [_vp, _i, _i64, _i64, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "qmm_beam_reorder": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp]),
     "qmm_forward_layer": (_i, [ctypes.POINTER(LayerConfig), ctypes.POINTER(LayerWeights), _vp, _vp, _i, _i, _i, _vp]),
     "qmm_matmul_fp16_nt_device": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp]),
     "qmm_matmul_fp16_nt_host": (_i, [_vp, _vp, _vp, _i, _i, _i]),

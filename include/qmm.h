@@ -45,7 +45,8 @@ enum qmm_ggml_type {
 enum qmm_dtype {
     QMM_DTYPE_F32 = 0,
     QMM_DTYPE_F16 = 1,
-    QMM_DTYPE_BF16 = 2
+    QMM_DTYPE_BF16 = 2,
+    QMM_DTYPE_E4M3 = 3 /* OCP float8 e4m3fn: paged caches only */
 };
 
 /* Thread-local message of the last failed call on this thread ("" if none). */
@@ -339,6 +340,105 @@ int qmm_gqa_attention_cached_host(const void* h_Q, const void* h_K_new, const vo
  * (src/kernels/attention.hip:603-695). */
 int qmm_forward_layer_host(const qmm_layer_config* cfg, const qmm_layer_weights* w, const void* h_x_in, void* h_x_out,
                            int layer_idx, int seq_len, int pos_offset);
+
+/* ---------------------------------------------------------------------------------
+ * Paged key/value cache: batches of sequences, drafted trees, beam search (device pointers,
+ * asynchronous on `stream`).  No counterpart in the reference, whose cache is one sequence's
+ * contiguous fp16 pool.
+ *
+ * A cache is K and V of [num_pages][kv_heads][page_size][head_dim] (head_dim contiguous, the other
+ * strides given in elements; num_layers of them layer_stride apart for the calls that touch every
+ * layer), page_size a power of two.  Row i of sequence b is slot i % page_size of page
+ * table[b][i / page_size].  Sequence b holds ctx[b] rows and has the new tokens
+ * cu[b] .. cu[b + 1] - 1 of the call's `tokens` (concatenated; a sequence may have none); they
+ * take the rows ctx[b], ctx[b] + 1, ...  table, cu and ctx are read on the device: a row whose page is
+ * outside the table or the pool is not written, copied or seen.
+ * --------------------------------------------------------------------------------- */
+typedef struct qmm_paged_kv {
+    void* k;
+    void* v;
+    const int32_t* table; /* [batch][table_width], rows table_stride apart */
+    const int32_t* cu;    /* [batch + 1]; not read by qmm_beam_reorder */
+    const int32_t* ctx;   /* [batch] */
+    int64_t table_stride;
+    int64_t k_layer, k_page, k_head, k_slot; /* strides in elements */
+    int64_t v_layer, v_page, v_head, v_slot;
+    int32_t table_width, batch;
+    int32_t dtype; /* QMM_DTYPE_F16, QMM_DTYPE_BF16, or QMM_DTYPE_E4M3 */
+    int32_t num_layers, num_pages, kv_heads, page_size, head_dim;
+    float k_scale, v_scale; /* E4M3: stored value * scale = value; 1 for the other types */
+} qmm_paged_kv;
+
+/* New tokens: k / v [tokens][kv_heads][head_dim], q / q_out [tokens][heads][head_dim] (strides of
+ * token and head in elements; q NULL: none; q_out may be q).  dtype F16 or BF16; the cache is of the same
+ * type or E4M3.  q and k are rotated over their first rotary_dim dimensions (0: not at all; even,
+ * at most 256) by the angle pos * freq_base^(-2 i / rotary_dim), pairs (2i, 2i + 1), or
+ * (i, i + rotary_dim / 2) when neox != 0; pos = positions[token], or the token's cache row when
+ * positions is NULL.  Angles are reduced in 64-bit fixed point, so that far positions keep their digits. */
+typedef struct qmm_paged_new {
+    const void* k;
+    const void* v;
+    const void* q;
+    void* q_out;
+    const int32_t* positions;
+    int64_t k_token, k_head, v_token, v_head, q_token, q_head, qo_token, qo_head;
+    int32_t tokens, heads, dtype, rotary_dim, neox;
+    float freq_base;
+} qmm_paged_new;
+
+/* Writes the new tokens' rotated keys and their values into the cache's pages and the rotated
+ * queries into q_out, one rounding per stored value (E4M3: of value / scale, saturated at 448).  Two
+ * tokens of one call must not share a cache row. */
+int qmm_paged_append(const qmm_paged_kv* kv, const qmm_paged_new* in, void* stream);
+
+/* Queries q [tokens][heads][head_dim] of the new tokens, out alike (16-bit float, the cache's type
+ * unless that is E4M3).  New token i of a sequence sees its ctx cached rows and, of the sequence's
+ * new rows j, those whose bit j % 32 of mask[token][j / 32] is set (words past mask_words: not
+ * seen), or j <= i when mask is NULL.  scale 0 means 1 / sqrt(head_dim).  No sequence has more than
+ * max_new new tokens (tokens past that are not computed). */
+typedef struct qmm_paged_query {
+    const void* q;
+    void* out;
+    const int32_t* mask;
+    int64_t q_token, q_head, out_token, out_head, mask_stride;
+    int32_t tokens, max_new, heads, dtype, mask_words;
+    float scale;
+} qmm_paged_query;
+
+/* out = softmax(scale q k^T) v over the rows that each token sees (fp32 softmax; a token that sees
+ * none gets 0; a row that it does not see has no effect, whatever it holds).  head_dim a
+ * multiple of 8 up to 256.  A call whose rows are split over workgroups needs `workspace`, device
+ * memory of qmm_paged_attention_workspace() bytes, 16-byte aligned; with NULL it uses the per-(device,
+ * stream) scratch of qmm_gqa_attention, under the same rules for capture. */
+size_t qmm_paged_attention_workspace(const qmm_paged_kv* kv, const qmm_paged_query* in);
+int qmm_paged_tree_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, void* workspace, size_t workspace_bytes,
+                             void* stream);
+
+/* After a drafted tree was verified: row ctx[b] + j of sequence b becomes its row ctx[b] + path[b][j],
+ * in every layer, for each entry of path ([batch][path_len], rows path_stride apart; entries outside
+ * the sequence's new tokens, -1 among them, are skipped), and lens[b] = ctx[b] + the entries taken.
+ * A path ascends, as the nodes of a tree do whose parents come first. */
+int qmm_paged_commit_path(const qmm_paged_kv* kv, const int32_t* path, int64_t path_stride, int path_len, int32_t* lens,
+                          void* stream);
+
+/* One step of beam search over logits [sentences][beams][vocab] (F32, F16 or BF16; strides in
+ * elements, vocab contiguous): the `beams` best totals scores[s][w] + log_softmax(logits[s][w]) of each
+ * sentence in descending order, with their beams and tokens; equal totals go to the lower beam, then
+ * the lower token.  A beam whose total is not a number counts as -inf.  beams <= 64.  scores and the
+ * outputs are contiguous [sentences][beams].  `workspace`: qmm_beam_select_workspace() bytes, 16-byte
+ * aligned, or NULL as above. */
+size_t qmm_beam_select_workspace(int dtype, int sentences, int beams, int vocab);
+int qmm_beam_select(const void* logits, int dtype, int64_t sentence_stride, int64_t beam_stride, const float* scores,
+                    int sentences, int beams, int vocab, float* out_scores, int32_t* out_parents, int32_t* out_tokens,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* The sequences of kv (kv->batch = sentences * beams, kv->ctx their lengths, kv->cu not read) follow
+ * the chosen parents ([sentences][beams], within the sentence): sequence (s, w) gets the length of its
+ * parent, shares the parent's full pages, and owns page fresh[s][w], into which the rows of the parent's
+ * open page are copied in every layer.  table_out [batch][table_width] (contiguous; -1 past the
+ * open page) and lens_out [batch] are not the inputs; the fresh pages are in no table that is read. */
+int qmm_beam_reorder(const qmm_paged_kv* kv, const int32_t* parents, const int32_t* fresh, int beams, int32_t* table_out,
+                     int32_t* lens_out, void* stream);
 
 /* One byte range of a file and its destination. */
 typedef struct qmm_file_range {
