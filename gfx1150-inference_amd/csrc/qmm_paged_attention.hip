@@ -150,20 +150,15 @@ __device__ __forceinline__ RowState scan_row(const View& v, const AttnArgs& a, c
 
 __device__ __forceinline__ int lanes_per_key(int D) { return D <= 64 ? 8 : D <= 128 ? 16 : 32; }
 
-// Every head size and alignment: one wave per row and range.  Block (x, y, z): head, range, token.
-template <class T, class C>
-__global__ __launch_bounds__(kThreads) void attention_lanes_kernel(View v, AttnArgs a, int aligned) {
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int t = blockIdx.x, split = blockIdx.y, head = blockIdx.z * 4 + w;
-    const int seq = sequence_of(v, t, lane);
-    if (seq >= v.c.batch || t < v.c.cu[seq] || head >= a.in.heads) return;
-    const Span s = span_of(v, a, seq);
-    const int begin = split * a.kps;
-    if (begin >= s.total && split > 0) return;  // the first range of a sequence without rows writes zeros
-    const int lpk = lanes_per_key(v.c.head_dim);
-    const RowState r = scan_row<T, C>(v, a, s, t - s.first, head, begin, min(s.total, begin + a.kps), lane, lpk, aligned != 0);
+// A sequence whose rows fit one range writes its output at once; the others leave each range's state for the join.
+__device__ __forceinline__ bool one_range(const AttnArgs& a, const Span& s) { return s.total <= a.kps; }
+
+// Writes what scan_row left (lanes below D / 8 hold 8 dimensions each).
+template <class T>
+__device__ __forceinline__ void write_state(const View& v, const AttnArgs& a, const Span& s, int t, int head, int split, const RowState& r,
+                                            int lane) {
     const int d0 = 8 * lane;
-    if (a.splits == 1) {
+    if (one_range(a, s)) {
         if (d0 >= v.c.head_dim) return;
         T* out = static_cast<T*>(a.in.out) + static_cast<int64_t>(t) * a.in.out_token + head * a.in.out_head;
         const float inv = r.l == 0.0f ? 0.0f : a.v_scale / r.l;
@@ -178,6 +173,604 @@ __global__ __launch_bounds__(kThreads) void attention_lanes_kernel(View v, AttnA
     }
 }
 
+// Every head size and alignment: one wave per row and range.  Block (x, y, z): token, range, heads.
+template <class T, class C>
+__global__ __launch_bounds__(kThreads) void attention_lanes_kernel(View v, AttnArgs a, int aligned) {
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int t = blockIdx.x, split = blockIdx.y, head = blockIdx.z * 4 + w;
+    const int seq = sequence_of(v, t, lane);
+    if (seq >= v.c.batch || t < v.c.cu[seq] || head >= a.in.heads) return;
+    const Span s = span_of(v, a, seq);
+    const int begin = split * a.kps;
+    if (begin >= s.total && split > 0) return;  // the first range of a sequence without rows writes zeros
+    const int lpk = lanes_per_key(v.c.head_dim);
+    const RowState r = scan_row<T, C>(v, a, s, t - s.first, head, begin, min(s.total, begin + a.kps), lane, lpk, aligned != 0);
+    write_state<T>(v, a, s, t, head, split, r, lane);
+}
+
+// ---- matrix-core kernels: shared parts ---------------------------------------------------------
+// Both take head_dim 64, 96, 128 and 256, pages of 16 rows and more, and 16-byte aligned operands.  A
+// range's page ids are read into LDS once, so that no load of a row waits for a load of the table.
+constexpr int kMaxRangePages = 1024 + 1;
+constexpr int kMaxRange = 16 * 1024;
+// The running maximum that the weights are relative to moves only when a score passes it by 2^kSlack, so that most
+// blocks of keys rescale nothing; weights enter the second product as 2^(x - m + kShift), f16's range used from
+// 2^(kSlack + kShift) down.  Both cancel against the sum.
+constexpr float kSlack = 8.0f, kShift = 5.0f;
+
+template <class T>
+struct Frag;
+template <>
+struct Frag<_Float16> {
+    using v8 = f16x8;
+    static __device__ __forceinline__ f32x4 mma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x16 mma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ uint32_t from_fp8(uint32_t w) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+    }
+    static __device__ __forceinline__ uint32_t from_fp8_hi(uint32_t w) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true));
+    }
+};
+template <>
+struct Frag<__bf16> {
+    using v8 = bf16x8;
+    static __device__ __forceinline__ f32x4 mma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x16 mma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ uint32_t from_fp8(uint32_t w) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+    }
+    static __device__ __forceinline__ uint32_t from_fp8_hi(uint32_t w) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true));
+    }
+};
+
+// The keys k0 .. k0 + 31 that new token i of the sequence sees, as bits (pages apart).
+__device__ __forceinline__ uint32_t visible32(const AttnArgs& a, const Span& s, int i, int k0) {
+    const int c = s.ctx - k0, e = s.total - k0;  // cached keys, keys at all
+    auto low = [](int n) { return n >= 32 ? 0xFFFFFFFFu : n > 0 ? (1u << n) - 1u : 0u; };
+    uint32_t m = low(c);
+    if (c < 32) {
+        if (a.in.mask == nullptr) {
+            m |= low(c + i + 1);
+        } else {
+            const int j = max(-c, 0), word = j >> 5;  // new token of the first key that is none of the cached
+            const int32_t* row = a.in.mask + (s.first + i) * a.in.mask_stride;
+            const uint32_t w0 = word < a.in.mask_words ? row[word] : 0, w1 = word + 1 < a.in.mask_words ? row[word + 1] : 0;
+            const uint32_t bits = static_cast<uint32_t>(((static_cast<uint64_t>(w1) << 32) | w0) >> (j & 31));
+            m |= bits << max(c, 0);
+        }
+    }
+    return m & low(e);
+}
+
+// Page ids of the rows [begin, end) into LDS; true if one of them is missing.
+__device__ __forceinline__ bool stage_pages(const View& v, int seq, int begin, int end, int* pages) {
+    bool missing = false;
+    if (begin < end) {
+        const int p0 = begin >> v.page_shift, n = ((end - 1) >> v.page_shift) - p0 + 1;
+        for (int p = threadIdx.x; p < n; p += kThreads) {
+            const int id = page_of(v, seq, (p0 + p) << v.page_shift);
+            pages[p] = id;
+            missing |= id < 0;
+        }
+    }
+    return __syncthreads_or(missing);
+}
+
+// ---- few rows: keys straight into registers ------------------------------------------------------
+// Up to 64 rows (tokens x query heads of one kv head) against one kv head's keys: decoding, small trees.  Bound by
+// reading K and V from HBM, each once.  A wave takes 32 keys at a time, no LDS on the way, and every
+// row tile of 16 uses them:
+//   * S^T = K Q^T on 16x16x32: lane (l, q) = (lane % 16, lane / 16) loads key l's dims 8 q.. of every 32 (fp8: 16 bytes of
+//     every 64, the queries' dims in the same order) and receives the scores of row l with keys 4q .. 4q + 3 of
+//     each 16;
+//   * those 8 keys are the k order of the second product's operand, so the weights go straight from the score
+//     registers into O^T += V^T P^T; lane (l, q) loads dims D/16 l .. of its 8 keys' values (16 lanes read one
+//     row) and v_perm transposes them in registers.
+// With one row tile the weights enter as hi + lo in the operands' type, two products: 16 bits and more, where memory
+// hides them.  With more tiles the products are a good part of the time and the weights are rounded once, half a
+// step of each weight (as large as the output's own rounding, and of either sign).
+// The 4 waves take every fourth 32-key block of the range and are joined through LDS in wave order.
+// Block x: kv head fastest, then range, then sequence.
+template <class T, class C, int D, int NT>
+__global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attention_rows_kernel(View v, AttnArgs a) {
+    using F = Frag<T>;
+    using v8 = typename F::v8;
+    constexpr bool kFp8 = std::is_same_v<C, Fp8>;
+    constexpr int kF = D / 32, kVB = D / 16 * static_cast<int>(sizeof(C)), kVW = D / 32;  // fragments; bytes of a value slice; its dwords of T
+    constexpr int kVAlign = (kVB & -kVB) < 16 ? kVB & -kVB : 16;
+    constexpr bool kLo = NT == 1;
+    constexpr int kRowF = D + 4, kWaves = kThreads / 64;
+    __shared__ __align__(16) float so[kWaves][16 * kRowF];
+    __shared__ float2 sml[kWaves][16];
+    __shared__ int pages[kMaxRangePages];
+    const int kvh = v.c.kv_heads, group = a.in.heads / kvh;
+    const int g = static_cast<int>(blockIdx.x % kvh);
+    const int rest = static_cast<int>(blockIdx.x / kvh);
+    const int split = rest % a.splits, seq = rest / a.splits;
+    const Span s = span_of(v, a, seq);
+    const int begin = split * a.kps;
+    if (s.n == 0 || (begin >= s.total && split > 0)) return;
+    const int end = min(s.total, begin + a.kps), p0 = begin >> v.page_shift;
+    const int n_rows = min(s.n, a.in.max_new) * group;
+    const int lane = threadIdx.x & 63, l = lane & 15, q = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    stage_pages(v, seq, begin, end, pages);
+
+    // queries: rows past the last repeat it
+    v8 qf[NT][kF];
+    int tok[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int r = min(16 * nt + l, n_rows - 1);
+        tok[nt] = r / group;
+        const T* qrow = static_cast<const T*>(a.in.q) + static_cast<int64_t>(s.first + tok[nt]) * a.in.q_token + (g * group + r % group) * a.in.q_head;
+#pragma unroll
+        for (int f = 0; f < kF; ++f) {
+            const int d = kFp8 && (f | 1) < kF ? 64 * (f >> 1) + 16 * q + 8 * (f & 1) : 32 * f + 8 * q;
+            __builtin_memcpy(&qf[nt][f], __builtin_assume_aligned(qrow + d, 16), 16);
+        }
+    }
+    f32x4 o[NT][D / 16];
+    float m_run[NT], l_run[NT];  // l_run: of this lane's keys
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        m_run[nt] = -INFINITY;
+        l_run[nt] = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) o[nt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    const C* kbase = static_cast<const C*>(v.c.k) + g * v.c.k_head;
+    const C* vbase = static_cast<const C*>(v.c.v) + g * v.c.v_head;
+    for (int kb = begin + 32 * w; kb < end; kb += 32 * kWaves) {
+        u32x4 kr[2][kFp8 ? (kF + 1) / 2 : kF];
+        uint8_t vr[8][kVB] __attribute__((aligned(4)));
+        bool ok[2];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+            // 16 keys share a page; rows of the page past the sequence's end are read and masked
+            const int k0 = kb + 16 * tt;
+            const int id = k0 < end ? __builtin_amdgcn_readfirstlane(pages[(k0 >> v.page_shift) - p0]) : -1;
+            ok[tt] = id >= 0;
+            const int64_t page = max(id, 0);
+            const int slot = k0 & (v.c.page_size - 1);
+            const C* kp = kbase + page * v.c.k_page + (slot + l) * v.c.k_slot;
+            if constexpr (kFp8) {
+#pragma unroll
+                for (int f = 0; f < kF / 2; ++f) kr[tt][f] = *reinterpret_cast<const u32x4*>(kp + 64 * f + 16 * q);
+                if constexpr (kF % 2) {
+                    const u32x2 x = *reinterpret_cast<const u32x2*>(kp + 32 * (kF - 1) + 8 * q);
+                    kr[tt][kF / 2] = u32x4{x[0], x[1], 0, 0};
+                }
+            } else {
+#pragma unroll
+                for (int f = 0; f < kF; ++f) kr[tt][f] = *reinterpret_cast<const u32x4*>(kp + 32 * f + 8 * q);
+            }
+            const C* vp = vbase + page * v.c.v_page + (slot + 4 * q) * v.c.v_slot + D / 16 * l;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) __builtin_memcpy(vr[4 * tt + j], __builtin_assume_aligned(vp + j * v.c.v_slot, kVAlign), kVB);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // every load of the block is out before its first product
+        const bool full = kb + 32 <= s.ctx && kb + 32 <= end && ok[0] && ok[1];
+        v8 kf[2][kF];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int f = 0; f < kF; ++f) {
+                if constexpr (kFp8) {
+                    const uint32_t x = kr[tt][f >> 1][2 * (f & 1)], y = kr[tt][f >> 1][2 * (f & 1) + 1];
+                    const u32x4 t = {F::from_fp8(x), F::from_fp8_hi(x), F::from_fp8(y), F::from_fp8_hi(y)};
+                    kf[tt][f] = __builtin_bit_cast(v8, t);
+                } else {
+                    kf[tt][f] = __builtin_bit_cast(v8, kr[tt][f]);
+                }
+            }
+        v8 ph[NT], pl[kLo ? NT : 1];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float x[8];
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) {
+                f32x4 sc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int f = 0; f < kF; ++f) sc = F::mma16(kf[tt][f], qf[nt][f], sc);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[4 * tt + i] = sc[i] * a.scale_log2;
+            }
+            if (!full) {
+                uint32_t vis = visible32(a, s, tok[nt], kb);
+                if (!ok[0]) vis &= 0xFFFF0000u;
+                if (!ok[1]) vis &= 0x0000FFFFu;
+                vis >>= 4 * q;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (!((vis >> (16 * (i >> 2) + (i & 3))) & 1)) x[i] = -INFINITY;
+            }
+            float mx = x[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
+            if (__ballot(mx > m_run[nt] + kSlack) != 0) {
+                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                const float mn = fmaxf(m_run[nt], mx);
+                const float f = m_run[nt] == mn ? 1.0f : __builtin_amdgcn_exp2f(m_run[nt] - mn);
+                l_run[nt] *= f;
+#pragma unroll
+                for (int dt = 0; dt < D / 16; ++dt) o[nt][dt] *= f;
+                m_run[nt] = mn;
+            }
+            const float base = m_run[nt] == -INFINITY ? 0.0f : m_run[nt] - kShift;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float p = __builtin_amdgcn_exp2f(x[i] - base);
+                l_run[nt] += p;
+                ph[nt][i] = static_cast<T>(p);
+                if constexpr (kLo) pl[nt][i] = static_cast<T>(p - static_cast<float>(ph[nt][i]));
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);  // and V's transposition waits for V alone
+        uint32_t vd[8][kVW];  // the value slices as pairs of T
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (kFp8) {
+#pragma unroll
+                for (int i = 0; i < kVW; ++i) {
+                    uint16_t h;
+                    __builtin_memcpy(&h, vr[j] + 2 * i, 2);
+                    vd[j][i] = F::from_fp8(h);
+                }
+            } else {
+                __builtin_memcpy(vd[j], vr[j], kVB);
+            }
+        }
+        if (!full) {  // rows that nobody sees may hold anything
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (!(ok[j >> 2] && kb + 16 * (j >> 2) + 4 * q + (j & 3) < s.total))
+#pragma unroll
+                    for (int i = 0; i < kVW; ++i) vd[j][i] = 0;
+        }
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) {  // operand row l is dim D/16 l + dt of the lane's 8 keys
+            u32x4 t;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                t[i] = __builtin_amdgcn_perm(vd[2 * i + 1][dt >> 1], vd[2 * i][dt >> 1], (dt & 1) ? 0x07060302u : 0x05040100u);
+            const v8 vf = __builtin_bit_cast(v8, t);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                o[nt][dt] = F::mma16(vf, ph[nt], o[nt][dt]);
+                if constexpr (kLo) o[nt][dt] = F::mma16(vf, pl[nt], o[nt][dt]);
+            }
+        }
+    }
+
+    // Lane (l, q) holds dims D/4 q + D/16 v + dt of row l in o[nt][dt][v].  A row tile at a time, 16 threads a row.
+    constexpr int kPer = D / 16;
+    const int mr = threadIdx.x >> 4, d0 = kPer * (threadIdx.x & 15);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        if (16 * nt >= n_rows) break;
+        float lr = l_run[nt];
+        lr += __shfl_xor(lr, 16, 64);
+        lr += __shfl_xor(lr, 32, 64);
+        if (nt > 0) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int dt = 0; dt < D / 16; dt += 2) {
+                float* at = &so[w][l * kRowF + D / 4 * q + D / 16 * i + dt];
+                at[0] = o[nt][dt][i];
+                at[1] = o[nt][dt + 1][i];
+            }
+        if (q == 0) sml[w][l] = float2{m_run[nt], lr};
+        __syncthreads();
+        const int r = 16 * nt + mr;
+        const bool live = r < n_rows;
+        float mm = -INFINITY, ls = 0.0f;
+        float acc[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) acc[j] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) mm = fmaxf(mm, sml[i][mr].x);
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+            const float2 ml = sml[i][mr];
+            if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // no key seen
+            const float f = ml.x == mm ? 1.0f : __builtin_amdgcn_exp2f(ml.x - mm);
+            ls += ml.y * f;
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) acc[j] += so[i][mr * kRowF + d0 + j] * f;
+        }
+        const int t = s.first + (live ? r / group : 0), head = g * group + (live ? r % group : 0);
+        // An infinite or NaN value makes the products NaN also in rows that do not see it, or with a weight that
+        // rounds to 0: such rows start over on the vector ALUs, unless their scores are NaN.
+        bool nan = false;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) nan |= acc[j] != acc[j];
+        const uint64_t bad = __ballot(nan && live && ls == ls);
+        const bool mine = (bad >> (lane & 48)) & 0xFFFFu;
+        if (live && !mine) {
+            if (one_range(a, s)) {
+                const float inv = ls == 0.0f ? 0.0f : a.v_scale / ls;
+                T h[kPer];
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) h[j] = static_cast<T>(acc[j] * inv);
+                T* out = static_cast<T*>(a.in.out) + static_cast<int64_t>(t) * a.in.out_token + head * a.in.out_head + d0;
+                __builtin_memcpy(__builtin_assume_aligned(out, kPer % 8 == 0 ? 16 : 4), h, sizeof(h));
+            } else {
+                // 2^-kShift off the sum and the output, so that they belong to the maximum
+                const int64_t at = (static_cast<int64_t>(split) * a.in.tokens + t) * a.in.heads + head;
+                float* po = a.part_o + at * D + d0;
+#pragma unroll
+                for (int j = 0; j < kPer; j += 2) *reinterpret_cast<f32x2*>(po + j) = f32x2{acc[j], acc[j + 1]};
+                if (d0 == 0) a.part_ml[at] = float2{mm - kShift, ls};
+            }
+        }
+        if (__builtin_expect(bad != 0, 0)) {
+#pragma unroll 1
+            for (int rr = 0; rr < 4; ++rr) {
+                if (!((bad >> (16 * rr)) & 0xFFFFu)) continue;
+                const int br = 16 * nt + 4 * w + rr;
+                const RowState st = scan_row<T, C>(v, a, s, br / group, g * group + br % group, begin, end, lane, lanes_per_key(D), true);
+                write_state<T>(v, a, s, s.first + br / group, g * group + br % group, split, st, lane);
+            }
+        }
+    }
+}
+
+// ---- many rows: keys through LDS -----------------------------------------------------------------
+// A workgroup of 4 waves owns 128 rows (tokens x query heads of one kv head), 32 a wave, and walks the keys in
+// tiles of 64, staged through LDS (two buffers, one barrier a tile) and taken 32 at a time:
+//   * S^T = K Q^T on 32x32x16, the wave's queries in registers: a lane holds one row (lane % 32) and 16 of the 32
+//     keys, the partner lane (lane ^ 32) the others;
+//   * the weights go from the S registers into O^T += V^T P^T without leaving the lane (the k order of each 16-key
+//     block is the order the lane holds its keys in); V is staged transposed ([dim][key]).  Weights are rounded to
+//     the operands' type once, half a step, of either sign;
+//   * the lanes keep sums of their own; maxima are exchanged only when the running one moves (kSlack).
+// Bound by the vector work of the weights, beside LDS reads and the products.
+// Block x: (kv head, range, sequence) x row tile, eight items side by side, so that an item's row tiles meet on
+// one XCD and its keys in one L2.
+constexpr int kTileRows = 128, kTileKeys = 64;
+
+template <int D>
+struct TileGeom {
+    static constexpr int kRowK = D + 8;           // elements per staged key row (16-byte pad)
+    static constexpr int kRowV = kTileKeys + 4;   // elements per staged V^T row (8-byte pad)
+    static constexpr int kK = kTileKeys * kRowK, kV = D * kRowV, kBuf = kK + kV;
+    static constexpr size_t kLds = 2 * static_cast<size_t>(kBuf) * 2;
+    static constexpr int kChunks = D / 8;
+    static constexpr int kKUnits = kTileKeys * kChunks / kThreads;
+    static constexpr int kVAll = kTileKeys / 2 * kChunks, kVUnits = (kVAll + kThreads - 1) / kThreads;
+};
+
+extern __shared__ __align__(16) uint16_t tile_lds[];
+
+template <class T, class C, int D>
+__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_tile_kernel(View v, AttnArgs a, int tiles, int items) {
+    using F = Frag<T>;
+    using v8 = typename F::v8;
+    using G = TileGeom<D>;
+    constexpr bool kFp8 = std::is_same_v<C, Fp8>;
+    using Raw = std::conditional_t<kFp8, u32x2, u32x4>;  // 8 elements of the cache
+    __shared__ int pages[kMaxRangePages];
+    const int kvh = v.c.kv_heads, group = a.in.heads / kvh;
+    const int tile = static_cast<int>(blockIdx.x / 8) % tiles;
+    const int item = static_cast<int>(blockIdx.x / 8) / tiles * 8 + static_cast<int>(blockIdx.x % 8);
+    if (item >= items) return;
+    const int g = item % kvh, split = item / kvh % a.splits, seq = item / kvh / a.splits;
+    const Span s = span_of(v, a, seq);
+    const int n_rows = min(s.n, a.in.max_new) * group, r0 = tile * kTileRows;
+    const int begin = split * a.kps;
+    if (r0 >= n_rows || (begin >= s.total && split > 0)) return;
+    const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = r0 + 32 * w + l32;
+    const bool row_live = r < n_rows;
+    const int i = min(r, n_rows - 1) / group, head = g * group + min(r, n_rows - 1) % group, t_out = s.first + i;
+    const int last = (min(r0 + kTileRows, n_rows) - 1) / group;
+    const int n_keys = a.in.mask ? s.total : min(s.total, s.ctx + last + 1);
+    const int end = min(n_keys, begin + a.kps), p0 = begin >> v.page_shift;
+    const int64_t part = (static_cast<int64_t>(split) * a.in.tokens + t_out) * a.in.heads + head;
+    if (begin >= end && begin > 0) {  // keys of later rows only
+        if (row_live && h == 0) a.part_ml[part] = float2{-INFINITY, 0.0f};
+        return;
+    }
+    const bool missing = stage_pages(v, seq, begin, end, pages);
+
+    v8 qf[D / 16];
+    {
+        const T* qrow = static_cast<const T*>(a.in.q) + static_cast<int64_t>(t_out) * a.in.q_token + head * a.in.q_head + 8 * h;
+#pragma unroll
+        for (int db = 0; db < D / 16; ++db) __builtin_memcpy(&qf[db], __builtin_assume_aligned(qrow + 16 * db, 16), 16);
+    }
+    const C* kbase = static_cast<const C*>(v.c.k) + g * v.c.k_head;
+    const C* vbase = static_cast<const C*>(v.c.v) + g * v.c.v_head;
+    const int n_pages = begin < end ? ((end - 1) >> v.page_shift) - p0 + 1 : 0;
+    auto page_at = [&](int key) { return pages[min((key >> v.page_shift) - p0, n_pages - 1)]; };  // keys past the end: its page
+
+    Raw kr[G::kKUnits], vr[G::kVUnits][2];
+    auto load = [&](int kb) {
+#pragma unroll
+        for (int u = 0; u < G::kKUnits; ++u) {
+            const int x = tid + kThreads * u, key = kb + x / G::kChunks, c = x % G::kChunks;
+            const int64_t page = max(page_at(key), 0);
+            kr[u] = *reinterpret_cast<const Raw*>(kbase + page * v.c.k_page + (key & (v.c.page_size - 1)) * v.c.k_slot + 8 * c);
+        }
+#pragma unroll
+        for (int u = 0; u < G::kVUnits; ++u) {
+            const int x = tid + kThreads * u, key = kb + 2 * (x % (kTileKeys / 2)), c = x / (kTileKeys / 2);
+            if (G::kVAll % kThreads == 0 || x < G::kVAll) {
+                const int64_t page = max(page_at(key), 0);  // a pair shares a page
+                const C* p = vbase + page * v.c.v_page + (key & (v.c.page_size - 1)) * v.c.v_slot + 8 * c;
+                vr[u][0] = *reinterpret_cast<const Raw*>(p);
+                vr[u][1] = *reinterpret_cast<const Raw*>(p + v.c.v_slot);
+            }
+        }
+    };
+    auto wide = [](Raw x) {
+        if constexpr (kFp8) return u32x4{F::from_fp8(x[0]), F::from_fp8_hi(x[0]), F::from_fp8(x[1]), F::from_fp8_hi(x[1])};
+        else return x;
+    };
+    auto store = [&](int kb, int buf) {
+        uint16_t* sk = tile_lds + buf * G::kBuf;
+        uint16_t* sv = sk + G::kK;
+#pragma unroll
+        for (int u = 0; u < G::kKUnits; ++u) {
+            const int x = tid + kThreads * u, key = x / G::kChunks, c = x % G::kChunks;
+            *reinterpret_cast<u32x4*>(sk + key * G::kRowK + 8 * c) = wide(kr[u]);
+        }
+        const bool whole = kb + kTileKeys <= s.total && !missing;
+#pragma unroll
+        for (int u = 0; u < G::kVUnits; ++u) {
+            const int x = tid + kThreads * u, kp = x % (kTileKeys / 2), c = x / (kTileKeys / 2);
+            if (G::kVAll % kThreads == 0 || x < G::kVAll) {
+                u32x4 lo = wide(vr[u][0]), hi = wide(vr[u][1]);
+                if (!whole) {  // rows that nobody sees may hold anything
+                    const int key = kb + 2 * kp;
+                    const bool ok = page_at(key) >= 0;
+                    if (!ok || key >= s.total) lo = u32x4{0, 0, 0, 0};
+                    if (!ok || key + 1 >= s.total) hi = u32x4{0, 0, 0, 0};
+                }
+                uint32_t* col = reinterpret_cast<uint32_t*>(sv + 8 * c * G::kRowV + 2 * kp);
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    col[(2 * m) * (G::kRowV / 2)] = __builtin_amdgcn_perm(hi[m], lo[m], 0x05040100u);
+                    col[(2 * m + 1) * (G::kRowV / 2)] = __builtin_amdgcn_perm(hi[m], lo[m], 0x07060302u);
+                }
+            }
+        }
+    };
+
+    f32x16 o[D / 32];
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
+    float m_run = -INFINITY, l_run = 0.0f;
+    const bool live = r0 + 32 * w < n_rows;  // waves without rows only stage
+    if (begin < end) {
+        load(begin);
+        store(begin, 0);
+    }
+    __syncthreads();
+    for (int kb = begin, buf = 0; kb < end; kb += kTileKeys, buf ^= 1) {
+        const bool more = kb + kTileKeys < end;
+        if (more) load(kb + kTileKeys);
+        if (live) {
+            const uint16_t* sk = tile_lds + buf * G::kBuf;
+            const uint16_t* sv = sk + G::kK;
+            const bool full = kb + kTileKeys <= s.ctx && kb + kTileKeys <= end && !missing;
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+                // register e is key 32 hh + 8 (e / 4) + 4 h + e % 4 of row l32
+                f32x16 x;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = 0.0f;
+#pragma unroll
+                for (int db = 0; db < D / 16; ++db) {
+                    v8 kf;
+                    __builtin_memcpy(&kf, __builtin_assume_aligned(sk + (32 * hh + l32) * G::kRowK + 16 * db + 8 * h, 16), 16);
+                    x = F::mma32(kf, qf[db], x);
+                }
+                if (a.scale_log2 < 0.0f) {  // the maximum below is of raw scores
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[e] = -x[e];
+                }
+                if (!full) {
+                    uint32_t vis = visible32(a, s, i, kb + 32 * hh);
+                    if (missing) {
+                        if (page_at(kb + 32 * hh) < 0) vis &= 0xFFFF0000u;
+                        if (page_at(kb + 32 * hh + 16) < 0) vis &= 0x0000FFFFu;
+                    }
+                    vis >>= 4 * h;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (!((vis >> (8 * (e >> 2) + (e & 3))) & 1)) x[e] = -INFINITY;
+                }
+                const float scale = fabsf(a.scale_log2);
+                float mx = x[0];
+#pragma unroll
+                for (int e = 1; e < 16; ++e) mx = fmaxf(mx, x[e]);
+                mx *= scale;
+                if (__ballot(mx > m_run + kSlack) != 0) {
+                    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                    const float mn = fmaxf(m_run, mx);
+                    const float f = m_run == mn ? 1.0f : __builtin_amdgcn_exp2f(m_run - mn);
+                    l_run *= f;
+#pragma unroll
+                    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[dt][e] *= f;
+                    m_run = mn;
+                }
+                const float base = m_run == -INFINITY ? 0.0f : m_run - kShift;
+                v8 pf[2];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float p = __builtin_amdgcn_exp2f(__fmaf_rn(x[e], scale, -base));
+                    l_run += p;
+                    pf[e >> 3][e & 7] = static_cast<T>(p);
+                }
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int dt = 0; dt < D / 32; ++dt) {
+                        const uint16_t* vrow = sv + (32 * dt + l32) * G::kRowV + 32 * hh + 16 * b + 4 * h;
+                        u32x2 f0, f1;
+                        __builtin_memcpy(&f0, __builtin_assume_aligned(vrow, 8), 8);
+                        __builtin_memcpy(&f1, __builtin_assume_aligned(vrow + 8, 8), 8);
+                        const u32x4 vf = {f0[0], f0[1], f1[0], f1[1]};
+                        o[dt] = F::mma32(__builtin_bit_cast(v8, vf), pf[b], o[dt]);
+                    }
+            }
+        }
+        if (more) store(kb + kTileKeys, buf ^ 1);
+        __syncthreads();
+    }
+    if (!live) return;
+    l_run += __shfl_xor(l_run, 32, 64);
+    bool nan = false;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) nan |= o[dt][e] != o[dt][e];
+    uint64_t bad = __ballot(nan && row_live && l_run == l_run);  // as in attention_rows_kernel
+    bad |= bad >> 32;
+    if (row_live && !((bad >> l32) & 1)) {
+        if (one_range(a, s)) {
+            const float inv = l_run == 0.0f ? 0.0f : a.v_scale / l_run;
+            T* out = static_cast<T*>(a.in.out) + static_cast<int64_t>(t_out) * a.in.out_token + head * a.in.out_head + 4 * h;
+#pragma unroll
+            for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4) {
+                    T v4[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v4[e] = static_cast<T>(o[dt][4 * q4 + e] * inv);
+                    __builtin_memcpy(__builtin_assume_aligned(out + 32 * dt + 8 * q4, 8), v4, 8);
+                }
+        } else {
+            float* po = a.part_o + part * D + 4 * h;
+#pragma unroll
+            for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4)
+                    *reinterpret_cast<f32x4*>(po + 32 * dt + 8 * q4) =
+                        f32x4{o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]};
+            if (h == 0) a.part_ml[part] = float2{m_run - kShift, l_run};
+        }
+    }
+    bad &= 0xFFFFFFFFu;
+    while (__builtin_expect(bad != 0, 0)) {
+        const int br = r0 + 32 * w + __builtin_ctzll(bad);
+        bad &= bad - 1;
+        const RowState st = scan_row<T, C>(v, a, s, br / group, g * group + br % group, begin, end, lane, lanes_per_key(D), true);
+        write_state<T>(v, a, s, s.first + br / group, g * group + br % group, split, st, lane);
+    }
+}
+
 // Joins the ranges of each row in their order: D / 4 threads a row, 4 ranges requested at once.
 // Block (x, y): token, heads.
 template <class T>
@@ -186,9 +779,10 @@ __global__ __launch_bounds__(kThreads) void attention_merge_kernel(View v, AttnA
     const int seq = sequence_of(v, t, threadIdx.x & 63);
     if (seq >= v.c.batch || t < v.c.cu[seq]) return;
     const Span s = span_of(v, a, seq);
+    if (one_range(a, s)) return;  // written by the range itself
     const int slot = threadIdx.x / per, d0 = 4 * (threadIdx.x % per), head = blockIdx.y * rows + slot;
     if (slot >= rows || head >= a.in.heads) return;
-    const int n = max((s.total + a.kps - 1) / a.kps, 1);
+    const int n = (s.total + a.kps - 1) / a.kps;
     const int64_t row = static_cast<int64_t>(t) * a.in.heads + head, step = static_cast<int64_t>(a.in.tokens) * a.in.heads;
     float m = -INFINITY, l = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -226,17 +820,45 @@ __global__ __launch_bounds__(kThreads) void attention_merge_kernel(View v, AttnA
 }
 
 // ---- host side -------------------------------------------------------------------------------
+// Which kernel serves a call, by the rows (tokens x query heads) that share a kv head, and how its keys are cut.
+enum class Kind { kLanes, kRows, kTile };
 struct Plan {
+    Kind kind;
+    int row_tiles;  // of 16 rows (kRows), 128 (kTile)
     int splits, kps;
     size_t o_bytes, bytes;
 };
 
+bool matrix_operands(const View& v, const qmm_paged_query& in) {
+    const int D = v.c.head_dim;
+    if ((D != 64 && D != 96 && D != 128 && D != 256) || v.c.page_size < 16 || v.c.num_pages == 0) return false;
+    const uint64_t els = static_cast<uint64_t>(v.c.k_page | v.c.k_head | v.c.k_slot | v.c.v_page | v.c.v_head | v.c.v_slot);
+    const uint64_t rows = static_cast<uint64_t>(in.q_token | in.q_head | in.out_token | in.out_head);
+    const uint64_t ptr = reinterpret_cast<uintptr_t>(v.c.k) | reinterpret_cast<uintptr_t>(v.c.v) | reinterpret_cast<uintptr_t>(in.q) |
+                         reinterpret_cast<uintptr_t>(in.out);
+    return els % (v.c.dtype == QMM_DTYPE_E4M3 ? 16 : 8) == 0 && rows % 8 == 0 && ptr % 16 == 0;
+}
+
 Plan plan(const View& v, const qmm_paged_query& in) {
     Plan p{};
-    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(static_cast<int64_t>(v.c.table_width) * v.c.page_size, INT32_MAX - 4096));
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(static_cast<int64_t>(v.c.table_width) * v.c.page_size, INT32_MAX - 65536));
     const int64_t rows = static_cast<int64_t>(in.tokens) * in.heads;
-    int64_t kps = 64;
-    while (kps < most && (rows * ((most + kps - 1) / kps) > 16384 || (most + kps - 1) / kps > 1024)) kps *= 2;
+    const int64_t per_kv = static_cast<int64_t>(std::min(in.max_new, in.tokens)) * (in.heads / v.c.kv_heads);
+    int64_t kps;
+    if (!matrix_operands(v, in) || per_kv > (1 << 28)) {
+        p.kind = Kind::kLanes;
+        kps = 64;
+        while (kps < most && (rows * ((most + kps - 1) / kps) > 16384 || (most + kps - 1) / kps > 1024)) kps *= 2;
+    } else {
+        // more row tiles of head_dim 256 do not fit a wave's registers
+        p.kind = per_kv <= (v.c.head_dim <= 128 ? 64 : 16) ? Kind::kRows : Kind::kTile;
+        const int tile = p.kind == Kind::kRows ? 16 : kTileRows;
+        p.row_tiles = static_cast<int>((per_kv + tile - 1) / tile);
+        const int64_t groups = static_cast<int64_t>(v.c.batch) * v.c.kv_heads * (p.kind == Kind::kRows ? 1 : p.row_tiles);
+        const int64_t target = p.kind == Kind::kRows ? 4096 : 512;
+        kps = p.kind == Kind::kRows ? 128 : 256;
+        while (kps < most && kps < kMaxRange && groups * ((most + kps - 1) / kps) > target) kps *= 2;
+    }
     p.kps = static_cast<int>(kps);
     p.splits = static_cast<int>((most + kps - 1) / kps);
     if (p.splits > 1) {
@@ -268,6 +890,33 @@ bool operands_aligned(const View& v, const qmm_paged_query& in) {
     return els % 8 == 0 && ptr % (fp8 ? 8 : 16) == 0;
 }
 
+template <class T, class C, int D>
+int launch_matrix(const View& v, const AttnArgs& a, const Plan& p, hipStream_t stream) {
+    const int64_t items = static_cast<int64_t>(v.c.batch) * v.c.kv_heads * p.splits;
+    const int64_t blocks = p.kind == Kind::kRows ? items : (items + 7) / 8 * 8 * p.row_tiles;
+    if (blocks > INT32_MAX) return bad("too many sequences, heads and tokens for one call.");
+    const dim3 grid(static_cast<unsigned>(blocks));
+    if (p.kind == Kind::kRows) {
+        auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, stream, v, a); };
+        if constexpr (D <= 128) {
+            if (p.row_tiles == 2) go(attention_rows_kernel<T, C, D, 2>);
+            else if (p.row_tiles > 2) go(attention_rows_kernel<T, C, D, 4>);
+        }
+        if (p.row_tiles == 1) go(attention_rows_kernel<T, C, D, 1>);
+        return QMM_OK;
+    }
+    using G = TileGeom<D>;
+    static std::once_flag once;
+    static hipError_t attr = hipSuccess;
+    std::call_once(once, [] {
+        attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_tile_kernel<T, C, D>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                   static_cast<int>(G::kLds));
+    });
+    if (attr != hipSuccess) return launched(attr, "paged attention LDS size");
+    hipLaunchKernelGGL((attention_tile_kernel<T, C, D>), grid, dim3(kThreads), G::kLds, stream, v, a, p.row_tiles, static_cast<int>(items));
+    return QMM_OK;
+}
+
 int tree_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     View v;
     const int rc = check_query(kv, in, &v);
@@ -293,16 +942,26 @@ int tree_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, void* work
     a.kps = p.kps;
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + p.o_bytes);
-    const int aligned = operands_aligned(v, *in) ? 1 : 0;
-    const dim3 grid(static_cast<unsigned>(in->tokens), static_cast<unsigned>(p.splits), static_cast<unsigned>((in->heads + 3) / 4));
-    auto go = [&](auto tc, auto cc) {
+    const bool fp8 = v.c.dtype == QMM_DTYPE_E4M3;
+    int rc2 = QMM_OK;
+    auto typed = [&](auto tc, auto cc) {
         using T = decltype(tc);
         using C = decltype(cc);
-        hipLaunchKernelGGL((attention_lanes_kernel<T, C>), grid, dim3(kThreads), 0, stream, v, a, aligned);
+        if (p.kind == Kind::kLanes) {
+            const dim3 grid(static_cast<unsigned>(in->tokens), static_cast<unsigned>(p.splits), static_cast<unsigned>((in->heads + 3) / 4));
+            hipLaunchKernelGGL((attention_lanes_kernel<T, C>), grid, dim3(kThreads), 0, stream, v, a, operands_aligned(v, *in) ? 1 : 0);
+            return;
+        }
+        switch (v.c.head_dim) {
+            case 64: rc2 = launch_matrix<T, C, 64>(v, a, p, stream); break;
+            case 96: rc2 = launch_matrix<T, C, 96>(v, a, p, stream); break;
+            case 128: rc2 = launch_matrix<T, C, 128>(v, a, p, stream); break;
+            default: rc2 = launch_matrix<T, C, 256>(v, a, p, stream); break;
+        }
     };
-    const bool fp8 = v.c.dtype == QMM_DTYPE_E4M3;
-    if (in->dtype == QMM_DTYPE_F16) fp8 ? go(_Float16{}, Fp8{}) : go(_Float16{}, _Float16{});
-    else fp8 ? go(__bf16{}, Fp8{}) : go(__bf16{}, __bf16{});
+    if (in->dtype == QMM_DTYPE_F16) fp8 ? typed(_Float16{}, Fp8{}) : typed(_Float16{}, _Float16{});
+    else fp8 ? typed(__bf16{}, Fp8{}) : typed(__bf16{}, __bf16{});
+    if (rc2 != QMM_OK) return rc2;
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return launched(e, "paged attention kernel launch");
     if (p.splits > 1) {
