@@ -3,9 +3,10 @@
 // over the rows j that row r = (token, query head) sees: the sequence's cached rows, and those of its new
 // rows that a bit mask (a drafted tree) or the order (a chain) lets it see.
 //
-// The keys of a sequence are cut into ranges of `kps`, one workgroup each, where the rows alone leave the
-// chip idle; a range's maximum (base 2), sum and unnormalised output are joined by a second kernel in the
-// order of the ranges, so a result depends on the call's sizes alone.
+// The keys of a sequence are cut into ranges, one workgroup each, where the rows alone leave the chip idle; a
+// range's maximum (base 2), sum and unnormalised output are joined by a second kernel in the order of the ranges,
+// so a result depends on the call's lengths alone.  How long a range is, every workgroup works out from all
+// sequences' lengths, which only the device knows (plan_call): the host sees no more than the width of the table.
 #include "qmm_paged.h"
 
 #include <algorithm>
@@ -23,9 +24,10 @@ struct AttnArgs {
     qmm_paged_query in;
     float scale_log2;  // scale * k_scale * log2 e
     float v_scale;
-    int splits, kps;   // ranges of keys in the grid, keys per range
-    float* part_o;     // [split][token][head][D]
-    float2* part_ml;   // [split][token][head]: maximum, sum
+    int kps;           // keys per range of the kernel without a plan
+    int target;        // workgroups that a plan cuts the call into
+    float* part_o;     // [partial row][D]
+    float2* part_ml;   // [partial row]: maximum, sum
 };
 
 // The new tokens of one sequence.
@@ -150,26 +152,22 @@ __device__ __forceinline__ RowState scan_row(const View& v, const AttnArgs& a, c
 
 __device__ __forceinline__ int lanes_per_key(int D) { return D <= 64 ? 8 : D <= 128 ? 16 : 32; }
 
-// A sequence whose rows fit one range writes its output at once; the others leave each range's state for the join.
-__device__ __forceinline__ bool one_range(const AttnArgs& a, const Span& s) { return s.total <= a.kps; }
-
-// Writes what scan_row left (lanes below D / 8 hold 8 dimensions each).
+// Writes what scan_row left (lanes below D / 8 hold 8 dimensions each): the output where its range is the only one
+// (part < 0), else the partial row.
 template <class T>
-__device__ __forceinline__ void write_state(const View& v, const AttnArgs& a, const Span& s, int t, int head, int split, const RowState& r,
-                                            int lane) {
+__device__ __forceinline__ void write_state(const View& v, const AttnArgs& a, int t, int head, int64_t part, const RowState& r, int lane) {
     const int d0 = 8 * lane;
-    if (one_range(a, s)) {
+    if (part < 0) {
         if (d0 >= v.c.head_dim) return;
         T* out = static_cast<T*>(a.in.out) + static_cast<int64_t>(t) * a.in.out_token + head * a.in.out_head;
         const float inv = r.l == 0.0f ? 0.0f : a.v_scale / r.l;
 #pragma unroll
         for (int e = 0; e < 8; ++e) out[d0 + e] = static_cast<T>(r.l == 0.0f ? 0.0f : r.o[e] * inv);
     } else {
-        const int64_t at = (static_cast<int64_t>(split) * a.in.tokens + t) * a.in.heads + head;
-        if (lane == 0) a.part_ml[at] = float2{r.m, r.l};
+        if (lane == 0) a.part_ml[part] = float2{r.m, r.l};
         if (d0 < v.c.head_dim)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) a.part_o[at * v.c.head_dim + d0 + e] = r.o[e];
+            for (int e = 0; e < 8; ++e) a.part_o[part * v.c.head_dim + d0 + e] = r.o[e];
     }
 }
 
@@ -185,14 +183,14 @@ __global__ __launch_bounds__(kThreads) void attention_lanes_kernel(View v, AttnA
     if (begin >= s.total && split > 0) return;  // the first range of a sequence without rows writes zeros
     const int lpk = lanes_per_key(v.c.head_dim);
     const RowState r = scan_row<T, C>(v, a, s, t - s.first, head, begin, min(s.total, begin + a.kps), lane, lpk, aligned != 0);
-    write_state<T>(v, a, s, t, head, split, r, lane);
+    const int64_t part = s.total <= a.kps ? -1 : (static_cast<int64_t>(split) * a.in.tokens + t) * a.in.heads + head;
+    write_state<T>(v, a, t, head, part, r, lane);
 }
 
 // ---- matrix-core kernels: shared parts ---------------------------------------------------------
-// Both take head_dim 64, 96, 128 and 256, pages of 16 rows and more, and 16-byte aligned operands.  A
-// range's page ids are read into LDS once, so that no load of a row waits for a load of the table.
-constexpr int kMaxRangePages = 1024 + 1;
-constexpr int kMaxRange = 16 * 1024;
+// Both take head_dim 64, 96, 128 and 256, pages of 16 rows and more, and 16-byte aligned operands.  The page
+// ids of up to kWindow keys of a range are read into LDS together, so that no load of a row waits for one of the table.
+constexpr int kWindow = 8 * 1024, kWindowPages = kWindow / 16 + 1;
 // The running maximum that the weights are relative to moves only when a score passes it by 2^kSlack, so that most
 // blocks of keys rescale nothing; weights enter the second product as 2^(x - m + kShift), f16's range used from
 // 2^(kSlack + kShift) down.  Both cancel against the sum.
@@ -244,6 +242,91 @@ __device__ __forceinline__ uint32_t visible32(const AttnArgs& a, const Span& s, 
     return m & low(e);
 }
 
+// How a call is cut, from its sequences' lengths; the same in every wave of every workgroup.
+//   steps      64 keys of a 128-row tile, or 128 keys of the one tile of few rows, is a step; a chain's row tiles
+//              see fewer keys than the last one does, so their mean counts;
+//   kps        keys per range: the steps of the whole call over `target` workgroups, so that a long sequence is cut
+//              and a short one beside it is not, whatever the table's width;
+//   blocks     (sequence, range, row tile, kv head), kv head fastest, in the sequences' order;
+//   partials   the rows of sequences with more than one range, in the same order.
+template <int kTile, int kStep>
+struct CallPlan {
+    static constexpr int kMinSteps = kTile == 128 ? 4 : 1;
+    int kps, seq, block;   // block within the sequence
+    int rows, tiles, ranges;  // of the sequence: tokens with rows, row tiles
+    int64_t first_part;    // of the sequence, in tokens
+
+    struct Lane {
+        int rows, tiles, total;
+        int64_t steps;
+    };
+    static __device__ __forceinline__ Lane lane_of(const View& v, const AttnArgs& a, int b) {
+        Lane x{0, 0, 0, 0};
+        if (b < v.c.batch) {
+            const Span s = span_of(v, a, b);
+            const int group = a.in.heads / v.c.kv_heads;
+            x.rows = min(s.n, a.in.max_new);
+            x.tiles = kTile == 128 ? (x.rows * group + kTile - 1) / kTile : x.rows > 0;
+            x.total = s.total;
+            const int seen = a.in.mask ? s.total : min(s.total, s.ctx + (s.n + 1) / 2);
+            x.steps = static_cast<int64_t>(max((seen + kStep - 1) / kStep, 1)) * x.tiles;
+        }
+        return x;
+    }
+    __device__ __forceinline__ int ranges_of(const Lane& x) const { return x.rows > 0 ? max((x.total - 1) / kps + 1, 1) : 0; }
+
+    // Finds the sequence of workgroup `at` (kBlock) or the place of sequence `at`; false: none.
+    template <bool kBlock>
+    __device__ __forceinline__ bool find(const View& v, const AttnArgs& a, int at, int lane) {
+        const int kvh = v.c.kv_heads;
+        int64_t steps = 0;
+        Lane x{};
+        for (int b0 = 0; b0 < v.c.batch; b0 += 64) {
+            x = lane_of(v, a, b0 + lane);
+            int64_t t = x.steps;
+            for (int o = 1; o < 64 && o < v.c.batch; o <<= 1) t += __shfl_xor(t, o, 64);
+            steps += t;
+        }
+        // lanes past the batch hold 0, but the sums above meet only within the next power of two of it
+        steps = __shfl(steps, 0, 64);
+        const int64_t u = max((steps * kvh + a.target - 1) / a.target, static_cast<int64_t>(kMinSteps));
+        kps = static_cast<int>(min(u * kStep, static_cast<int64_t>(1) << 30));
+        int64_t blocks = 0, parts = 0;
+        for (int b0 = 0; b0 < v.c.batch; b0 += 64) {
+            if (v.c.batch > 64) x = lane_of(v, a, b0 + lane);
+            const int n = ranges_of(x);
+            const int64_t own_blocks = static_cast<int64_t>(n) * x.tiles * kvh, own_parts = n > 1 ? static_cast<int64_t>(n) * x.rows : 0;
+            int64_t sb = own_blocks, sp = own_parts;
+            for (int o = 1; o < 64 && o < v.c.batch; o <<= 1) {
+                const int64_t ub = __shfl_up(sb, o, 64), up = __shfl_up(sp, o, 64);
+                if (lane >= o) {
+                    sb += ub;
+                    sp += up;
+                }
+            }
+            const int here = min(v.c.batch - b0, 64);
+            int hit;
+            if constexpr (kBlock) hit = static_cast<int>(__popcll(__ballot(lane < here && blocks + sb <= at)));
+            else hit = at - b0;
+            if (hit >= 0 && hit < here) {
+                seq = b0 + hit;
+                rows = __shfl(x.rows, hit, 64);
+                tiles = __shfl(x.tiles, hit, 64);
+                ranges = __shfl(n, hit, 64);
+                block = static_cast<int>(at - (blocks + __shfl(sb - own_blocks, hit, 64)));
+                first_part = parts + __shfl(sp - own_parts, hit, 64);
+                return true;
+            }
+            blocks += __shfl(sb, here - 1, 64);
+            parts += __shfl(sp, here - 1, 64);
+        }
+        return false;
+    }
+    __device__ __forceinline__ int64_t part_of(const AttnArgs& a, int range, int i, int head) const {
+        return ranges == 1 ? -1 : (first_part + static_cast<int64_t>(range) * rows + i) * a.in.heads + head;
+    }
+};
+
 // Page ids of the rows [begin, end) into LDS; true if one of them is missing.
 __device__ __forceinline__ bool stage_pages(const View& v, int seq, int begin, int end, int* pages) {
     bool missing = false;
@@ -272,7 +355,8 @@ __device__ __forceinline__ bool stage_pages(const View& v, int seq, int begin, i
 // hides them.  With more tiles the products are a good part of the time and the weights are rounded once, half a
 // step of each weight (as large as the output's own rounding, and of either sign).
 // The 4 waves take every fourth 32-key block of the range and are joined through LDS in wave order.
-// Block x: kv head fastest, then range, then sequence.
+constexpr int kRowsStep = 128;
+
 template <class T, class C, int D, int NT>
 __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attention_rows_kernel(View v, AttnArgs a) {
     using F = Frag<T>;
@@ -284,19 +368,17 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
     constexpr int kRowF = D + 4, kWaves = kThreads / 64;
     __shared__ __align__(16) float so[kWaves][16 * kRowF];
     __shared__ float2 sml[kWaves][16];
-    __shared__ int pages[kMaxRangePages];
+    __shared__ int pages[kWindowPages];
     const int kvh = v.c.kv_heads, group = a.in.heads / kvh;
-    const int g = static_cast<int>(blockIdx.x % kvh);
-    const int rest = static_cast<int>(blockIdx.x / kvh);
-    const int split = rest % a.splits, seq = rest / a.splits;
-    const Span s = span_of(v, a, seq);
-    const int begin = split * a.kps;
-    if (s.n == 0 || (begin >= s.total && split > 0)) return;
-    const int end = min(s.total, begin + a.kps), p0 = begin >> v.page_shift;
-    const int n_rows = min(s.n, a.in.max_new) * group;
     const int lane = threadIdx.x & 63, l = lane & 15, q = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    stage_pages(v, seq, begin, end, pages);
+    CallPlan<16, kRowsStep> cp;
+    if (!cp.template find<true>(v, a, static_cast<int>(blockIdx.x), lane)) return;
+    const int g = __builtin_amdgcn_readfirstlane(cp.block % kvh), range = __builtin_amdgcn_readfirstlane(cp.block / kvh);
+    const Span s = span_of(v, a, __builtin_amdgcn_readfirstlane(cp.seq));
+    const int kps = __builtin_amdgcn_readfirstlane(cp.kps);
+    const int begin = range * kps, end = min(s.total, begin + kps);
+    const int n_rows = min(s.n, a.in.max_new) * group;
 
     // queries: rows past the last repeat it
     v8 qf[NT][kF];
@@ -323,7 +405,11 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
     }
     const C* kbase = static_cast<const C*>(v.c.k) + g * v.c.k_head;
     const C* vbase = static_cast<const C*>(v.c.v) + g * v.c.v_head;
-    for (int kb = begin + 32 * w; kb < end; kb += 32 * kWaves) {
+    for (int from = begin; from < end; from += kWindow) {
+    const int until = min(end, from + kWindow), p0 = from >> v.page_shift;
+    if (from > begin) __syncthreads();
+    stage_pages(v, s.seq, from, until, pages);
+    for (int kb = from + 32 * w; kb < until; kb += 32 * kWaves) {
         u32x4 kr[2][kFp8 ? (kF + 1) / 2 : kF];
         uint8_t vr[8][kVB] __attribute__((aligned(4)));
         bool ok[2];
@@ -445,6 +531,7 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
             }
         }
     }
+    }
 
     // Lane (l, q) holds dims D/4 q + D/16 v + dt of row l in o[nt][dt][v].  A row tile at a time, 16 threads a row.
     constexpr int kPer = D / 16;
@@ -484,6 +571,7 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
             for (int j = 0; j < kPer; ++j) acc[j] += so[i][mr * kRowF + d0 + j] * f;
         }
         const int t = s.first + (live ? r / group : 0), head = g * group + (live ? r % group : 0);
+        const int64_t part = cp.part_of(a, range, t - s.first, head);
         // An infinite or NaN value makes the products NaN also in rows that do not see it, or with a weight that
         // rounds to 0: such rows start over on the vector ALUs, unless their scores are NaN.
         bool nan = false;
@@ -492,7 +580,7 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
         const uint64_t bad = __ballot(nan && live && ls == ls);
         const bool mine = (bad >> (lane & 48)) & 0xFFFFu;
         if (live && !mine) {
-            if (one_range(a, s)) {
+            if (part < 0) {
                 const float inv = ls == 0.0f ? 0.0f : a.v_scale / ls;
                 T h[kPer];
 #pragma unroll
@@ -501,11 +589,10 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
                 __builtin_memcpy(__builtin_assume_aligned(out, kPer % 8 == 0 ? 16 : 4), h, sizeof(h));
             } else {
                 // 2^-kShift off the sum and the output, so that they belong to the maximum
-                const int64_t at = (static_cast<int64_t>(split) * a.in.tokens + t) * a.in.heads + head;
-                float* po = a.part_o + at * D + d0;
+                float* po = a.part_o + part * D + d0;
 #pragma unroll
                 for (int j = 0; j < kPer; j += 2) *reinterpret_cast<f32x2*>(po + j) = f32x2{acc[j], acc[j + 1]};
-                if (d0 == 0) a.part_ml[at] = float2{mm - kShift, ls};
+                if (d0 == 0) a.part_ml[part] = float2{mm - kShift, ls};
             }
         }
         if (__builtin_expect(bad != 0, 0)) {
@@ -514,7 +601,7 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
                 if (!((bad >> (16 * rr)) & 0xFFFFu)) continue;
                 const int br = 16 * nt + 4 * w + rr;
                 const RowState st = scan_row<T, C>(v, a, s, br / group, g * group + br % group, begin, end, lane, lanes_per_key(D), true);
-                write_state<T>(v, a, s, s.first + br / group, g * group + br % group, split, st, lane);
+                write_state<T>(v, a, s.first + br / group, g * group + br % group, cp.part_of(a, range, br / group, g * group + br % group), st, lane);
             }
         }
     }
@@ -530,8 +617,8 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
 //     the operands' type once, half a step, of either sign;
 //   * the lanes keep sums of their own; maxima are exchanged only when the running one moves (kSlack).
 // Bound by the vector work of the weights, beside LDS reads and the products.
-// Block x: (kv head, range, sequence) x row tile, eight items side by side, so that an item's row tiles meet on
-// one XCD and its keys in one L2.
+// The kv heads come fastest in the grid: with 8 of them (or 16, ..) the row tiles of one meet on one XCD and its
+// keys in one L2.
 constexpr int kTileRows = 128, kTileKeys = 64;
 
 template <int D>
@@ -548,36 +635,36 @@ struct TileGeom {
 extern __shared__ __align__(16) uint16_t tile_lds[];
 
 template <class T, class C, int D>
-__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_tile_kernel(View v, AttnArgs a, int tiles, int items) {
+__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_tile_kernel(View v, AttnArgs a) {
     using F = Frag<T>;
     using v8 = typename F::v8;
     using G = TileGeom<D>;
     constexpr bool kFp8 = std::is_same_v<C, Fp8>;
     using Raw = std::conditional_t<kFp8, u32x2, u32x4>;  // 8 elements of the cache
-    __shared__ int pages[kMaxRangePages];
+    __shared__ int pages[kWindowPages];
     const int kvh = v.c.kv_heads, group = a.in.heads / kvh;
-    const int tile = static_cast<int>(blockIdx.x / 8) % tiles;
-    const int item = static_cast<int>(blockIdx.x / 8) / tiles * 8 + static_cast<int>(blockIdx.x % 8);
-    if (item >= items) return;
-    const int g = item % kvh, split = item / kvh % a.splits, seq = item / kvh / a.splits;
-    const Span s = span_of(v, a, seq);
-    const int n_rows = min(s.n, a.in.max_new) * group, r0 = tile * kTileRows;
-    const int begin = split * a.kps;
-    if (r0 >= n_rows || (begin >= s.total && split > 0)) return;
     const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    CallPlan<kTileRows, kTileKeys> cp;
+    if (!cp.template find<true>(v, a, static_cast<int>(blockIdx.x), lane)) return;
+    const int g = __builtin_amdgcn_readfirstlane(cp.block % kvh), rest = __builtin_amdgcn_readfirstlane(cp.block / kvh);
+    const int tile = rest % __builtin_amdgcn_readfirstlane(cp.tiles), range = rest / __builtin_amdgcn_readfirstlane(cp.tiles);
+    const Span s = span_of(v, a, __builtin_amdgcn_readfirstlane(cp.seq));
+    const int kps = __builtin_amdgcn_readfirstlane(cp.kps), begin = range * kps;
+    const int n_rows = min(s.n, a.in.max_new) * group, r0 = tile * kTileRows;
     const int r = r0 + 32 * w + l32;
     const bool row_live = r < n_rows;
     const int i = min(r, n_rows - 1) / group, head = g * group + min(r, n_rows - 1) % group, t_out = s.first + i;
     const int last = (min(r0 + kTileRows, n_rows) - 1) / group;
     const int n_keys = a.in.mask ? s.total : min(s.total, s.ctx + last + 1);
-    const int end = min(n_keys, begin + a.kps), p0 = begin >> v.page_shift;
-    const int64_t part = (static_cast<int64_t>(split) * a.in.tokens + t_out) * a.in.heads + head;
-    if (begin >= end && begin > 0) {  // keys of later rows only
+    const int end = min(n_keys, begin + kps);
+    const int64_t part = cp.part_of(a, range, i, head);
+    if (begin >= end && range > 0) {  // keys of later rows only
         if (row_live && h == 0) a.part_ml[part] = float2{-INFINITY, 0.0f};
         return;
     }
-    const bool missing = stage_pages(v, seq, begin, end, pages);
+    int from = begin, until = min(end, begin + kWindow);  // the keys whose pages are staged
+    bool missing = stage_pages(v, s.seq, from, until, pages);
 
     v8 qf[D / 16];
     {
@@ -587,8 +674,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_tile_ker
     }
     const C* kbase = static_cast<const C*>(v.c.k) + g * v.c.k_head;
     const C* vbase = static_cast<const C*>(v.c.v) + g * v.c.v_head;
-    const int n_pages = begin < end ? ((end - 1) >> v.page_shift) - p0 + 1 : 0;
-    auto page_at = [&](int key) { return pages[min((key >> v.page_shift) - p0, n_pages - 1)]; };  // keys past the end: its page
+    auto page_at = [&](int key) { return pages[(min(key, until - 1) >> v.page_shift) - (from >> v.page_shift)]; };  // past the end: the last page
 
     Raw kr[G::kKUnits], vr[G::kVUnits][2];
     auto load = [&](int kb) {
@@ -655,13 +741,35 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_tile_ker
         store(begin, 0);
     }
     __syncthreads();
+    // which 16 keys of a tile have their page
+    auto bits_at = [&](int kb) {
+        uint32_t b = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b |= (page_at(kb + 16 * e) >= 0 ? 1u : 0u) << e;
+        return b;
+    };
+    uint32_t page_bits = 15;
     for (int kb = begin, buf = 0; kb < end; kb += kTileKeys, buf ^= 1) {
         const bool more = kb + kTileKeys < end;
-        if (more) load(kb + kTileKeys);
+        const bool was_missing = missing;
+        if (more) {
+            if (kb + kTileKeys >= until) {  // the last barrier ended every use of the old pages but this tile's masks
+                if (missing) page_bits = bits_at(kb);
+                __syncthreads();
+                from = until;
+                until = min(end, from + kWindow);
+                missing = stage_pages(v, s.seq, from, until, pages);
+            } else if (missing) {
+                page_bits = bits_at(kb);
+            }
+            load(kb + kTileKeys);
+        } else if (missing) {
+            page_bits = bits_at(kb);
+        }
         if (live) {
             const uint16_t* sk = tile_lds + buf * G::kBuf;
             const uint16_t* sv = sk + G::kK;
-            const bool full = kb + kTileKeys <= s.ctx && kb + kTileKeys <= end && !missing;
+            const bool full = kb + kTileKeys <= s.ctx && kb + kTileKeys <= end && !was_missing;
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
                 // register e is key 32 hh + 8 (e / 4) + 4 h + e % 4 of row l32
@@ -680,9 +788,9 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_tile_ker
                 }
                 if (!full) {
                     uint32_t vis = visible32(a, s, i, kb + 32 * hh);
-                    if (missing) {
-                        if (page_at(kb + 32 * hh) < 0) vis &= 0xFFFF0000u;
-                        if (page_at(kb + 32 * hh + 16) < 0) vis &= 0x0000FFFFu;
+                    if (was_missing) {
+                        if (!((page_bits >> (2 * hh)) & 1)) vis &= 0xFFFF0000u;
+                        if (!((page_bits >> (2 * hh)) & 2)) vis &= 0x0000FFFFu;
                     }
                     vis >>= 4 * h;
 #pragma unroll
@@ -739,7 +847,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_tile_ker
     uint64_t bad = __ballot(nan && row_live && l_run == l_run);  // as in attention_rows_kernel
     bad |= bad >> 32;
     if (row_live && !((bad >> l32) & 1)) {
-        if (one_range(a, s)) {
+        if (part < 0) {
             const float inv = l_run == 0.0f ? 0.0f : a.v_scale / l_run;
             T* out = static_cast<T*>(a.in.out) + static_cast<int64_t>(t_out) * a.in.out_token + head * a.in.out_head + 4 * h;
 #pragma unroll
@@ -767,23 +875,37 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_tile_ker
         const int br = r0 + 32 * w + __builtin_ctzll(bad);
         bad &= bad - 1;
         const RowState st = scan_row<T, C>(v, a, s, br / group, g * group + br % group, begin, end, lane, lanes_per_key(D), true);
-        write_state<T>(v, a, s, s.first + br / group, g * group + br % group, split, st, lane);
+        write_state<T>(v, a, s.first + br / group, g * group + br % group, cp.part_of(a, range, br / group, g * group + br % group), st, lane);
     }
 }
 
 // Joins the ranges of each row in their order: D / 4 threads a row, 4 ranges requested at once.
 // Block (x, y): token, heads.
-template <class T>
+template <class T, int kTile, int kStep>
 __global__ __launch_bounds__(kThreads) void attention_merge_kernel(View v, AttnArgs a) {
-    const int t = blockIdx.x, D = v.c.head_dim, per = D / 4, rows = kThreads / per;
-    const int seq = sequence_of(v, t, threadIdx.x & 63);
+    const int t = blockIdx.x, D = v.c.head_dim, per = D / 4, rows = kThreads / per, lane = threadIdx.x & 63;
+    const int seq = sequence_of(v, t, lane);
     if (seq >= v.c.batch || t < v.c.cu[seq]) return;
-    const Span s = span_of(v, a, seq);
-    if (one_range(a, s)) return;  // written by the range itself
+    int n;
+    int64_t row, step;  // the first range's partial row of head 0, rows between ranges
+    if constexpr (kTile > 0) {
+        CallPlan<kTile, kStep> cp;
+        cp.template find<false>(v, a, seq, lane);
+        const int i = t - max(v.c.cu[seq], 0);
+        if (cp.ranges <= 1 || i >= cp.rows) return;  // written by the range itself
+        n = cp.ranges;
+        row = cp.part_of(a, 0, i, 0);
+        step = static_cast<int64_t>(cp.rows) * a.in.heads;
+    } else {
+        const Span s = span_of(v, a, seq);
+        if (s.total <= a.kps) return;
+        n = (s.total + a.kps - 1) / a.kps;
+        row = static_cast<int64_t>(t) * a.in.heads;
+        step = static_cast<int64_t>(a.in.tokens) * a.in.heads;
+    }
     const int slot = threadIdx.x / per, d0 = 4 * (threadIdx.x % per), head = blockIdx.y * rows + slot;
     if (slot >= rows || head >= a.in.heads) return;
-    const int n = (s.total + a.kps - 1) / a.kps;
-    const int64_t row = static_cast<int64_t>(t) * a.in.heads + head, step = static_cast<int64_t>(a.in.tokens) * a.in.heads;
+    row += head;
     float m = -INFINITY, l = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int c0 = 0; c0 < n; c0 += 4) {
@@ -820,12 +942,17 @@ __global__ __launch_bounds__(kThreads) void attention_merge_kernel(View v, AttnA
 }
 
 // ---- host side -------------------------------------------------------------------------------
+int env_int(const char* n, int d) { const char* e = getenv(n); return e ? atoi(e) : d; }
 // Which kernel serves a call, by the rows (tokens x query heads) that share a kv head, and how its keys are cut.
 enum class Kind { kLanes, kRows, kTile };
 struct Plan {
     Kind kind;
-    int row_tiles;  // of 16 rows (kRows), 128 (kTile)
-    int splits, kps;
+    int row_tiles;      // of 16 rows (kRows)
+    int kps, splits;    // kLanes
+    int target;         // the others: workgroups to cut the call into ..
+    int64_t blocks;     // .. and what that makes at most
+    bool merge;
+    int64_t parts;      // partial rows at most
     size_t o_bytes, bytes;
 };
 
@@ -844,26 +971,36 @@ Plan plan(const View& v, const qmm_paged_query& in) {
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(static_cast<int64_t>(v.c.table_width) * v.c.page_size, INT32_MAX - 65536));
     const int64_t rows = static_cast<int64_t>(in.tokens) * in.heads;
     const int64_t per_kv = static_cast<int64_t>(std::min(in.max_new, in.tokens)) * (in.heads / v.c.kv_heads);
-    int64_t kps;
+    const int kvh = v.c.kv_heads;
     if (!matrix_operands(v, in) || per_kv > (1 << 28)) {
         p.kind = Kind::kLanes;
-        kps = 64;
+        int64_t kps = 64;
         while (kps < most && (rows * ((most + kps - 1) / kps) > 16384 || (most + kps - 1) / kps > 1024)) kps *= 2;
+        p.kps = static_cast<int>(kps);
+        p.splits = static_cast<int>((most + kps - 1) / kps);
+        p.merge = p.splits > 1;
+        p.parts = rows * p.splits;
     } else {
         // more row tiles of head_dim 256 do not fit a wave's registers
         p.kind = per_kv <= (v.c.head_dim <= 128 ? 64 : 16) ? Kind::kRows : Kind::kTile;
-        const int tile = p.kind == Kind::kRows ? 16 : kTileRows;
-        p.row_tiles = static_cast<int>((per_kv + tile - 1) / tile);
-        const int64_t groups = static_cast<int64_t>(v.c.batch) * v.c.kv_heads * (p.kind == Kind::kRows ? 1 : p.row_tiles);
-        const int64_t target = p.kind == Kind::kRows ? 4096 : 512;
-        kps = p.kind == Kind::kRows ? 128 : 256;
-        while (kps < most && kps < kMaxRange && groups * ((most + kps - 1) / kps) > target) kps *= 2;
+        const bool few = p.kind == Kind::kRows;
+        p.row_tiles = few ? static_cast<int>((per_kv + 15) / 16) : 0;
+        p.target = few ? env_int("T_ROWS", 1024) : env_int("T_TILE", 512);
+        // A plan's ranges are at least `least` keys.  With W steps in all and u = ceil(W / target) steps a range, the
+        // ranges of all row tiles are at most 2 W / u and one more per row tile (a chain's last tile sees up to twice
+        // the mean), and those of sequences with more than one range at most twice that, 4 target.
+        const int64_t least = few ? kRowsStep : kTileKeys * CallPlan<kTileRows, kTileKeys>::kMinSteps;
+        const int64_t most_ranges = (most + least - 1) / least;
+        const int64_t seqs = std::min(v.c.batch, in.tokens);
+        const int64_t items = kvh * (few ? seqs : seqs + (static_cast<int64_t>(in.tokens) * (in.heads / kvh) + kTileRows - 1) / kTileRows);
+        p.blocks = std::min(items * most_ranges, 2 * static_cast<int64_t>(p.target) + items);
+        p.merge = most_ranges > 1;
+        const int64_t tile_rows = few ? 16 * p.row_tiles : kTileRows;
+        p.parts = std::min(rows * most_ranges, 4 * p.target * tile_rows);
     }
-    p.kps = static_cast<int>(kps);
-    p.splits = static_cast<int>((most + kps - 1) / kps);
-    if (p.splits > 1) {
-        p.o_bytes = static_cast<size_t>(p.splits) * rows * v.c.head_dim * sizeof(float);
-        p.bytes = p.o_bytes + static_cast<size_t>(p.splits) * rows * sizeof(float2);
+    if (p.merge) {
+        p.o_bytes = static_cast<size_t>(p.parts) * v.c.head_dim * sizeof(float);
+        p.bytes = p.o_bytes + static_cast<size_t>(p.parts) * sizeof(float2);
     }
     return p;
 }
@@ -892,10 +1029,8 @@ bool operands_aligned(const View& v, const qmm_paged_query& in) {
 
 template <class T, class C, int D>
 int launch_matrix(const View& v, const AttnArgs& a, const Plan& p, hipStream_t stream) {
-    const int64_t items = static_cast<int64_t>(v.c.batch) * v.c.kv_heads * p.splits;
-    const int64_t blocks = p.kind == Kind::kRows ? items : (items + 7) / 8 * 8 * p.row_tiles;
-    if (blocks > INT32_MAX) return bad("too many sequences, heads and tokens for one call.");
-    const dim3 grid(static_cast<unsigned>(blocks));
+    if (p.blocks > INT32_MAX) return bad("too many sequences, heads and tokens for one call.");
+    const dim3 grid(static_cast<unsigned>(p.blocks));
     if (p.kind == Kind::kRows) {
         auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, stream, v, a); };
         if constexpr (D <= 128) {
@@ -913,7 +1048,7 @@ int launch_matrix(const View& v, const AttnArgs& a, const Plan& p, hipStream_t s
                                    static_cast<int>(G::kLds));
     });
     if (attr != hipSuccess) return launched(attr, "paged attention LDS size");
-    hipLaunchKernelGGL((attention_tile_kernel<T, C, D>), grid, dim3(kThreads), G::kLds, stream, v, a, p.row_tiles, static_cast<int>(items));
+    hipLaunchKernelGGL((attention_tile_kernel<T, C, D>), grid, dim3(kThreads), G::kLds, stream, v, a);
     return QMM_OK;
 }
 
@@ -938,8 +1073,8 @@ int tree_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, void* work
     const float scale = in->scale != 0.0f ? in->scale : 1.0f / std::sqrt(static_cast<float>(v.c.head_dim));
     a.scale_log2 = scale * v.c.k_scale * 1.4426950408889634f;
     a.v_scale = v.c.v_scale;
-    a.splits = p.splits;
     a.kps = p.kps;
+    a.target = p.target;
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + p.o_bytes);
     const bool fp8 = v.c.dtype == QMM_DTYPE_E4M3;
@@ -964,11 +1099,17 @@ int tree_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, void* work
     if (rc2 != QMM_OK) return rc2;
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return launched(e, "paged attention kernel launch");
-    if (p.splits > 1) {
+    if (p.merge) {
         const int rows = kThreads / (v.c.head_dim / 4);
         const dim3 mgrid(static_cast<unsigned>(in->tokens), static_cast<unsigned>((in->heads + rows - 1) / rows));
-        if (in->dtype == QMM_DTYPE_F16) hipLaunchKernelGGL(attention_merge_kernel<_Float16>, mgrid, dim3(kThreads), 0, stream, v, a);
-        else hipLaunchKernelGGL(attention_merge_kernel<__bf16>, mgrid, dim3(kThreads), 0, stream, v, a);
+        auto merge = [&](auto tc) {
+            using T = decltype(tc);
+            auto go = [&](auto kern) { hipLaunchKernelGGL(kern, mgrid, dim3(kThreads), 0, stream, v, a); };
+            if (p.kind == Kind::kLanes) go(attention_merge_kernel<T, 0, 0>);
+            else if (p.kind == Kind::kRows) go(attention_merge_kernel<T, 16, kRowsStep>);
+            else go(attention_merge_kernel<T, kTileRows, kTileKeys>);
+        };
+        in->dtype == QMM_DTYPE_F16 ? merge(_Float16{}) : merge(__bf16{});
         e = hipGetLastError();
     }
     return launched(e, "paged attention merge kernel launch");
