@@ -251,7 +251,7 @@ __device__ __forceinline__ uint32_t visible32(const AttnArgs& a, const Span& s, 
 //   partials   the rows of sequences with more than one range, in the same order.
 template <int kTile, int kStep>
 struct CallPlan {
-    static constexpr int kMinSteps = kTile == 128 ? 4 : 1;
+    static constexpr int kMinSteps = kTile >= 128 ? 4 : 1;
     int kps, seq, block;   // block within the sequence
     int rows, tiles, ranges;  // of the sequence: tokens with rows, row tiles
     int64_t first_part;    // of the sequence, in tokens
@@ -266,7 +266,7 @@ struct CallPlan {
             const Span s = span_of(v, a, b);
             const int group = a.in.heads / v.c.kv_heads;
             x.rows = min(s.n, a.in.max_new);
-            x.tiles = kTile == 128 ? (x.rows * group + kTile - 1) / kTile : x.rows > 0;
+            x.tiles = kTile >= 128 ? (x.rows * group + kTile - 1) / kTile : x.rows > 0;
             x.total = s.total;
             const int seen = a.in.mask ? s.total : min(s.total, s.ctx + (s.n + 1) / 2);
             x.steps = static_cast<int64_t>(max((seen + kStep - 1) / kStep, 1)) * x.tiles;
@@ -608,137 +608,166 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
 }
 
 // ---- many rows: keys through LDS -----------------------------------------------------------------
-// A workgroup of 4 waves owns 128 rows (tokens x query heads of one kv head), 32 a wave, and walks the keys in
+// A workgroup of 4 waves owns 128 RT rows (tokens x query heads of one kv head), 32 RT a wave, and walks the keys in
 // tiles of 64, staged through LDS (two buffers, one barrier a tile) and taken 32 at a time:
 //   * S^T = K Q^T on 32x32x16, the wave's queries in registers: a lane holds one row (lane % 32) and 16 of the 32
 //     keys, the partner lane (lane ^ 32) the others;
 //   * the weights go from the S registers into O^T += V^T P^T without leaving the lane (the k order of each 16-key
-//     block is the order the lane holds its keys in); V is staged transposed ([dim][key]).  Weights are rounded to
-//     the operands' type once, half a step, of either sign;
+//     block is the order the lane holds its keys in).  Weights are rounded to the operands' type once, half a step, of
+//     either sign;
 //   * the lanes keep sums of their own; maxima are exchanged only when the running one moves (kSlack).
-// Bound by the vector work of the weights, beside LDS reads and the products.
-// The kv heads come fastest in the grid: with 8 of them (or 16, ..) the row tiles of one meet on one XCD and its
-// keys in one L2.
+// Wave w stages keys 16 w .. 16 w + 15 of a tile, which share a page: a scalar address and lane offsets that never change,
+// copied straight into LDS (global_load_lds; an fp8 cache goes through registers, converted on the way).  Both K
+// and V lie as they are in memory, with the 16-byte pieces of a row exchanged by its number (TileGeom) so that neither the
+// key fragments (16 rows, one piece) nor V's transposing reads (ds_read_b64_tr_b16: 4 rows, two pieces) meet on a bank.
+// Bound by the vector work of the weights beside the products.  The kv heads come fastest in the grid: with 8 of them
+// (or 16, ..) the row tiles of one meet on one XCD and its keys in one L2.
 constexpr int kTileRows = 128, kTileKeys = 64;
 
 template <int D>
 struct TileGeom {
-    static constexpr int kRowK = D + 8;           // elements per staged key row (16-byte pad)
-    static constexpr int kRowV = kTileKeys + 4;   // elements per staged V^T row (8-byte pad)
-    static constexpr int kK = kTileKeys * kRowK, kV = D * kRowV, kBuf = kK + kV;
+    static constexpr int kTileE = kTileKeys * D;      // elements of one staged tile
+    static constexpr int kBuf = 2 * kTileE;           // K and V
     static constexpr size_t kLds = 2 * static_cast<size_t>(kBuf) * 2;
-    static constexpr int kChunks = D / 8;
-    static constexpr int kKUnits = kTileKeys * kChunks / kThreads;
-    static constexpr int kVAll = kTileKeys / 2 * kChunks, kVUnits = (kVAll + kThreads - 1) / kThreads;
+    static constexpr int kChunks = D / 8, kPieces = D / 32;  // 16-byte pieces of a row; of 16 rows, per lane
+    // what the piece number is XORed with
+    static __device__ __forceinline__ int swap_k(int row) { return D == 64 ? (row >> 1) & 7 : D == 96 ? (row >> 2) & 3 : row & 15; }
+    static __device__ __forceinline__ int swap_v(int row) { return D == 64 ? ((row >> 1) & 3) << 1 : D == 96 ? 0 : (row & 7) << 1; }
 };
 
 extern __shared__ __align__(16) uint16_t tile_lds[];
 
-template <class T, class C, int D>
-__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_tile_kernel(View v, AttnArgs a) {
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+using LdsPtr = __attribute__((address_space(3))) uint16_t*;
+
+// 16 bytes per lane from base + off into LDS at m0 + 16 lane
+__device__ __forceinline__ void copy_to_lds(const void* base, uint32_t off, uint32_t lds) {
+    __asm__ volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
+}
+
+template <class T, class C, int D, int RT>
+__global__ __launch_bounds__(kThreads, D <= 128 && RT == 1 ? 2 : 1) void attention_tile_kernel(View v, AttnArgs a) {
     using F = Frag<T>;
     using v8 = typename F::v8;
     using G = TileGeom<D>;
     constexpr bool kFp8 = std::is_same_v<C, Fp8>;
-    using Raw = std::conditional_t<kFp8, u32x2, u32x4>;  // 8 elements of the cache
     __shared__ int pages[kWindowPages];
     const int kvh = v.c.kv_heads, group = a.in.heads / kvh;
     const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    CallPlan<kTileRows, kTileKeys> cp;
+    CallPlan<kTileRows * RT, kTileKeys> cp;
     if (!cp.template find<true>(v, a, static_cast<int>(blockIdx.x), lane)) return;
     const int g = __builtin_amdgcn_readfirstlane(cp.block % kvh), rest = __builtin_amdgcn_readfirstlane(cp.block / kvh);
-    const int tile = rest % __builtin_amdgcn_readfirstlane(cp.tiles), range = rest / __builtin_amdgcn_readfirstlane(cp.tiles);
+    const int tiles = __builtin_amdgcn_readfirstlane(cp.tiles), tile = rest % tiles, range = rest / tiles;
     const Span s = span_of(v, a, __builtin_amdgcn_readfirstlane(cp.seq));
     const int kps = __builtin_amdgcn_readfirstlane(cp.kps), begin = range * kps;
-    const int n_rows = min(s.n, a.in.max_new) * group, r0 = tile * kTileRows;
-    const int r = r0 + 32 * w + l32;
-    const bool row_live = r < n_rows;
-    const int i = min(r, n_rows - 1) / group, head = g * group + min(r, n_rows - 1) % group, t_out = s.first + i;
-    const int last = (min(r0 + kTileRows, n_rows) - 1) / group;
+    const int n_rows = min(s.n, a.in.max_new) * group, r0 = tile * kTileRows * RT, rw = r0 + 32 * RT * w;
+    const int last = (min(r0 + kTileRows * RT, n_rows) - 1) / group;
     const int n_keys = a.in.mask ? s.total : min(s.total, s.ctx + last + 1);
     const int end = min(n_keys, begin + kps);
-    const int64_t part = cp.part_of(a, range, i, head);
+    int i[RT], head[RT];  // of row rw + 32 rt + l32; rows past the last repeat it
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int r = min(rw + 32 * rt + l32, n_rows - 1);
+        i[rt] = r / group;
+        head[rt] = g * group + r % group;
+    }
     if (begin >= end && range > 0) {  // keys of later rows only
-        if (row_live && h == 0) a.part_ml[part] = float2{-INFINITY, 0.0f};
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+            if (rw + 32 * rt + l32 < n_rows && h == 0) a.part_ml[cp.part_of(a, range, i[rt], head[rt])] = float2{-INFINITY, 0.0f};
         return;
     }
     int from = begin, until = min(end, begin + kWindow);  // the keys whose pages are staged
     bool missing = stage_pages(v, s.seq, from, until, pages);
 
-    v8 qf[D / 16];
-    {
-        const T* qrow = static_cast<const T*>(a.in.q) + static_cast<int64_t>(t_out) * a.in.q_token + head * a.in.q_head + 8 * h;
+    // a negative scale: the same scores from -q and its magnitude
+    const float scale = fabsf(a.scale_log2);
+    v8 qf[RT][D / 16];
 #pragma unroll
-        for (int db = 0; db < D / 16; ++db) __builtin_memcpy(&qf[db], __builtin_assume_aligned(qrow + 16 * db, 16), 16);
+    for (int rt = 0; rt < RT; ++rt) {
+        const T* qrow = static_cast<const T*>(a.in.q) + static_cast<int64_t>(s.first + i[rt]) * a.in.q_token + head[rt] * a.in.q_head + 8 * h;
+#pragma unroll
+        for (int db = 0; db < D / 16; ++db) {
+            __builtin_memcpy(&qf[rt][db], __builtin_assume_aligned(qrow + 16 * db, 16), 16);
+            if (a.scale_log2 < 0.0f) qf[rt][db] = -qf[rt][db];
+        }
     }
     const C* kbase = static_cast<const C*>(v.c.k) + g * v.c.k_head;
     const C* vbase = static_cast<const C*>(v.c.v) + g * v.c.v_head;
     auto page_at = [&](int key) { return pages[(min(key, until - 1) >> v.page_shift) - (from >> v.page_shift)]; };  // past the end: the last page
 
-    Raw kr[G::kKUnits], vr[G::kVUnits][2];
-    auto load = [&](int kb) {
+    // piece 64 j + lane of the wave's 16 rows
+    uint32_t k_off[G::kPieces], v_off[G::kPieces];
 #pragma unroll
-        for (int u = 0; u < G::kKUnits; ++u) {
-            const int x = tid + kThreads * u, key = kb + x / G::kChunks, c = x % G::kChunks;
-            const int64_t page = max(page_at(key), 0);
-            kr[u] = *reinterpret_cast<const Raw*>(kbase + page * v.c.k_page + (key & (v.c.page_size - 1)) * v.c.k_slot + 8 * c);
-        }
+    for (int j = 0; j < G::kPieces; ++j) {
+        const int row = (64 * j + lane) / G::kChunks, pos = (64 * j + lane) % G::kChunks;
+        k_off[j] = static_cast<uint32_t>((row * v.c.k_slot + 8 * (pos ^ G::swap_k(row))) * static_cast<int>(sizeof(C)));
+        v_off[j] = static_cast<uint32_t>((row * v.c.v_slot + 8 * (pos ^ G::swap_v(row))) * static_cast<int>(sizeof(C)));
+    }
+    uint16_t* const mine = tile_lds + 16 * w * D;  // of buffer 0's K
+    const uint32_t mine_at = __builtin_amdgcn_readfirstlane(reinterpret_cast<uintptr_t>((LdsPtr)mine));
+    u32x2 kr[kFp8 ? G::kPieces : 1], vr[kFp8 ? G::kPieces : 1];
+    auto load = [&](int kb, int buf) {
+        const int key = kb + 16 * w, slot = key & (v.c.page_size - 1);
+        const int64_t page = max(__builtin_amdgcn_readfirstlane(page_at(key)), 0);
+        const C* kp = kbase + page * v.c.k_page + slot * v.c.k_slot;
+        const C* vp = vbase + page * v.c.v_page + slot * v.c.v_slot;
 #pragma unroll
-        for (int u = 0; u < G::kVUnits; ++u) {
-            const int x = tid + kThreads * u, key = kb + 2 * (x % (kTileKeys / 2)), c = x / (kTileKeys / 2);
-            if (G::kVAll % kThreads == 0 || x < G::kVAll) {
-                const int64_t page = max(page_at(key), 0);  // a pair shares a page
-                const C* p = vbase + page * v.c.v_page + (key & (v.c.page_size - 1)) * v.c.v_slot + 8 * c;
-                vr[u][0] = *reinterpret_cast<const Raw*>(p);
-                vr[u][1] = *reinterpret_cast<const Raw*>(p + v.c.v_slot);
+        for (int j = 0; j < G::kPieces; ++j) {
+            if constexpr (kFp8) {
+                kr[j] = *reinterpret_cast<const u32x2*>(reinterpret_cast<const char*>(kp) + k_off[j]);
+                vr[j] = *reinterpret_cast<const u32x2*>(reinterpret_cast<const char*>(vp) + v_off[j]);
+            } else {
+                copy_to_lds(kp, k_off[j], mine_at + 2 * (buf * G::kBuf) + 1024 * j);
+                copy_to_lds(vp, v_off[j], mine_at + 2 * (buf * G::kBuf + G::kTileE) + 1024 * j);
             }
         }
     };
-    auto wide = [](Raw x) {
-        if constexpr (kFp8) return u32x4{F::from_fp8(x[0]), F::from_fp8_hi(x[0]), F::from_fp8(x[1]), F::from_fp8_hi(x[1])};
-        else return x;
-    };
-    auto store = [&](int kb, int buf) {
-        uint16_t* sk = tile_lds + buf * G::kBuf;
-        uint16_t* sv = sk + G::kK;
+    // the wave's part of the tile is in LDS afterwards, zeros for the values of rows that nobody sees
+    auto land = [&](int kb, int buf) {
+        uint16_t* sk = mine + buf * G::kBuf + 8 * lane;
+        uint16_t* sv = sk + G::kTileE;
+        if constexpr (kFp8) {
+            auto wide = [](u32x2 x) { return u32x4{F::from_fp8(x[0]), F::from_fp8_hi(x[0]), F::from_fp8(x[1]), F::from_fp8_hi(x[1])}; };
 #pragma unroll
-        for (int u = 0; u < G::kKUnits; ++u) {
-            const int x = tid + kThreads * u, key = x / G::kChunks, c = x % G::kChunks;
-            *reinterpret_cast<u32x4*>(sk + key * G::kRowK + 8 * c) = wide(kr[u]);
-        }
-        const bool whole = kb + kTileKeys <= s.total && !missing;
-#pragma unroll
-        for (int u = 0; u < G::kVUnits; ++u) {
-            const int x = tid + kThreads * u, kp = x % (kTileKeys / 2), c = x / (kTileKeys / 2);
-            if (G::kVAll % kThreads == 0 || x < G::kVAll) {
-                u32x4 lo = wide(vr[u][0]), hi = wide(vr[u][1]);
-                if (!whole) {  // rows that nobody sees may hold anything
-                    const int key = kb + 2 * kp;
-                    const bool ok = page_at(key) >= 0;
-                    if (!ok || key >= s.total) lo = u32x4{0, 0, 0, 0};
-                    if (!ok || key + 1 >= s.total) hi = u32x4{0, 0, 0, 0};
-                }
-                uint32_t* col = reinterpret_cast<uint32_t*>(sv + 8 * c * G::kRowV + 2 * kp);
-#pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                    col[(2 * m) * (G::kRowV / 2)] = __builtin_amdgcn_perm(hi[m], lo[m], 0x05040100u);
-                    col[(2 * m + 1) * (G::kRowV / 2)] = __builtin_amdgcn_perm(hi[m], lo[m], 0x07060302u);
-                }
+            for (int j = 0; j < G::kPieces; ++j) {
+                *reinterpret_cast<u32x4*>(sk + 512 * j) = wide(kr[j]);
+                *reinterpret_cast<u32x4*>(sv + 512 * j) = wide(vr[j]);
             }
+        } else {
+            __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        if (kb + kTileKeys > s.total || missing) {
+            const int key = kb + 16 * w;
+            const bool none = page_at(key) < 0;
+#pragma unroll
+            for (int j = 0; j < G::kPieces; ++j)
+                if (none || key + (64 * j + lane) / G::kChunks >= s.total) *reinterpret_cast<u32x4*>(sv + 512 * j) = u32x4{0, 0, 0, 0};
         }
     };
 
-    f32x16 o[D / 32];
+    f32x16 o[RT][D / 32];
+    float m_run[RT], l_run[RT];
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
+    for (int rt = 0; rt < RT; ++rt) {
+        m_run[rt] = -INFINITY;
+        l_run[rt] = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
-    float m_run = -INFINITY, l_run = 0.0f;
-    const bool live = r0 + 32 * w < n_rows;  // waves without rows only stage
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[rt][dt][e] = 0.0f;
+    }
+    // fragment addresses within a buffer: key row l32, piece 2 db + h; and, of the lane's 16, key 4 h + lane / 4, dims
+    // 16 (l32 / 16) + 4 (lane % 4) of every 32
+    const int kx = h ^ G::swap_k(l32);
+    const uint16_t* k_row = tile_lds + l32 * D;
+    const int vrow = 4 * h + ((lane & 15) >> 2), vx = (2 * (l32 >> 4) + ((lane & 3) >> 1)) ^ G::swap_v(vrow);
+    const uint16_t* v_row = tile_lds + G::kTileE + vrow * D + 4 * (lane & 1);
+    const bool live = rw < n_rows;  // waves without rows only stage
     if (begin < end) {
-        load(begin);
-        store(begin, 0);
+        load(begin, 0);
+        land(begin, 0);
     }
     __syncthreads();
     // which 16 keys of a tile have their page
@@ -752,130 +781,131 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_tile_ker
     for (int kb = begin, buf = 0; kb < end; kb += kTileKeys, buf ^= 1) {
         const bool more = kb + kTileKeys < end;
         const bool was_missing = missing;
+        if (missing) page_bits = bits_at(kb);
         if (more) {
-            if (kb + kTileKeys >= until) {  // the last barrier ended every use of the old pages but this tile's masks
-                if (missing) page_bits = bits_at(kb);
+            if (kb + kTileKeys >= until) {  // every wave is past its last use of the old pages: the loop's barrier, bits_at
                 __syncthreads();
                 from = until;
                 until = min(end, from + kWindow);
                 missing = stage_pages(v, s.seq, from, until, pages);
-            } else if (missing) {
-                page_bits = bits_at(kb);
             }
-            load(kb + kTileKeys);
-        } else if (missing) {
-            page_bits = bits_at(kb);
+            load(kb + kTileKeys, buf ^ 1);
         }
         if (live) {
-            const uint16_t* sk = tile_lds + buf * G::kBuf;
-            const uint16_t* sv = sk + G::kK;
             const bool full = kb + kTileKeys <= s.ctx && kb + kTileKeys <= end && !was_missing;
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
                 // register e is key 32 hh + 8 (e / 4) + 4 h + e % 4 of row l32
-                f32x16 x;
+                f32x16 x[RT];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = 0.0f;
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[rt][e] = 0.0f;
 #pragma unroll
                 for (int db = 0; db < D / 16; ++db) {
                     v8 kf;
-                    __builtin_memcpy(&kf, __builtin_assume_aligned(sk + (32 * hh + l32) * G::kRowK + 16 * db + 8 * h, 16), 16);
-                    x = F::mma32(kf, qf[db], x);
-                }
-                if (a.scale_log2 < 0.0f) {  // the maximum below is of raw scores
+                    __builtin_memcpy(&kf, __builtin_assume_aligned(k_row + buf * G::kBuf + 32 * hh * D + 8 * ((2 * db) ^ kx), 16), 16);
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) x[e] = -x[e];
+                    for (int rt = 0; rt < RT; ++rt) x[rt] = F::mma32(kf, qf[rt][db], x[rt]);
                 }
-                if (!full) {
-                    uint32_t vis = visible32(a, s, i, kb + 32 * hh);
-                    if (was_missing) {
-                        if (!((page_bits >> (2 * hh)) & 1)) vis &= 0xFFFF0000u;
-                        if (!((page_bits >> (2 * hh)) & 2)) vis &= 0x0000FFFFu;
+                v8 pf[RT][2];
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    if (!full) {
+                        uint32_t vis = visible32(a, s, i[rt], kb + 32 * hh);
+                        if (was_missing) {
+                            if (!((page_bits >> (2 * hh)) & 1)) vis &= 0xFFFF0000u;
+                            if (!((page_bits >> (2 * hh)) & 2)) vis &= 0x0000FFFFu;
+                        }
+                        vis >>= 4 * h;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (!((vis >> (8 * (e >> 2) + (e & 3))) & 1)) x[rt][e] = -INFINITY;
                     }
-                    vis >>= 4 * h;
+                    float mx = x[rt][0];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (!((vis >> (8 * (e >> 2) + (e & 3))) & 1)) x[e] = -INFINITY;
-                }
-                const float scale = fabsf(a.scale_log2);
-                float mx = x[0];
+                    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, x[rt][e]);
+                    mx *= scale;
+                    if (__ballot(mx > m_run[rt] + kSlack) != 0) {
+                        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                        const float mn = fmaxf(m_run[rt], mx);
+                        const float f = m_run[rt] == mn ? 1.0f : __builtin_amdgcn_exp2f(m_run[rt] - mn);
+                        l_run[rt] *= f;
 #pragma unroll
-                for (int e = 1; e < 16; ++e) mx = fmaxf(mx, x[e]);
-                mx *= scale;
-                if (__ballot(mx > m_run + kSlack) != 0) {
-                    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-                    const float mn = fmaxf(m_run, mx);
-                    const float f = m_run == mn ? 1.0f : __builtin_amdgcn_exp2f(m_run - mn);
-                    l_run *= f;
+                        for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-                    for (int dt = 0; dt < D / 32; ++dt)
+                            for (int e = 0; e < 16; ++e) o[rt][dt][e] *= f;
+                        m_run[rt] = mn;
+                    }
+                    const float base = m_run[rt] == -INFINITY ? 0.0f : m_run[rt] - kShift;
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) o[dt][e] *= f;
-                    m_run = mn;
-                }
-                const float base = m_run == -INFINITY ? 0.0f : m_run - kShift;
-                v8 pf[2];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float p = __builtin_amdgcn_exp2f(__fmaf_rn(x[e], scale, -base));
-                    l_run += p;
-                    pf[e >> 3][e & 7] = static_cast<T>(p);
+                    for (int e = 0; e < 16; ++e) {
+                        const float p = __builtin_amdgcn_exp2f(__fmaf_rn(x[rt][e], scale, -base));
+                        l_run[rt] += p;
+                        pf[rt][e >> 3][e & 7] = static_cast<T>(p);
+                    }
                 }
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
                     for (int dt = 0; dt < D / 32; ++dt) {
-                        const uint16_t* vrow = sv + (32 * dt + l32) * G::kRowV + 32 * hh + 16 * b + 4 * h;
-                        u32x2 f0, f1;
-                        __builtin_memcpy(&f0, __builtin_assume_aligned(vrow, 8), 8);
-                        __builtin_memcpy(&f1, __builtin_assume_aligned(vrow + 8, 8), 8);
-                        const u32x4 vf = {f0[0], f0[1], f1[0], f1[1]};
-                        o[dt] = F::mma32(__builtin_bit_cast(v8, vf), pf[b], o[dt]);
+                        const uint16_t* at = v_row + buf * G::kBuf + (32 * hh + 16 * b) * D + 8 * ((4 * dt) ^ vx);
+                        const s16x4 f0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+                        const s16x4 f1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 8 * D));
+                        const v8 vf = __builtin_bit_cast(v8, __builtin_shufflevector(f0, f1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) o[rt][dt] = F::mma32(vf, pf[rt][b], o[rt][dt]);
                     }
             }
         }
-        if (more) store(kb + kTileKeys, buf ^ 1);
+        if (more) land(kb + kTileKeys, buf ^ 1);
         __syncthreads();
     }
     if (!live) return;
-    l_run += __shfl_xor(l_run, 32, 64);
-    bool nan = false;
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
+    for (int rt = 0; rt < RT; ++rt) {
+        const bool row_live = rw + 32 * rt + l32 < n_rows;
+        const int64_t part = cp.part_of(a, range, i[rt], head[rt]);
+        const float l = l_run[rt] + __shfl_xor(l_run[rt], 32, 64);
+        bool nan = false;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) nan |= o[dt][e] != o[dt][e];
-    uint64_t bad = __ballot(nan && row_live && l_run == l_run);  // as in attention_rows_kernel
-    bad |= bad >> 32;
-    if (row_live && !((bad >> l32) & 1)) {
-        if (part < 0) {
-            const float inv = l_run == 0.0f ? 0.0f : a.v_scale / l_run;
-            T* out = static_cast<T*>(a.in.out) + static_cast<int64_t>(t_out) * a.in.out_token + head * a.in.out_head + 4 * h;
+        for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-            for (int dt = 0; dt < D / 32; ++dt)
+            for (int e = 0; e < 16; ++e) nan |= o[rt][dt][e] != o[rt][dt][e];
+        uint64_t bad = __ballot(nan && row_live && l == l);  // as in attention_rows_kernel
+        bad |= bad >> 32;
+        if (row_live && !((bad >> l32) & 1)) {
+            if (part < 0) {
+                const float inv = l == 0.0f ? 0.0f : a.v_scale / l;
+                T* out = static_cast<T*>(a.in.out) + static_cast<int64_t>(s.first + i[rt]) * a.in.out_token + head[rt] * a.in.out_head + 4 * h;
 #pragma unroll
-                for (int q4 = 0; q4 < 4; ++q4) {
-                    T v4[4];
+                for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v4[e] = static_cast<T>(o[dt][4 * q4 + e] * inv);
-                    __builtin_memcpy(__builtin_assume_aligned(out + 32 * dt + 8 * q4, 8), v4, 8);
-                }
-        } else {
-            float* po = a.part_o + part * D + 4 * h;
+                    for (int q4 = 0; q4 < 4; ++q4) {
+                        T v4[4];
 #pragma unroll
-            for (int dt = 0; dt < D / 32; ++dt)
+                        for (int e = 0; e < 4; ++e) v4[e] = static_cast<T>(o[rt][dt][4 * q4 + e] * inv);
+                        __builtin_memcpy(__builtin_assume_aligned(out + 32 * dt + 8 * q4, 8), v4, 8);
+                    }
+            } else {
+                float* po = a.part_o + part * D + 4 * h;
 #pragma unroll
-                for (int q4 = 0; q4 < 4; ++q4)
-                    *reinterpret_cast<f32x4*>(po + 32 * dt + 8 * q4) =
-                        f32x4{o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]};
-            if (h == 0) a.part_ml[part] = float2{m_run - kShift, l_run};
+                for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+                    for (int q4 = 0; q4 < 4; ++q4)
+                        *reinterpret_cast<f32x4*>(po + 32 * dt + 8 * q4) =
+                            f32x4{o[rt][dt][4 * q4], o[rt][dt][4 * q4 + 1], o[rt][dt][4 * q4 + 2], o[rt][dt][4 * q4 + 3]};
+                if (h == 0) a.part_ml[part] = float2{m_run[rt] - kShift, l};
+            }
         }
-    }
-    bad &= 0xFFFFFFFFu;
-    while (__builtin_expect(bad != 0, 0)) {
-        const int br = r0 + 32 * w + __builtin_ctzll(bad);
-        bad &= bad - 1;
-        const RowState st = scan_row<T, C>(v, a, s, br / group, g * group + br % group, begin, end, lane, lanes_per_key(D), true);
-        write_state<T>(v, a, s.first + br / group, g * group + br % group, cp.part_of(a, range, br / group, g * group + br % group), st, lane);
+        bad &= 0xFFFFFFFFu;
+        while (__builtin_expect(bad != 0, 0)) {
+            const int br = rw + 32 * rt + __builtin_ctzll(bad);
+            bad &= bad - 1;
+            const int bi = br / group, bh = g * group + br % group;
+            const RowState st = scan_row<T, C>(v, a, s, bi, bh, begin, end, lane, lanes_per_key(D), true);
+            write_state<T>(v, a, s.first + bi, bh, cp.part_of(a, range, bi, bh), st, lane);
+        }
     }
 }
 
@@ -963,6 +993,9 @@ bool matrix_operands(const View& v, const qmm_paged_query& in) {
     const uint64_t rows = static_cast<uint64_t>(in.q_token | in.q_head | in.out_token | in.out_head);
     const uint64_t ptr = reinterpret_cast<uintptr_t>(v.c.k) | reinterpret_cast<uintptr_t>(v.c.v) | reinterpret_cast<uintptr_t>(in.q) |
                          reinterpret_cast<uintptr_t>(in.out);
+    // 16 slots are within 2^31 bytes of each other
+    for (int64_t slot : {v.c.k_slot, v.c.v_slot})
+        if (slot < 0 || slot >= 1 << 25) return false;
     return els % (v.c.dtype == QMM_DTYPE_E4M3 ? 16 : 8) == 0 && rows % 8 == 0 && ptr % 16 == 0;
 }
 
@@ -1044,11 +1077,11 @@ int launch_matrix(const View& v, const AttnArgs& a, const Plan& p, hipStream_t s
     static std::once_flag once;
     static hipError_t attr = hipSuccess;
     std::call_once(once, [] {
-        attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_tile_kernel<T, C, D>), hipFuncAttributeMaxDynamicSharedMemorySize,
+        attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_tile_kernel<T, C, D, 1>), hipFuncAttributeMaxDynamicSharedMemorySize,
                                    static_cast<int>(G::kLds));
     });
     if (attr != hipSuccess) return launched(attr, "paged attention LDS size");
-    hipLaunchKernelGGL((attention_tile_kernel<T, C, D>), grid, dim3(kThreads), G::kLds, stream, v, a);
+    hipLaunchKernelGGL((attention_tile_kernel<T, C, D, 1>), grid, dim3(kThreads), G::kLds, stream, v, a);
     return QMM_OK;
 }
 
