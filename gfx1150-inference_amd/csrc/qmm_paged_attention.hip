@@ -7,6 +7,7 @@
 // range's maximum (base 2), sum and unnormalised output are joined by a second kernel in the order of the ranges,
 // so a result depends on the call's lengths alone.  How long a range is, every workgroup works out from all
 // sequences' lengths, which only the device knows (plan_call): the host sees no more than the width of the table.
+#include "qmm_device.h"
 #include "qmm_paged.h"
 
 #include <algorithm>
@@ -25,7 +26,7 @@ struct AttnArgs {
     float scale_log2;  // scale * k_scale * log2 e
     float v_scale;
     int kps;           // keys per range of the kernel without a plan
-    int target;        // workgroups that a plan cuts the call into
+    int slots;         // workgroups that a plan cuts the call into: those that run at once
     float* part_o;     // [partial row][D]
     float2* part_ml;   // [partial row]: maximum, sum
 };
@@ -245,20 +246,23 @@ __device__ __forceinline__ uint32_t visible32(const AttnArgs& a, const Span& s, 
 // How a call is cut, from its sequences' lengths; the same in every wave of every workgroup.
 //   steps      64 keys of a 128-row tile, or 128 keys of the one tile of few rows, is a step; a chain's row tiles
 //              see fewer keys than the last one does, so their mean counts;
-//   kps        keys per range: the steps of the whole call over `target` workgroups, so that a long sequence is cut
-//              and a short one beside it is not, whatever the table's width;
+//   ranges     a sequence of S steps a row tile is cut into ceil(S / u) ranges of the same length, u the smallest of
+//              eight lengths from W / slots (W: the steps of the call) to twice that whose workgroups all find a place
+//              (`slots`) at once, W / slots where none does.  So a long sequence is cut and a short one beside it is
+//              not, whatever the table's width;
 //   blocks     (sequence, range, row tile, kv head), kv head fastest, in the sequences' order;
 //   partials   the rows of sequences with more than one range, in the same order.
 template <int kTile, int kStep>
 struct CallPlan {
-    static constexpr int kMinSteps = kTile >= 128 ? 4 : 1;
-    int kps, seq, block;   // block within the sequence
+    static constexpr int kMinSteps = kTile >= 128 ? 4 : 1, kTries = 8;
+    int seq, block;           // block within the sequence
     int rows, tiles, ranges;  // of the sequence: tokens with rows, row tiles
-    int64_t first_part;    // of the sequence, in tokens
+    int keys;                 // per range
+    int64_t first_part;       // of the sequence, in tokens
 
     struct Lane {
-        int rows, tiles, total;
-        int64_t steps;
+        int rows, tiles, steps;  // steps of all keys of a row tile
+        int64_t work;            // mean steps of all row tiles
     };
     static __device__ __forceinline__ Lane lane_of(const View& v, const AttnArgs& a, int b) {
         Lane x{0, 0, 0, 0};
@@ -267,34 +271,53 @@ struct CallPlan {
             const int group = a.in.heads / v.c.kv_heads;
             x.rows = min(s.n, a.in.max_new);
             x.tiles = kTile >= 128 ? (x.rows * group + kTile - 1) / kTile : x.rows > 0;
-            x.total = s.total;
+            x.steps = x.rows > 0 ? max((s.total + kStep - 1) / kStep, 1) : 0;
             const int seen = a.in.mask ? s.total : min(s.total, s.ctx + (s.n + 1) / 2);
-            x.steps = static_cast<int64_t>(max((seen + kStep - 1) / kStep, 1)) * x.tiles;
+            x.work = static_cast<int64_t>(max((seen + kStep - 1) / kStep, 1)) * x.tiles;
         }
         return x;
     }
-    __device__ __forceinline__ int ranges_of(const Lane& x) const { return x.rows > 0 ? max((x.total - 1) / kps + 1, 1) : 0; }
+    static __device__ __forceinline__ int64_t length(int64_t work, int slots, int c) {
+        return max((work * (kTries + c) + kTries * static_cast<int64_t>(slots) - 1) / (kTries * static_cast<int64_t>(slots)), static_cast<int64_t>(kMinSteps));
+    }
+    static __device__ __forceinline__ int ranges_of(const Lane& x, int u) { return (x.steps + u - 1) / u; }
 
     // Finds the sequence of workgroup `at` (kBlock) or the place of sequence `at`; false: none.
     template <bool kBlock>
     __device__ __forceinline__ bool find(const View& v, const AttnArgs& a, int at, int lane) {
         const int kvh = v.c.kv_heads;
-        int64_t steps = 0;
+        // sums over lanes 0 .. batch - 1 (all 64 of a full chunk) meet in lane 0; the lanes past the batch hold 0
+        auto sum = [&](auto t) {
+            for (int o = 1; o < 64 && o < v.c.batch; o <<= 1) t += __shfl_xor(t, o, 64);
+            return __shfl(t, 0, 64);
+        };
+        int64_t work = 0;
         Lane x{};
         for (int b0 = 0; b0 < v.c.batch; b0 += 64) {
             x = lane_of(v, a, b0 + lane);
-            int64_t t = x.steps;
-            for (int o = 1; o < 64 && o < v.c.batch; o <<= 1) t += __shfl_xor(t, o, 64);
-            steps += t;
+            work += sum(x.work);
         }
-        // lanes past the batch hold 0, but the sums above meet only within the next power of two of it
-        steps = __shfl(steps, 0, 64);
-        const int64_t u = max((steps * kvh + a.target - 1) / a.target, static_cast<int64_t>(kMinSteps));
-        kps = static_cast<int>(min(u * kStep, static_cast<int64_t>(1) << 30));
+        work *= kvh;
+        int64_t count[kTries];
+        int u[kTries];
+#pragma unroll
+        for (int c = 0; c < kTries; ++c) {
+            count[c] = 0;
+            u[c] = static_cast<int>(min(length(work, a.slots, c), static_cast<int64_t>(1) << 23));
+        }
+        for (int b0 = 0; b0 < v.c.batch; b0 += 64) {
+            if (v.c.batch > 64) x = lane_of(v, a, b0 + lane);
+#pragma unroll
+            for (int c = 0; c < kTries; ++c) count[c] += sum(min(ranges_of(x, u[c]) * static_cast<int64_t>(x.tiles), static_cast<int64_t>(1) << 40));
+        }
+        int best = u[0];
+#pragma unroll
+        for (int c = kTries - 1; c >= 0; --c)
+            if (count[c] * kvh <= a.slots) best = u[c];
         int64_t blocks = 0, parts = 0;
         for (int b0 = 0; b0 < v.c.batch; b0 += 64) {
             if (v.c.batch > 64) x = lane_of(v, a, b0 + lane);
-            const int n = ranges_of(x);
+            const int n = ranges_of(x, best);
             const int64_t own_blocks = static_cast<int64_t>(n) * x.tiles * kvh, own_parts = n > 1 ? static_cast<int64_t>(n) * x.rows : 0;
             int64_t sb = own_blocks, sp = own_parts;
             for (int o = 1; o < 64 && o < v.c.batch; o <<= 1) {
@@ -313,6 +336,7 @@ struct CallPlan {
                 rows = __shfl(x.rows, hit, 64);
                 tiles = __shfl(x.tiles, hit, 64);
                 ranges = __shfl(n, hit, 64);
+                keys = ranges > 0 ? (__shfl(x.steps, hit, 64) + ranges - 1) / ranges * kStep : kStep;
                 block = static_cast<int>(at - (blocks + __shfl(sb - own_blocks, hit, 64)));
                 first_part = parts + __shfl(sp - own_parts, hit, 64);
                 return true;
@@ -376,7 +400,7 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
     if (!cp.template find<true>(v, a, static_cast<int>(blockIdx.x), lane)) return;
     const int g = __builtin_amdgcn_readfirstlane(cp.block % kvh), range = __builtin_amdgcn_readfirstlane(cp.block / kvh);
     const Span s = span_of(v, a, __builtin_amdgcn_readfirstlane(cp.seq));
-    const int kps = __builtin_amdgcn_readfirstlane(cp.kps);
+    const int kps = __builtin_amdgcn_readfirstlane(cp.keys);
     const int begin = range * kps, end = min(s.total, begin + kps);
     const int n_rows = min(s.n, a.in.max_new) * group;
 
@@ -645,57 +669,48 @@ __device__ __forceinline__ void copy_to_lds(const void* base, uint32_t off, uint
     __asm__ volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
 }
 
-template <class T, class C, int D, int RT>
-__global__ __launch_bounds__(kThreads, D <= 128 && RT == 1 ? 2 : 1) void attention_tile_kernel(View v, AttnArgs a) {
+template <class T, class C, int D>
+__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_tile_kernel(View v, AttnArgs a) {
     using F = Frag<T>;
     using v8 = typename F::v8;
     using G = TileGeom<D>;
     constexpr bool kFp8 = std::is_same_v<C, Fp8>;
-    __shared__ int pages[kWindowPages];
+    __shared__ int has_page[4][4];  // [tile % 4][16 keys], kept where a page of the range is missing
     const int kvh = v.c.kv_heads, group = a.in.heads / kvh;
     const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    CallPlan<kTileRows * RT, kTileKeys> cp;
+    CallPlan<kTileRows, kTileKeys> cp;
     if (!cp.template find<true>(v, a, static_cast<int>(blockIdx.x), lane)) return;
     const int g = __builtin_amdgcn_readfirstlane(cp.block % kvh), rest = __builtin_amdgcn_readfirstlane(cp.block / kvh);
     const int tiles = __builtin_amdgcn_readfirstlane(cp.tiles), tile = rest % tiles, range = rest / tiles;
     const Span s = span_of(v, a, __builtin_amdgcn_readfirstlane(cp.seq));
-    const int kps = __builtin_amdgcn_readfirstlane(cp.kps), begin = range * kps;
-    const int n_rows = min(s.n, a.in.max_new) * group, r0 = tile * kTileRows * RT, rw = r0 + 32 * RT * w;
-    const int last = (min(r0 + kTileRows * RT, n_rows) - 1) / group;
+    const int kps = __builtin_amdgcn_readfirstlane(cp.keys), begin = range * kps;
+    const int n_rows = min(s.n, a.in.max_new) * group, r0 = tile * kTileRows, rw = r0 + 32 * w;
+    const int last = (min(r0 + kTileRows, n_rows) - 1) / group;
     const int n_keys = a.in.mask ? s.total : min(s.total, s.ctx + last + 1);
     const int end = min(n_keys, begin + kps);
-    int i[RT], head[RT];  // of row rw + 32 rt + l32; rows past the last repeat it
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int r = min(rw + 32 * rt + l32, n_rows - 1);
-        i[rt] = r / group;
-        head[rt] = g * group + r % group;
-    }
+    // row rw + l32; rows past the last repeat it
+    const bool row_live = rw + l32 < n_rows;
+    const int r = min(rw + l32, n_rows - 1), i = r / group, head = g * group + r % group;
+    const int64_t part = cp.part_of(a, range, i, head);
     if (begin >= end && range > 0) {  // keys of later rows only
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-            if (rw + 32 * rt + l32 < n_rows && h == 0) a.part_ml[cp.part_of(a, range, i[rt], head[rt])] = float2{-INFINITY, 0.0f};
+        if (row_live && h == 0) a.part_ml[part] = float2{-INFINITY, 0.0f};
         return;
     }
-    int from = begin, until = min(end, begin + kWindow);  // the keys whose pages are staged
-    bool missing = stage_pages(v, s.seq, from, until, pages);
 
     // a negative scale: the same scores from -q and its magnitude
     const float scale = fabsf(a.scale_log2);
-    v8 qf[RT][D / 16];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const T* qrow = static_cast<const T*>(a.in.q) + static_cast<int64_t>(s.first + i[rt]) * a.in.q_token + head[rt] * a.in.q_head + 8 * h;
+    v8 qf[D / 16];
+    {
+        const T* qrow = static_cast<const T*>(a.in.q) + static_cast<int64_t>(s.first + i) * a.in.q_token + head * a.in.q_head + 8 * h;
 #pragma unroll
         for (int db = 0; db < D / 16; ++db) {
-            __builtin_memcpy(&qf[rt][db], __builtin_assume_aligned(qrow + 16 * db, 16), 16);
-            if (a.scale_log2 < 0.0f) qf[rt][db] = -qf[rt][db];
+            __builtin_memcpy(&qf[db], __builtin_assume_aligned(qrow + 16 * db, 16), 16);
+            if (a.scale_log2 < 0.0f) qf[db] = -qf[db];
         }
     }
     const C* kbase = static_cast<const C*>(v.c.k) + g * v.c.k_head;
     const C* vbase = static_cast<const C*>(v.c.v) + g * v.c.v_head;
-    auto page_at = [&](int key) { return pages[(min(key, until - 1) >> v.page_shift) - (from >> v.page_shift)]; };  // past the end: the last page
 
     // piece 64 j + lane of the wave's 16 rows
     uint32_t k_off[G::kPieces], v_off[G::kPieces];
@@ -707,205 +722,259 @@ __global__ __launch_bounds__(kThreads, D <= 128 && RT == 1 ? 2 : 1) void attenti
     }
     uint16_t* const mine = tile_lds + 16 * w * D;  // of buffer 0's K
     const uint32_t mine_at = __builtin_amdgcn_readfirstlane(reinterpret_cast<uintptr_t>((LdsPtr)mine));
+    const int n_tiles = (end - begin + kTileKeys - 1) / kTileKeys;
+    auto key_of = [&](int t) { return begin + kTileKeys * t + 16 * w; };  // the wave's first key of tile t
+    // Its page's entry of the table; rows of a page past the sequence's end are read and masked.  A vector load: the
+    // LDS reads of a step would wait for a scalar one, whose result is due two steps later.
+    int zero = 0;
+    __asm__("" : "+v"(zero));
+    auto entry = [&](int t) {
+        const int p = min(key_of(t) >> v.page_shift, v.c.table_width - 1);
+        return v.c.table[static_cast<int64_t>(s.seq) * v.c.table_stride + (p + zero)];
+    };
+    auto usable = [&](int id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(v.c.num_pages); };
+    auto page = [&](int id) {
+        const int u = __builtin_amdgcn_readfirstlane(id);
+        return static_cast<int64_t>(usable(u) ? u : 0);
+    };
+    bool missing = false;  // does the range miss a page?
     u32x2 kr[kFp8 ? G::kPieces : 1], vr[kFp8 ? G::kPieces : 1];
-    auto load = [&](int kb, int buf) {
-        const int key = kb + 16 * w, slot = key & (v.c.page_size - 1);
-        const int64_t page = max(__builtin_amdgcn_readfirstlane(page_at(key)), 0);
-        const C* kp = kbase + page * v.c.k_page + slot * v.c.k_slot;
-        const C* vp = vbase + page * v.c.v_page + slot * v.c.v_slot;
+    auto load_k = [&](int t, int id) {
+        const C* p = kbase + page(id) * v.c.k_page + (key_of(t) & (v.c.page_size - 1)) * v.c.k_slot;
 #pragma unroll
         for (int j = 0; j < G::kPieces; ++j) {
-            if constexpr (kFp8) {
-                kr[j] = *reinterpret_cast<const u32x2*>(reinterpret_cast<const char*>(kp) + k_off[j]);
-                vr[j] = *reinterpret_cast<const u32x2*>(reinterpret_cast<const char*>(vp) + v_off[j]);
-            } else {
-                copy_to_lds(kp, k_off[j], mine_at + 2 * (buf * G::kBuf) + 1024 * j);
-                copy_to_lds(vp, v_off[j], mine_at + 2 * (buf * G::kBuf + G::kTileE) + 1024 * j);
-            }
+            if constexpr (kFp8) kr[j] = *reinterpret_cast<const u32x2*>(reinterpret_cast<const char*>(p) + k_off[j]);
+            else copy_to_lds(p, k_off[j], mine_at + 2 * ((t & 1) * G::kBuf) + 1024 * j);
         }
     };
-    // the wave's part of the tile is in LDS afterwards, zeros for the values of rows that nobody sees
-    auto land = [&](int kb, int buf) {
-        uint16_t* sk = mine + buf * G::kBuf + 8 * lane;
-        uint16_t* sv = sk + G::kTileE;
-        if constexpr (kFp8) {
-            auto wide = [](u32x2 x) { return u32x4{F::from_fp8(x[0]), F::from_fp8_hi(x[0]), F::from_fp8(x[1]), F::from_fp8_hi(x[1])}; };
+    auto load_v = [&](int t, int id) {
+        const C* p = vbase + page(id) * v.c.v_page + (key_of(t) & (v.c.page_size - 1)) * v.c.v_slot;
 #pragma unroll
-            for (int j = 0; j < G::kPieces; ++j) {
-                *reinterpret_cast<u32x4*>(sk + 512 * j) = wide(kr[j]);
-                *reinterpret_cast<u32x4*>(sv + 512 * j) = wide(vr[j]);
-            }
-        } else {
-            __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        for (int j = 0; j < G::kPieces; ++j) {
+            if constexpr (kFp8) vr[j] = *reinterpret_cast<const u32x2*>(reinterpret_cast<const char*>(p) + v_off[j]);
+            else copy_to_lds(p, v_off[j], mine_at + 2 * ((t & 1) * G::kBuf + G::kTileE) + 1024 * j);
         }
-        if (kb + kTileKeys > s.total || missing) {
-            const int key = kb + 16 * w;
-            const bool none = page_at(key) < 0;
+    };
+    auto wide = [](u32x2 x) { return u32x4{F::from_fp8(x[0]), F::from_fp8_hi(x[0]), F::from_fp8(x[1]), F::from_fp8_hi(x[1])}; };
+    auto land_k = [&](int t) {
+        if constexpr (kFp8)
+#pragma unroll
+            for (int j = 0; j < G::kPieces; ++j) *reinterpret_cast<u32x4*>(mine + (t & 1) * G::kBuf + 8 * lane + 512 * j) = wide(kr[j]);
+    };
+    // zeros for the values of rows that nobody sees, which may hold anything
+    auto land_v = [&](int t, int id) {
+        uint16_t* sv = mine + (t & 1) * G::kBuf + G::kTileE + 8 * lane;
+        if constexpr (kFp8) {
+#pragma unroll
+            for (int j = 0; j < G::kPieces; ++j) *reinterpret_cast<u32x4*>(sv + 512 * j) = wide(vr[j]);
+        } else {
+            __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");  // and the keys'
+        }
+        if (key_of(t) + 16 > s.total || missing || t == 0) {  // tile 0 lands before `missing` is known
 #pragma unroll
             for (int j = 0; j < G::kPieces; ++j)
-                if (none || key + (64 * j + lane) / G::kChunks >= s.total) *reinterpret_cast<u32x4*>(sv + 512 * j) = u32x4{0, 0, 0, 0};
+                if (!usable(id) || key_of(t) + (64 * j + lane) / G::kChunks >= s.total) *reinterpret_cast<u32x4*>(sv + 512 * j) = u32x4{0, 0, 0, 0};
         }
     };
 
-    f32x16 o[RT][D / 32];
-    float m_run[RT], l_run[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        m_run[rt] = -INFINITY;
-        l_run[rt] = 0.0f;
-#pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[rt][dt][e] = 0.0f;
-    }
     // fragment addresses within a buffer: key row l32, piece 2 db + h; and, of the lane's 16, key 4 h + lane / 4, dims
     // 16 (l32 / 16) + 4 (lane % 4) of every 32
     const int kx = h ^ G::swap_k(l32);
     const uint16_t* k_row = tile_lds + l32 * D;
     const int vrow = 4 * h + ((lane & 15) >> 2), vx = (2 * (l32 >> 4) + ((lane & 3) >> 1)) ^ G::swap_v(vrow);
     const uint16_t* v_row = tile_lds + G::kTileE + vrow * D + 4 * (lane & 1);
-    const bool live = rw < n_rows;  // waves without rows only stage
-    if (begin < end) {
-        load(begin, 0);
-        land(begin, 0);
-    }
-    __syncthreads();
-    // which 16 keys of a tile have their page
-    auto bits_at = [&](int kb) {
-        uint32_t b = 0;
+
+    f32x16 o[D / 32];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) b |= (page_at(kb + 16 * e) >= 0 ? 1u : 0u) << e;
-        return b;
-    };
-    uint32_t page_bits = 15;
-    for (int kb = begin, buf = 0; kb < end; kb += kTileKeys, buf ^= 1) {
-        const bool more = kb + kTileKeys < end;
-        const bool was_missing = missing;
-        if (missing) page_bits = bits_at(kb);
-        if (more) {
-            if (kb + kTileKeys >= until) {  // every wave is past its last use of the old pages: the loop's barrier, bits_at
-                __syncthreads();
-                from = until;
-                until = min(end, from + kWindow);
-                missing = stage_pages(v, s.seq, from, until, pages);
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
+    float m_run = -INFINITY, l_run = 0.0f;
+    const bool live = rw < n_rows;  // waves without rows only stage
+
+    // register e of half hh is key 32 hh + 8 (e / 4) + 4 h + e % 4 of row l32
+    auto scores = [&](int t, f32x16 (&x)[2]) {
+        const uint16_t* sk = k_row + (t & 1) * G::kBuf;
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[hh][e] = 0.0f;
+#pragma unroll
+            for (int db = 0; db < D / 16; ++db) {
+                v8 kf;
+                __builtin_memcpy(&kf, __builtin_assume_aligned(sk + 32 * hh * D + 8 * ((2 * db) ^ kx), 16), 16);
+                x[hh] = F::mma32(kf, qf[db], x[hh]);
             }
-            load(kb + kTileKeys, buf ^ 1);
+        }
+    };
+    // Tile t, whose scores are in x, while the scores of the next are formed in y.  Its keys are two tiles ahead
+    // of the copies, its values one.
+    auto step = [&](int t, f32x16 (&x)[2], f32x16 (&y)[2], int& id1, int& id2) {
+        const int id3 = entry(t + 3);
+        if (t + 1 < n_tiles) load_v(t + 1, id1);
+        if (t + 2 < n_tiles) {
+            load_k(t + 2, id2);
+            if (missing && lane == 0) has_page[(t + 2) & 3][w] = usable(id2);
         }
         if (live) {
-            const bool full = kb + kTileKeys <= s.ctx && kb + kTileKeys <= end && !was_missing;
+            const int kb = begin + kTileKeys * t;
+            if (kb + kTileKeys > s.ctx || kb + kTileKeys > end || missing) {
 #pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-                // register e is key 32 hh + 8 (e / 4) + 4 h + e % 4 of row l32
-                f32x16 x[RT];
+                for (int hh = 0; hh < 2; ++hh) {
+                    uint32_t vis = visible32(a, s, i, kb + 32 * hh);
+                    if (missing) {
+                        if (!has_page[t & 3][2 * hh]) vis &= 0xFFFF0000u;
+                        if (!has_page[t & 3][2 * hh + 1]) vis &= 0x0000FFFFu;
+                    }
+                    vis >>= 4 * h;
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) x[rt][e] = 0.0f;
-#pragma unroll
-                for (int db = 0; db < D / 16; ++db) {
-                    v8 kf;
-                    __builtin_memcpy(&kf, __builtin_assume_aligned(k_row + buf * G::kBuf + 32 * hh * D + 8 * ((2 * db) ^ kx), 16), 16);
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) x[rt] = F::mma32(kf, qf[rt][db], x[rt]);
+                    for (int e = 0; e < 16; ++e)
+                        if (!((vis >> (8 * (e >> 2) + (e & 3))) & 1)) x[hh][e] = -INFINITY;
                 }
-                v8 pf[RT][2];
+            }
+            float mx = x[0][0];
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    if (!full) {
-                        uint32_t vis = visible32(a, s, i[rt], kb + 32 * hh);
-                        if (was_missing) {
-                            if (!((page_bits >> (2 * hh)) & 1)) vis &= 0xFFFF0000u;
-                            if (!((page_bits >> (2 * hh)) & 2)) vis &= 0x0000FFFFu;
-                        }
-                        vis >>= 4 * h;
+            for (int e = 1; e < 32; ++e) mx = fmaxf(mx, x[e >> 4][e & 15]);
+            mx *= scale;
+            if (__ballot(mx > m_run + kSlack) != 0) {
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                const float mn = fmaxf(m_run, mx);
+                const float f = m_run == mn ? 1.0f : __builtin_amdgcn_exp2f(m_run - mn);
+                l_run *= f;
 #pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            if (!((vis >> (8 * (e >> 2) + (e & 3))) & 1)) x[rt][e] = -INFINITY;
-                    }
-                    float mx = x[rt][0];
+                for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-                    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, x[rt][e]);
-                    mx *= scale;
-                    if (__ballot(mx > m_run[rt] + kSlack) != 0) {
-                        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-                        const float mn = fmaxf(m_run[rt], mx);
-                        const float f = m_run[rt] == mn ? 1.0f : __builtin_amdgcn_exp2f(m_run[rt] - mn);
-                        l_run[rt] *= f;
+                    for (int e = 0; e < 16; ++e) o[dt][e] *= f;
+                m_run = mn;
+            }
+            const float base = m_run == -INFINITY ? 0.0f : m_run - kShift;
+            // The next tile's scores (past the last tile: of stale keys, unused), this tile's weights and its second
+            // product, in steps of one matrix instruction whose order the compiler keeps: left alone, it lets every
+            // product wait for its own LDS read and the weights wait for the products.  Fragments are read kAhead
+            // products ahead; a third of the weights is left for the second product's steps.
+            constexpr int kM = D / 8, kPerB = D / 32, kAhead = 4;
+            const uint16_t* sk = k_row + ((t + 1) & 1) * G::kBuf;
+            const uint16_t* sv = v_row + (t & 1) * G::kBuf;
+            v8 kf[kM], vf[kM], pf[4];
+            auto read_k = [&](int n) {
+                __builtin_memcpy(&kf[n], __builtin_assume_aligned(sk + 32 * (n & 1) * D + 8 * ((2 * (n >> 1)) ^ kx), 16), 16);
+            };
+            auto read_v = [&](int n) {
+                const uint16_t* at = sv + 16 * (n / kPerB) * D + 8 * ((4 * (n % kPerB)) ^ vx);
+                const s16x4 f0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+                const s16x4 f1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 8 * D));
+                vf[n] = __builtin_bit_cast(v8, __builtin_shufflevector(f0, f1, 0, 1, 2, 3, 4, 5, 6, 7));
+            };
+            auto weight = [&](int e) {
+                const float p = __builtin_amdgcn_exp2f(__fmaf_rn(x[e >> 4][e & 15], scale, -base));
+                l_run += p;
+                pf[e >> 3][e & 7] = static_cast<T>(p);
+            };
+            constexpr int kFirst = 20;  // weights beside the first product
 #pragma unroll
-                        for (int dt = 0; dt < D / 32; ++dt)
+            for (int n = 0; n < kAhead; ++n) read_k(n);
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) o[rt][dt][e] *= f;
-                        m_run[rt] = mn;
-                    }
-                    const float base = m_run[rt] == -INFINITY ? 0.0f : m_run[rt] - kShift;
+            for (int n = 0; n < kM; ++n) {
+                if (n + kAhead < kM) read_k(n + kAhead);
+                else read_v(n + kAhead - kM);
+                if (n < 2)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float p = __builtin_amdgcn_exp2f(__fmaf_rn(x[rt][e], scale, -base));
-                        l_run[rt] += p;
-                        pf[rt][e >> 3][e & 7] = static_cast<T>(p);
-                    }
-                }
+                    for (int e = 0; e < 16; ++e) y[n][e] = 0.0f;
+                y[n & 1] = F::mma32(kf[n], qf[n >> 1], y[n & 1]);
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+                for (int e = kFirst * n / kM; e < kFirst * (n + 1) / kM; ++e) weight(e);
+                __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
-                    for (int dt = 0; dt < D / 32; ++dt) {
-                        const uint16_t* at = v_row + buf * G::kBuf + (32 * hh + 16 * b) * D + 8 * ((4 * dt) ^ vx);
-                        const s16x4 f0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
-                        const s16x4 f1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 8 * D));
-                        const v8 vf = __builtin_bit_cast(v8, __builtin_shufflevector(f0, f1, 0, 1, 2, 3, 4, 5, 6, 7));
+            for (int n = 0; n < kM; ++n) {
+                if (n + kAhead < kM) read_v(n + kAhead);
+                o[n % kPerB] = F::mma32(vf[n], pf[n / kPerB], o[n % kPerB]);
 #pragma unroll
-                        for (int rt = 0; rt < RT; ++rt) o[rt][dt] = F::mma32(vf, pf[rt][b], o[rt][dt]);
-                    }
+                for (int e = kFirst + (32 - kFirst) * 2 * n / kM; e < kFirst + (32 - kFirst) * 2 * (n + 1) / kM && e < 32; ++e) weight(e);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
-        if (more) land(kb + kTileKeys, buf ^ 1);
+        if (t + 2 < n_tiles) land_k(t + 2);
+        if (t + 1 < n_tiles) land_v(t + 1, id1);
         __syncthreads();
+        id1 = id2;
+        id2 = id3;
+    };
+
+    if (n_tiles > 0) {
+        int id0 = entry(0), id1 = entry(1), id2 = entry(2);
+        for (int p = (begin >> v.page_shift) + tid; p <= (end - 1) >> v.page_shift; p += kThreads)
+            missing |= page_of(v, s.seq, p << v.page_shift) < 0;
+        load_k(0, id0);
+        load_v(0, id0);
+        if (!kFp8 && n_tiles > 1) load_k(1, id1);
+        land_k(0);
+        land_v(0, id0);
+        missing = __syncthreads_or(missing);
+        if (missing && lane == 0) {
+            has_page[0][w] = usable(id0);
+            has_page[1][w] = usable(id1);
+        }
+        if (kFp8 && n_tiles > 1) load_k(1, id1);
+        f32x16 xa[2], xb[2];
+        if (live) scores(0, xa);
+        if (kFp8 && n_tiles > 1) land_k(1);
+        __syncthreads();
+        for (int t = 0; t < n_tiles; t += 2) {
+            step(t, xa, xb, id1, id2);
+            if (t + 1 < n_tiles) step(t + 1, xb, xa, id1, id2);
+        }
     }
     if (!live) return;
+    l_run += __shfl_xor(l_run, 32, 64);
+    bool nan = false;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const bool row_live = rw + 32 * rt + l32 < n_rows;
-        const int64_t part = cp.part_of(a, range, i[rt], head[rt]);
-        const float l = l_run[rt] + __shfl_xor(l_run[rt], 32, 64);
-        bool nan = false;
+    for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt)
+        for (int e = 0; e < 16; ++e) nan |= o[dt][e] != o[dt][e];
+    uint64_t bad = __ballot(nan && row_live && l_run == l_run);  // as in attention_rows_kernel
+    bad = (bad | bad >> 32) & 0xFFFFFFFFu;
+    // Out through the wave's quarter of LDS (its last tile's barrier is behind every wave), so that a store covers whole rows,
+    // not 16 bytes of each: 16-byte pieces, exchanged by the row's number against bank conflicts.
+    const float inv = part < 0 ? (l_run == 0.0f ? 0.0f : a.v_scale / l_run) : 1.0f;
+    float* mine_f = reinterpret_cast<float*>(tile_lds) + 32 * D * w;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) nan |= o[rt][dt][e] != o[rt][dt][e];
-        uint64_t bad = __ballot(nan && row_live && l == l);  // as in attention_rows_kernel
-        bad |= bad >> 32;
-        if (row_live && !((bad >> l32) & 1)) {
-            if (part < 0) {
-                const float inv = l == 0.0f ? 0.0f : a.v_scale / l;
-                T* out = static_cast<T*>(a.in.out) + static_cast<int64_t>(s.first + i[rt]) * a.in.out_token + head[rt] * a.in.out_head + 4 * h;
+    for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-                for (int dt = 0; dt < D / 32; ++dt)
+        for (int q4 = 0; q4 < 4; ++q4) {
+            const f32x4 x = {o[dt][4 * q4] * inv, o[dt][4 * q4 + 1] * inv, o[dt][4 * q4 + 2] * inv, o[dt][4 * q4 + 3] * inv};
+            *reinterpret_cast<f32x4*>(mine_f + l32 * D + 4 * ((8 * dt + 2 * q4 + h) ^ (l32 & 7))) = x;
+        }
+    wave_lds_sync();
+    if (part >= 0 && row_live && h == 0 && !((bad >> l32) & 1)) a.part_ml[part] = float2{m_run - kShift, l_run};
+    const int n_wave = min(n_rows - rw, 32);
+    if (cp.ranges == 1) {
+        for (int u = lane; u < n_wave * G::kChunks; u += 64) {
+            const int row = u / G::kChunks, c = u % G::kChunks, ri = (rw + row) / group, rh = g * group + (rw + row) % group;
+            if ((bad >> row) & 1) continue;
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(mine_f + row * D + 4 * ((2 * c) ^ (row & 7)));
+            const f32x4 hi = *reinterpret_cast<const f32x4*>(mine_f + row * D + 4 * ((2 * c + 1) ^ (row & 7)));
+            v8 x;
 #pragma unroll
-                    for (int q4 = 0; q4 < 4; ++q4) {
-                        T v4[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) v4[e] = static_cast<T>(o[rt][dt][4 * q4 + e] * inv);
-                        __builtin_memcpy(__builtin_assume_aligned(out + 32 * dt + 8 * q4, 8), v4, 8);
-                    }
-            } else {
-                float* po = a.part_o + part * D + 4 * h;
-#pragma unroll
-                for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-                    for (int q4 = 0; q4 < 4; ++q4)
-                        *reinterpret_cast<f32x4*>(po + 32 * dt + 8 * q4) =
-                            f32x4{o[rt][dt][4 * q4], o[rt][dt][4 * q4 + 1], o[rt][dt][4 * q4 + 2], o[rt][dt][4 * q4 + 3]};
-                if (h == 0) a.part_ml[part] = float2{m_run[rt] - kShift, l};
+            for (int e = 0; e < 4; ++e) {
+                x[e] = static_cast<T>(lo[e]);
+                x[4 + e] = static_cast<T>(hi[e]);
             }
+            *reinterpret_cast<v8*>(static_cast<T*>(a.in.out) + static_cast<int64_t>(s.first + ri) * a.in.out_token + rh * a.in.out_head + 8 * c) = x;
         }
-        bad &= 0xFFFFFFFFu;
-        while (__builtin_expect(bad != 0, 0)) {
-            const int br = rw + 32 * rt + __builtin_ctzll(bad);
-            bad &= bad - 1;
-            const int bi = br / group, bh = g * group + br % group;
-            const RowState st = scan_row<T, C>(v, a, s, bi, bh, begin, end, lane, lanes_per_key(D), true);
-            write_state<T>(v, a, s.first + bi, bh, cp.part_of(a, range, bi, bh), st, lane);
+    } else {
+        for (int u = lane; u < n_wave * (D / 4); u += 64) {
+            const int row = u / (D / 4), c = u % (D / 4), ri = (rw + row) / group, rh = g * group + (rw + row) % group;
+            if ((bad >> row) & 1) continue;
+            *reinterpret_cast<f32x4*>(a.part_o + cp.part_of(a, range, ri, rh) * D + 4 * c) =
+                *reinterpret_cast<const f32x4*>(mine_f + row * D + 4 * (c ^ (row & 7)));
         }
+    }
+    while (__builtin_expect(bad != 0, 0)) {
+        const int br = rw + __builtin_ctzll(bad), bi = br / group, bh = g * group + br % group;
+        bad &= bad - 1;
+        const RowState st = scan_row<T, C>(v, a, s, bi, bh, begin, end, lane, lanes_per_key(D), true);
+        write_state<T>(v, a, s.first + bi, bh, cp.part_of(a, range, bi, bh), st, lane);
     }
 }
 
@@ -979,7 +1048,7 @@ struct Plan {
     Kind kind;
     int row_tiles;      // of 16 rows (kRows)
     int kps, splits;    // kLanes
-    int target;         // the others: workgroups to cut the call into ..
+    int slots;          // the others: workgroups to cut the call into ..
     int64_t blocks;     // .. and what that makes at most
     bool merge;
     int64_t parts;      // partial rows at most
@@ -1018,18 +1087,18 @@ Plan plan(const View& v, const qmm_paged_query& in) {
         p.kind = per_kv <= (v.c.head_dim <= 128 ? 64 : 16) ? Kind::kRows : Kind::kTile;
         const bool few = p.kind == Kind::kRows;
         p.row_tiles = few ? static_cast<int>((per_kv + 15) / 16) : 0;
-        p.target = few ? env_int("T_ROWS", 1024) : env_int("T_TILE", 512);
-        // A plan's ranges are at least `least` keys.  With W steps in all and u = ceil(W / target) steps a range, the
-        // ranges of all row tiles are at most 2 W / u and one more per row tile (a chain's last tile sees up to twice
-        // the mean), and those of sequences with more than one range at most twice that, 4 target.
+        p.slots = few ? env_int("T_ROWS", 768) : env_int("T_TILE", 512);
+        // A plan's ranges are cut by a length of at least `least` keys.  With W steps in all and u >= W / slots steps a
+        // range, the ranges of all row tiles are at most 2 W / u and one more per row tile (a chain's last tile sees up to
+        // twice the mean), and those of sequences with more than one range at most twice that, 4 slots.
         const int64_t least = few ? kRowsStep : kTileKeys * CallPlan<kTileRows, kTileKeys>::kMinSteps;
         const int64_t most_ranges = (most + least - 1) / least;
         const int64_t seqs = std::min(v.c.batch, in.tokens);
         const int64_t items = kvh * (few ? seqs : seqs + (static_cast<int64_t>(in.tokens) * (in.heads / kvh) + kTileRows - 1) / kTileRows);
-        p.blocks = std::min(items * most_ranges, 2 * static_cast<int64_t>(p.target) + items);
+        p.blocks = std::min(items * most_ranges, 2 * static_cast<int64_t>(p.slots) + items);
         p.merge = most_ranges > 1;
         const int64_t tile_rows = few ? 16 * p.row_tiles : kTileRows;
-        p.parts = std::min(rows * most_ranges, 4 * p.target * tile_rows);
+        p.parts = std::min(rows * most_ranges, 4 * static_cast<int64_t>(p.slots) * tile_rows);
     }
     if (p.merge) {
         p.o_bytes = static_cast<size_t>(p.parts) * v.c.head_dim * sizeof(float);
@@ -1077,11 +1146,11 @@ int launch_matrix(const View& v, const AttnArgs& a, const Plan& p, hipStream_t s
     static std::once_flag once;
     static hipError_t attr = hipSuccess;
     std::call_once(once, [] {
-        attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_tile_kernel<T, C, D, 1>), hipFuncAttributeMaxDynamicSharedMemorySize,
+        attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_tile_kernel<T, C, D>), hipFuncAttributeMaxDynamicSharedMemorySize,
                                    static_cast<int>(G::kLds));
     });
     if (attr != hipSuccess) return launched(attr, "paged attention LDS size");
-    hipLaunchKernelGGL((attention_tile_kernel<T, C, D, 1>), grid, dim3(kThreads), G::kLds, stream, v, a);
+    hipLaunchKernelGGL((attention_tile_kernel<T, C, D>), grid, dim3(kThreads), G::kLds, stream, v, a);
     return QMM_OK;
 }
 
@@ -1107,7 +1176,7 @@ int tree_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, void* work
     a.scale_log2 = scale * v.c.k_scale * 1.4426950408889634f;
     a.v_scale = v.c.v_scale;
     a.kps = p.kps;
-    a.target = p.target;
+    a.slots = p.slots;
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + p.o_bytes);
     const bool fp8 = v.c.dtype == QMM_DTYPE_E4M3;
