@@ -12,6 +12,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <map>
 #include <mutex>
 #include <type_traits>
 
@@ -29,6 +30,7 @@ struct AttnArgs {
     int slots;         // workgroups that a plan cuts the call into: those that run at once
     float* part_o;     // [partial row][D]
     float2* part_ml;   // [partial row]: maximum, sum
+    int4* cut;         // [token]: ranges, its first partial row and the rows between ranges, in tokens
 };
 
 // The new tokens of one sequence.
@@ -247,108 +249,106 @@ __device__ __forceinline__ uint32_t visible32(const AttnArgs& a, const Span& s, 
 //   steps      64 keys of a 128-row tile, or 128 keys of the one tile of few rows, is a step; a chain's row tiles
 //              see fewer keys than the last one does, so their mean counts;
 //   ranges     a sequence of S steps a row tile is cut into ceil(S / u) ranges of the same length, u the smallest of
-//              eight lengths from W / slots (W: the steps of the call) to twice that whose workgroups all find a place
+//              four lengths from W / slots (W: the steps of the call) to 1.75 times that whose workgroups all find a place
 //              (`slots`) at once, W / slots where none does.  So a long sequence is cut and a short one beside it is
 //              not, whatever the table's width;
 //   blocks     (sequence, range, row tile, kv head), kv head fastest, in the sequences' order;
 //   partials   the rows of sequences with more than one range, in the same order.
 template <int kTile, int kStep>
 struct CallPlan {
-    static constexpr int kMinSteps = kTile >= 128 ? 4 : 1, kTries = 8;
+    static constexpr int kMinSteps = kTile >= 128 ? 4 : 1, kTries = 4;
     int seq, block;           // block within the sequence
     int rows, tiles, ranges;  // of the sequence: tokens with rows, row tiles
     int keys;                 // per range
-    int64_t first_part;       // of the sequence, in tokens
+    int first_part;           // of the sequence, in tokens
 
     struct Lane {
         int rows, tiles, steps;  // steps of all keys of a row tile
-        int64_t work;            // mean steps of all row tiles
+        float work;              // mean steps of all row tiles
     };
     static __device__ __forceinline__ Lane lane_of(const View& v, const AttnArgs& a, int b) {
-        Lane x{0, 0, 0, 0};
+        Lane x{0, 0, 0, 0.0f};
         if (b < v.c.batch) {
             const Span s = span_of(v, a, b);
-            const int group = a.in.heads / v.c.kv_heads;
             x.rows = min(s.n, a.in.max_new);
-            x.tiles = kTile >= 128 ? (x.rows * group + kTile - 1) / kTile : x.rows > 0;
+            x.tiles = kTile >= 128 ? (x.rows * (a.in.heads / v.c.kv_heads) + kTile - 1) / kTile : x.rows > 0;
             x.steps = x.rows > 0 ? max((s.total + kStep - 1) / kStep, 1) : 0;
             const int seen = a.in.mask ? s.total : min(s.total, s.ctx + (s.n + 1) / 2);
-            x.work = static_cast<int64_t>(max((seen + kStep - 1) / kStep, 1)) * x.tiles;
+            x.work = static_cast<float>(max((seen + kStep - 1) / kStep, 1)) * static_cast<float>(x.tiles);
         }
         return x;
     }
-    static __device__ __forceinline__ int64_t length(int64_t work, int slots, int c) {
-        return max((work * (kTries + c) + kTries * static_cast<int64_t>(slots) - 1) / (kTries * static_cast<int64_t>(slots)), static_cast<int64_t>(kMinSteps));
-    }
-    static __device__ __forceinline__ int ranges_of(const Lane& x, int u) { return (x.steps + u - 1) / u; }
 
-    // Finds the sequence of workgroup `at` (kBlock) or the place of sequence `at`; false: none.
-    template <bool kBlock>
+    // Finds the sequence of workgroup `at`; false: there is none.  Lengths and counts of workgroups are compared in fp32,
+    // whose roundings are the same everywhere.
     __device__ __forceinline__ bool find(const View& v, const AttnArgs& a, int at, int lane) {
         const int kvh = v.c.kv_heads;
         // sums over lanes 0 .. batch - 1 (all 64 of a full chunk) meet in lane 0; the lanes past the batch hold 0
-        auto sum = [&](auto t) {
+        auto sum = [&](float t) {
             for (int o = 1; o < 64 && o < v.c.batch; o <<= 1) t += __shfl_xor(t, o, 64);
             return __shfl(t, 0, 64);
         };
-        int64_t work = 0;
+        float work = 0.0f;
         Lane x{};
         for (int b0 = 0; b0 < v.c.batch; b0 += 64) {
             x = lane_of(v, a, b0 + lane);
             work += sum(x.work);
         }
-        work *= kvh;
-        int64_t count[kTries];
+        // 1e-5 covers the roundings: a length is never below W / slots
+        const float shortest = work * static_cast<float>(kvh) / static_cast<float>(a.slots) * 1.00001f;
         int u[kTries];
+        float count[kTries];
 #pragma unroll
         for (int c = 0; c < kTries; ++c) {
-            count[c] = 0;
-            u[c] = static_cast<int>(min(length(work, a.slots, c), static_cast<int64_t>(1) << 23));
+            u[c] = max(static_cast<int>(fminf(ceilf(shortest * (1.0f + 0.25f * static_cast<float>(c))), 8388608.0f)), kMinSteps);
+            count[c] = 0.0f;
         }
+        auto ranges_of = [&](int steps, int len) { return static_cast<int>((static_cast<uint32_t>(steps) + len - 1) / static_cast<uint32_t>(len)); };
         for (int b0 = 0; b0 < v.c.batch; b0 += 64) {
             if (v.c.batch > 64) x = lane_of(v, a, b0 + lane);
 #pragma unroll
-            for (int c = 0; c < kTries; ++c) count[c] += sum(min(ranges_of(x, u[c]) * static_cast<int64_t>(x.tiles), static_cast<int64_t>(1) << 40));
+            for (int c = 0; c < kTries; ++c) count[c] += sum(static_cast<float>(ranges_of(x.steps, u[c])) * static_cast<float>(x.tiles));
         }
         int best = u[0];
 #pragma unroll
         for (int c = kTries - 1; c >= 0; --c)
-            if (count[c] * kvh <= a.slots) best = u[c];
-        int64_t blocks = 0, parts = 0;
+            if (count[c] * static_cast<float>(kvh) <= static_cast<float>(a.slots)) best = u[c];
+        int blocks = 0, parts = 0;
         for (int b0 = 0; b0 < v.c.batch; b0 += 64) {
             if (v.c.batch > 64) x = lane_of(v, a, b0 + lane);
-            const int n = ranges_of(x, best);
-            const int64_t own_blocks = static_cast<int64_t>(n) * x.tiles * kvh, own_parts = n > 1 ? static_cast<int64_t>(n) * x.rows : 0;
-            int64_t sb = own_blocks, sp = own_parts;
+            const int n = ranges_of(x.steps, best);
+            const int own_blocks = n * x.tiles * kvh, own_parts = n > 1 ? n * x.rows : 0;
+            int sb = own_blocks, sp = own_parts;
             for (int o = 1; o < 64 && o < v.c.batch; o <<= 1) {
-                const int64_t ub = __shfl_up(sb, o, 64), up = __shfl_up(sp, o, 64);
+                const int ub = __shfl_up(sb, o, 64), up = __shfl_up(sp, o, 64);
                 if (lane >= o) {
                     sb += ub;
                     sp += up;
                 }
             }
             const int here = min(v.c.batch - b0, 64);
-            int hit;
-            if constexpr (kBlock) hit = static_cast<int>(__popcll(__ballot(lane < here && blocks + sb <= at)));
-            else hit = at - b0;
-            if (hit >= 0 && hit < here) {
+            const int hit = static_cast<int>(__popcll(__ballot(lane < here && blocks + sb <= at)));
+            if (hit < here) {
+                auto of = [&](int t) { return __builtin_amdgcn_readlane(t, hit); };
                 seq = b0 + hit;
-                rows = __shfl(x.rows, hit, 64);
-                tiles = __shfl(x.tiles, hit, 64);
-                ranges = __shfl(n, hit, 64);
-                keys = ranges > 0 ? (__shfl(x.steps, hit, 64) + ranges - 1) / ranges * kStep : kStep;
-                block = static_cast<int>(at - (blocks + __shfl(sb - own_blocks, hit, 64)));
-                first_part = parts + __shfl(sp - own_parts, hit, 64);
+                rows = of(x.rows);
+                tiles = of(x.tiles);
+                ranges = of(n);
+                keys = (of(x.steps) + ranges - 1) / ranges * kStep;
+                block = at - (blocks + of(sb - own_blocks));
+                first_part = parts + of(sp - own_parts);
                 return true;
             }
-            blocks += __shfl(sb, here - 1, 64);
-            parts += __shfl(sp, here - 1, 64);
+            blocks += __builtin_amdgcn_readlane(sb, here - 1);
+            parts += __builtin_amdgcn_readlane(sp, here - 1);
         }
         return false;
     }
     __device__ __forceinline__ int64_t part_of(const AttnArgs& a, int range, int i, int head) const {
         return ranges == 1 ? -1 : (first_part + static_cast<int64_t>(range) * rows + i) * a.in.heads + head;
     }
+    // what the join needs to know of token i of the sequence
+    __device__ __forceinline__ int4 cut_of(int i) const { return int4{ranges, first_part + i, rows, 0}; }
 };
 
 // Page ids of the rows [begin, end) into LDS; true if one of them is missing.
@@ -397,12 +397,13 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
     const int lane = threadIdx.x & 63, l = lane & 15, q = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     CallPlan<16, kRowsStep> cp;
-    if (!cp.template find<true>(v, a, static_cast<int>(blockIdx.x), lane)) return;
-    const int g = __builtin_amdgcn_readfirstlane(cp.block % kvh), range = __builtin_amdgcn_readfirstlane(cp.block / kvh);
-    const Span s = span_of(v, a, __builtin_amdgcn_readfirstlane(cp.seq));
-    const int kps = __builtin_amdgcn_readfirstlane(cp.keys);
+    if (!cp.find(v, a, static_cast<int>(blockIdx.x), lane)) return;
+    const int g = cp.block % kvh, range = cp.block / kvh;
+    const Span s = span_of(v, a, cp.seq);
+    const int kps = cp.keys;
     const int begin = range * kps, end = min(s.total, begin + kps);
-    const int n_rows = min(s.n, a.in.max_new) * group;
+    const int n_rows = cp.rows * group;
+    if (g == 0 && range == 0 && a.cut && static_cast<int>(threadIdx.x) < cp.rows) a.cut[s.first + threadIdx.x] = cp.cut_of(threadIdx.x);
 
     // queries: rows past the last repeat it
     v8 qf[NT][kF];
@@ -680,13 +681,15 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_tile_ker
     const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     CallPlan<kTileRows, kTileKeys> cp;
-    if (!cp.template find<true>(v, a, static_cast<int>(blockIdx.x), lane)) return;
-    const int g = __builtin_amdgcn_readfirstlane(cp.block % kvh), rest = __builtin_amdgcn_readfirstlane(cp.block / kvh);
-    const int tiles = __builtin_amdgcn_readfirstlane(cp.tiles), tile = rest % tiles, range = rest / tiles;
-    const Span s = span_of(v, a, __builtin_amdgcn_readfirstlane(cp.seq));
-    const int kps = __builtin_amdgcn_readfirstlane(cp.keys), begin = range * kps;
-    const int n_rows = min(s.n, a.in.max_new) * group, r0 = tile * kTileRows, rw = r0 + 32 * w;
+    if (!cp.find(v, a, static_cast<int>(blockIdx.x), lane)) return;
+    const int g = cp.block % kvh, rest = cp.block / kvh;
+    const int tiles = cp.tiles, tile = rest % tiles, range = rest / tiles;
+    const Span s = span_of(v, a, cp.seq);
+    const int kps = cp.keys, begin = range * kps;
+    const int n_rows = cp.rows * group, r0 = tile * kTileRows, rw = r0 + 32 * w;
     const int last = (min(r0 + kTileRows, n_rows) - 1) / group;
+    if (g == 0 && range == 0 && a.cut)
+        for (int t = r0 / group + tid; t <= last; t += kThreads) a.cut[s.first + t] = cp.cut_of(t);
     const int n_keys = a.in.mask ? s.total : min(s.total, s.ctx + last + 1);
     const int end = min(n_keys, begin + kps);
     // row rw + l32; rows past the last repeat it
@@ -980,28 +983,23 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_tile_ker
 
 // Joins the ranges of each row in their order: D / 4 threads a row, 4 ranges requested at once.
 // Block (x, y): token, heads.
-template <class T, int kTile, int kStep>
+template <class T, bool kPlanned>
 __global__ __launch_bounds__(kThreads) void attention_merge_kernel(View v, AttnArgs a) {
     const int t = blockIdx.x, D = v.c.head_dim, per = D / 4, rows = kThreads / per, lane = threadIdx.x & 63;
+    int4 cut = {0, 0, 0, 0};
+    if constexpr (kPlanned) cut = a.cut[t];  // not written for a token of no sequence, or past max_new
     const int seq = sequence_of(v, t, lane);
     if (seq >= v.c.batch || t < v.c.cu[seq]) return;
-    int n;
-    int64_t row, step;  // the first range's partial row of head 0, rows between ranges
-    if constexpr (kTile > 0) {
-        CallPlan<kTile, kStep> cp;
-        cp.template find<false>(v, a, seq, lane);
-        const int i = t - max(v.c.cu[seq], 0);
-        if (cp.ranges <= 1 || i >= cp.rows) return;  // written by the range itself
-        n = cp.ranges;
-        row = cp.part_of(a, 0, i, 0);
-        step = static_cast<int64_t>(cp.rows) * a.in.heads;
+    if constexpr (kPlanned) {
+        if (t - max(v.c.cu[seq], 0) >= a.in.max_new) return;
     } else {
         const Span s = span_of(v, a, seq);
-        if (s.total <= a.kps) return;
-        n = (s.total + a.kps - 1) / a.kps;
-        row = static_cast<int64_t>(t) * a.in.heads;
-        step = static_cast<int64_t>(a.in.tokens) * a.in.heads;
+        cut = int4{(s.total + a.kps - 1) / a.kps, t, a.in.tokens, 0};
     }
+    if (cut.x <= 1) return;  // written by the range itself
+    const int n = cut.x;
+    int64_t row = static_cast<int64_t>(cut.y) * a.in.heads;
+    const int64_t step = static_cast<int64_t>(cut.z) * a.in.heads;  // between ranges
     const int slot = threadIdx.x / per, d0 = 4 * (threadIdx.x % per), head = blockIdx.y * rows + slot;
     if (slot >= rows || head >= a.in.heads) return;
     row += head;
@@ -1041,7 +1039,6 @@ __global__ __launch_bounds__(kThreads) void attention_merge_kernel(View v, AttnA
 }
 
 // ---- host side -------------------------------------------------------------------------------
-int env_int(const char* n, int d) { const char* e = getenv(n); return e ? atoi(e) : d; }
 // Which kernel serves a call, by the rows (tokens x query heads) that share a kv head, and how its keys are cut.
 enum class Kind { kLanes, kRows, kTile };
 struct Plan {
@@ -1052,7 +1049,7 @@ struct Plan {
     int64_t blocks;     // .. and what that makes at most
     bool merge;
     int64_t parts;      // partial rows at most
-    size_t o_bytes, bytes;
+    size_t o_bytes, ml_bytes, bytes;
 };
 
 bool matrix_operands(const View& v, const qmm_paged_query& in) {
@@ -1066,6 +1063,53 @@ bool matrix_operands(const View& v, const qmm_paged_query& in) {
     for (int64_t slot : {v.c.k_slot, v.c.v_slot})
         if (slot < 0 || slot >= 1 << 25) return false;
     return els % (v.c.dtype == QMM_DTYPE_E4M3 ? 16 : 8) == 0 && rows % 8 == 0 && ptr % 16 == 0;
+}
+
+// Calls f with the kernel that serves a plan's kind, row tiles and the call's types.
+template <class T, class C, int D, class Fn>
+auto with_matrix_kernel(Kind kind, int row_tiles, Fn f) {
+    if (kind == Kind::kTile) return f(attention_tile_kernel<T, C, D>, TileGeom<D>::kLds);
+    if constexpr (D <= 128) {
+        if (row_tiles == 2) return f(attention_rows_kernel<T, C, D, 2>, size_t{0});
+        if (row_tiles > 2) return f(attention_rows_kernel<T, C, D, 4>, size_t{0});
+    }
+    return f(attention_rows_kernel<T, C, D, 1>, size_t{0});
+}
+
+template <class Fn>
+auto with_matrix_kernel(const View& v, const qmm_paged_query& in, Kind kind, int row_tiles, Fn f) {
+    auto types = [&](auto tc, auto cc) {
+        using T = decltype(tc);
+        using C = decltype(cc);
+        switch (v.c.head_dim) {
+            case 64: return with_matrix_kernel<T, C, 64>(kind, row_tiles, f);
+            case 96: return with_matrix_kernel<T, C, 96>(kind, row_tiles, f);
+            case 128: return with_matrix_kernel<T, C, 128>(kind, row_tiles, f);
+            default: return with_matrix_kernel<T, C, 256>(kind, row_tiles, f);
+        }
+    };
+    const bool fp8 = v.c.dtype == QMM_DTYPE_E4M3;
+    if (in.dtype == QMM_DTYPE_F16) return fp8 ? types(_Float16{}, Fp8{}) : types(_Float16{}, _Float16{});
+    return fp8 ? types(__bf16{}, Fp8{}) : types(__bf16{}, __bf16{});
+}
+
+// Workgroups of a kernel that run at once, asked for once per kernel (every device is the same chip).
+template <class K>
+int kernel_slots(K kern, size_t lds) {
+    static std::mutex mu;
+    static std::map<const void*, int> known;
+    const void* key = reinterpret_cast<const void*>(kern);
+    std::lock_guard<std::mutex> lock(mu);
+    const auto it = known.find(key);
+    if (it != known.end()) return it->second;
+    int per_cu = 0, dev = 0, cus = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
+        (lds > 65536 && hipFuncSetAttribute(key, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)) != hipSuccess) ||
+        hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kern, kThreads, lds) != hipSuccess || per_cu < 1 || cus < 1) {
+        (void)hipGetLastError();
+        return 256;  // without a device: argument checks only
+    }
+    return known[key] = per_cu * cus;
 }
 
 Plan plan(const View& v, const qmm_paged_query& in) {
@@ -1087,7 +1131,7 @@ Plan plan(const View& v, const qmm_paged_query& in) {
         p.kind = per_kv <= (v.c.head_dim <= 128 ? 64 : 16) ? Kind::kRows : Kind::kTile;
         const bool few = p.kind == Kind::kRows;
         p.row_tiles = few ? static_cast<int>((per_kv + 15) / 16) : 0;
-        p.slots = few ? env_int("T_ROWS", 768) : env_int("T_TILE", 512);
+        p.slots = with_matrix_kernel(v, in, p.kind, p.row_tiles, [](auto kern, size_t lds) { return kernel_slots(kern, lds); });
         // A plan's ranges are cut by a length of at least `least` keys.  With W steps in all and u >= W / slots steps a
         // range, the ranges of all row tiles are at most 2 W / u and one more per row tile (a chain's last tile sees up to
         // twice the mean), and those of sequences with more than one range at most twice that, 4 slots.
@@ -1102,7 +1146,8 @@ Plan plan(const View& v, const qmm_paged_query& in) {
     }
     if (p.merge) {
         p.o_bytes = static_cast<size_t>(p.parts) * v.c.head_dim * sizeof(float);
-        p.bytes = p.o_bytes + static_cast<size_t>(p.parts) * sizeof(float2);
+        p.ml_bytes = (static_cast<size_t>(p.parts) * sizeof(float2) + 15) / 16 * 16;
+        p.bytes = p.o_bytes + p.ml_bytes + static_cast<size_t>(in.tokens) * sizeof(int4);
     }
     return p;
 }
@@ -1129,31 +1174,6 @@ bool operands_aligned(const View& v, const qmm_paged_query& in) {
     return els % 8 == 0 && ptr % (fp8 ? 8 : 16) == 0;
 }
 
-template <class T, class C, int D>
-int launch_matrix(const View& v, const AttnArgs& a, const Plan& p, hipStream_t stream) {
-    if (p.blocks > INT32_MAX) return bad("too many sequences, heads and tokens for one call.");
-    const dim3 grid(static_cast<unsigned>(p.blocks));
-    if (p.kind == Kind::kRows) {
-        auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, stream, v, a); };
-        if constexpr (D <= 128) {
-            if (p.row_tiles == 2) go(attention_rows_kernel<T, C, D, 2>);
-            else if (p.row_tiles > 2) go(attention_rows_kernel<T, C, D, 4>);
-        }
-        if (p.row_tiles == 1) go(attention_rows_kernel<T, C, D, 1>);
-        return QMM_OK;
-    }
-    using G = TileGeom<D>;
-    static std::once_flag once;
-    static hipError_t attr = hipSuccess;
-    std::call_once(once, [] {
-        attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_tile_kernel<T, C, D>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                   static_cast<int>(G::kLds));
-    });
-    if (attr != hipSuccess) return launched(attr, "paged attention LDS size");
-    hipLaunchKernelGGL((attention_tile_kernel<T, C, D>), grid, dim3(kThreads), G::kLds, stream, v, a);
-    return QMM_OK;
-}
-
 int tree_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     View v;
     const int rc = check_query(kv, in, &v);
@@ -1178,27 +1198,23 @@ int tree_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, void* work
     a.kps = p.kps;
     a.slots = p.slots;
     a.part_o = static_cast<float*>(workspace);
-    a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + p.o_bytes);
-    const bool fp8 = v.c.dtype == QMM_DTYPE_E4M3;
-    int rc2 = QMM_OK;
-    auto typed = [&](auto tc, auto cc) {
-        using T = decltype(tc);
-        using C = decltype(cc);
-        if (p.kind == Kind::kLanes) {
-            const dim3 grid(static_cast<unsigned>(in->tokens), static_cast<unsigned>(p.splits), static_cast<unsigned>((in->heads + 3) / 4));
-            hipLaunchKernelGGL((attention_lanes_kernel<T, C>), grid, dim3(kThreads), 0, stream, v, a, operands_aligned(v, *in) ? 1 : 0);
-            return;
-        }
-        switch (v.c.head_dim) {
-            case 64: rc2 = launch_matrix<T, C, 64>(v, a, p, stream); break;
-            case 96: rc2 = launch_matrix<T, C, 96>(v, a, p, stream); break;
-            case 128: rc2 = launch_matrix<T, C, 128>(v, a, p, stream); break;
-            default: rc2 = launch_matrix<T, C, 256>(v, a, p, stream); break;
-        }
-    };
-    if (in->dtype == QMM_DTYPE_F16) fp8 ? typed(_Float16{}, Fp8{}) : typed(_Float16{}, _Float16{});
-    else fp8 ? typed(__bf16{}, Fp8{}) : typed(__bf16{}, __bf16{});
-    if (rc2 != QMM_OK) return rc2;
+    if (p.merge) {
+        a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + p.o_bytes);
+        a.cut = reinterpret_cast<int4*>(static_cast<char*>(workspace) + p.o_bytes + p.ml_bytes);
+    }
+    if (p.kind == Kind::kLanes) {
+        const dim3 grid(static_cast<unsigned>(in->tokens), static_cast<unsigned>(p.splits), static_cast<unsigned>((in->heads + 3) / 4));
+        const int aligned = operands_aligned(v, *in) ? 1 : 0;
+        auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, stream, v, a, aligned); };
+        const bool fp8 = v.c.dtype == QMM_DTYPE_E4M3;
+        if (in->dtype == QMM_DTYPE_F16) fp8 ? go(attention_lanes_kernel<_Float16, Fp8>) : go(attention_lanes_kernel<_Float16, _Float16>);
+        else fp8 ? go(attention_lanes_kernel<__bf16, Fp8>) : go(attention_lanes_kernel<__bf16, __bf16>);
+    } else {
+        if (p.blocks > INT32_MAX) return bad("too many sequences, heads and tokens for one call.");
+        with_matrix_kernel(v, *in, p.kind, p.row_tiles, [&](auto kern, size_t lds) {
+            hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(p.blocks)), dim3(kThreads), lds, stream, v, a);
+        });
+    }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return launched(e, "paged attention kernel launch");
     if (p.merge) {
@@ -1207,9 +1223,8 @@ int tree_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, void* work
         auto merge = [&](auto tc) {
             using T = decltype(tc);
             auto go = [&](auto kern) { hipLaunchKernelGGL(kern, mgrid, dim3(kThreads), 0, stream, v, a); };
-            if (p.kind == Kind::kLanes) go(attention_merge_kernel<T, 0, 0>);
-            else if (p.kind == Kind::kRows) go(attention_merge_kernel<T, 16, kRowsStep>);
-            else go(attention_merge_kernel<T, kTileRows, kTileKeys>);
+            if (p.kind == Kind::kLanes) go(attention_merge_kernel<T, false>);
+            else go(attention_merge_kernel<T, true>);
         };
         in->dtype == QMM_DTYPE_F16 ? merge(_Float16{}) : merge(__bf16{});
         e = hipGetLastError();
