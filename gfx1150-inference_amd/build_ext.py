@@ -3,9 +3,11 @@
 * ``libqmm_gfx950.so`` - the HIP kernels and the C ABI declared in ``include/qmm.h``
   (hipcc, ``--offload-arch=gfx950``);
 * ``matmul_module<EXT_SUFFIX>`` - the drop-in pybind11 module, host-only C++ linked against
-  ``libqmm_gfx950.so`` with an ``$ORIGIN`` rpath.
+  ``libqmm_gfx950.so`` with an ``$ORIGIN`` rpath;
+* ``paged_module<EXT_SUFFIX>`` - the paged-cache and beam-search calls for torch tensors, linked alike (torch's
+  own libraries are those that ``import torch`` has loaded).
 
-Both land next to this file, so they travel with the source tree.  Run as
+All land next to this file, so they travel with the source tree.  Run as
 ``python gfx1150-inference_amd/build_ext.py`` or through ``__graft_entry__.build()``.
 """
 
@@ -87,13 +89,40 @@ def build_matmul_module() -> str:
     return out
 
 
+def paged_module_path() -> str:
+    return os.path.join(PKG_DIR, "paged_module" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def build_paged_module() -> str:
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    rocm = os.path.dirname(os.path.dirname(os.path.realpath(HIPCC)))
+    out = paged_module_path()
+    tmp = out + ".tmp"
+    cmd = [
+        "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_API_INCLUDE_EXTENSION_H",
+        f"-I{root}/include", f"-I{root}/include/torch/csrc/api/include", f"-I{rocm}/include",
+        f"-I{sysconfig.get_paths()['include']}", f"-I{INCLUDE}",
+        os.path.join(CSRC, "paged_module.cpp"),
+        f"-L{PKG_DIR}", "-l:" + LIB_NAME, f"-L{root}/lib", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python",
+        "-Wl,-rpath,$ORIGIN", "-o", tmp,
+    ]
+    _run(cmd)
+    os.replace(tmp, out)
+    return out
+
+
 def build_all() -> None:
     build_libqmm()
     build_matmul_module()
+    build_paged_module()
 
 
 if __name__ == "__main__":
     build_all()
     print(LIB_PATH)
     print(matmul_module_path())
+    print(paged_module_path())
     sys.exit(0)

@@ -1,8 +1,9 @@
-"""CPU tests of the paged-cache and beam entry points: the packed arguments match the C structures, and every refusal
+"""CPU tests of the paged-cache and beam entry points: the ctypes mirrors match the C structures, and every refusal
 comes before any GPU work (pointers here are never dereferenced)."""
 
 import ctypes
-import struct
+import os
+import subprocess
 
 import pytest
 
@@ -44,13 +45,21 @@ def _refused(rc, text=""):
     assert text in qmm.last_error(), qmm.last_error()
 
 
-def test_packed_arguments_match_the_structures():
-    for packed, mirror in ((paged._KV, qmm.PagedKV), (paged._NEW, qmm.PagedNew), (paged._QUERY, qmm.PagedQuery)):
-        assert packed.size == ctypes.sizeof(mirror)
-        values = tuple(range(1, len(mirror._fields_) + 1))
-        c = mirror.from_buffer_copy(packed.pack(*values))
-        assert [int(getattr(c, n)) for n, _ in mirror._fields_] == list(values)
-    assert struct.calcsize("@P") == 8
+def test_structures_match_the_header(tmp_path):
+    """The ctypes mirrors have the size and the field offsets of include/qmm.h's structures."""
+    names = {"qmm_paged_kv": qmm.PagedKV, "qmm_paged_new": qmm.PagedNew, "qmm_paged_query": qmm.PagedQuery}
+    lines = ['#include "qmm.h"', "#include <stdio.h>", "int main(void) {"]
+    for c, m in names.items():
+        lines += [f'printf("%zu\\n", offsetof({c}, {f[0]}));' for f in m._fields_] + [f'printf("%zu\\n", sizeof({c}));']
+    src = tmp_path / "s.c"
+    src.write_text("\n".join(lines + ["return 0; }"]))
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    subprocess.run(["gcc", "-I" + include, str(src), "-o", str(tmp_path / "s")], check=True)
+    got = [int(x) for x in subprocess.run([str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout.split()]
+    want = []
+    for m in names.values():
+        want += [getattr(m, f[0]).offset for f in m._fields_] + [ctypes.sizeof(m)]
+    assert got == want
 
 
 BAD_KV = [dict(dtype=qmm.DTYPE_F32), dict(dtype=7), dict(batch=-1), dict(batch=70000), dict(num_pages=-1), dict(table_width=-1),
