@@ -50,11 +50,12 @@ __device__ __forceinline__ float wave_max(float x) {
     return x;
 }
 
-// The largest t that at least n of the wave's keys reach (n <= 64), one bit at a time.
+// The largest t, of sign, exponent and 11 bits of the float, that at least n of the wave's keys reach (n <= 64), one
+// bit at a time.
 __device__ __forceinline__ uint32_t wave_threshold(uint32_t key, int n) {
     uint32_t t = 0;
 #pragma unroll 1
-    for (int bit = 31; bit >= 0; --bit) {
+    for (int bit = 31; bit >= 12; --bit) {
         const uint32_t c = t | (1u << bit);
         if (__popcll(__ballot(key >= c)) >= n) t = c;
     }
@@ -65,15 +66,16 @@ __device__ __forceinline__ int lanes_below(uint64_t mask) {
     return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
 }
 
-// exp(d), d <= 0: 2^(d log2 e) with the product's rounding put back, since the terms' errors would otherwise
-// share a sign and move a beam against the others.
+// exp(d), d <= 0, as 2^(d log2 e) with log2 e in two parts: the rounding of the constant alone would give the terms' errors
+// one sign and move a beam against the others; the product's rounding has either.
 __device__ __forceinline__ float exp_of(float d) {
-    constexpr float kLog2e = 1.44269502162933349609f, kLog2eLow = 1.92596299112661746887e-8f, kLn2 = 0.693147182f;
-    d = d < -200.0f ? -200.0f : d;  // exp is 0 there; -inf would leave a NaN in `rest`
-    const float t = d * kLog2e;
-    const float rest = __fmaf_rn(d, kLog2eLow, __fmaf_rn(d, kLog2e, -t));
-    const float p = __builtin_amdgcn_exp2f(t);
-    return __fmaf_rn(p, rest * kLn2, p);
+    constexpr float kLog2e = 1.44269502162933349609f, kLog2eLow = 1.92596299112661746887e-8f;
+    return __builtin_amdgcn_exp2f(__fmaf_rn(d, kLog2e, d * kLog2eLow));
+}
+
+// The float whose order_key is k.
+__device__ __forceinline__ float key_value(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
 template <class T>
@@ -119,10 +121,15 @@ __global__ __launch_bounds__(kThreads) void select_chunk_kernel(const T* __restr
             for (int e = 0; e < kP; ++e) x[j * kP + e] = at + e < vocab ? static_cast<float>(base[at + e]) : -INFINITY;
         }
     }
-    // the chunk's maximum and sum
-    float m = -INFINITY;
+    // the wave's maximum and sum
+    float piece_best[kN], m = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < E; ++e) m = fmaxf(m, x[e]);
+    for (int j = 0; j < kN; ++j) {
+        piece_best[j] = x[j * kP];
+#pragma unroll
+        for (int e = 1; e < kP; ++e) piece_best[j] = fmaxf(piece_best[j], x[j * kP + e]);
+        m = fmaxf(m, piece_best[j]);
+    }
     const float lane_best = m;
     m = wave_max(m);
     const float ref = m == -INFINITY ? 0.0f : m;  // nothing but -inf: every term is 0
@@ -136,11 +143,11 @@ __global__ __launch_bounds__(kThreads) void select_chunk_kernel(const T* __restr
     auto token_of = [&](int e) { return first + ((e / kP) * kThreads + tid) * kP + e % kP; };
     auto inside = [&](int token) { return token < vocab; };
     uint64_t* mine = list + w * kWaveList;
-    auto put = [&](bool take, int e, int n) {
+    auto put = [&](bool take, uint32_t key, int e, int n) {
         const uint64_t mask = __ballot(take);
         if (mask == 0) return n;
         const int at = n + lanes_below(mask);
-        if (take && at < kWaveList) mine[at] = (static_cast<uint64_t>(order_key(x[e])) << 32) | static_cast<uint32_t>(~token_of(e));
+        if (take && at < kWaveList) mine[at] = (static_cast<uint64_t>(key) << 32) | static_cast<uint32_t>(~token_of(e));
         return n + static_cast<int>(__popcll(mask));
     };
     int n = 0;
@@ -151,39 +158,46 @@ __global__ __launch_bounds__(kThreads) void select_chunk_kernel(const T* __restr
             if (lane < n) mine[lane] = static_cast<uint32_t>(~(first + lane));
         }
     } else {
-        uint32_t t = wave_threshold(order_key(lane_best), beams);
+        // (a piece at a time: few hold one).  What lies past the vocabulary is -inf, and NaN reaches nothing, so a bound
+        // of -inf takes the other way too.
+        const float least = key_value(wave_threshold(order_key(lane_best), beams));
+        if (least > -INFINITY) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) n = put(order_key(x[e]) >= t && inside(token_of(e)), e, n);
-        if (n > kWaveList) {
+            for (int j = 0; j < kN; ++j) {
+                if (__ballot(piece_best[j] >= least) == 0) continue;
+#pragma unroll
+                for (int e = 0; e < kP; ++e) n = put(x[j * kP + e] >= least, order_key(x[j * kP + e]), j * kP + e, n);
+            }
+        }
+        if (n > kWaveList || !(least > -INFINITY)) {
             // many equal logits: the exact bound, then the lowest tokens of those that equal it
-            t = 0;
+            uint32_t k[E], t = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) k[e] = inside(token_of(e)) ? order_key(x[e]) : 0;  // 0: below every key
 #pragma unroll 1
             for (int bit = 31; bit >= 0; --bit) {
                 const uint32_t c = t | (1u << bit);
                 int count = 0;
 #pragma unroll
-                for (int e = 0; e < E; ++e) count += static_cast<int>(__popcll(__ballot(order_key(x[e]) >= c && inside(token_of(e)))));
+                for (int e = 0; e < E; ++e) count += static_cast<int>(__popcll(__ballot(k[e] >= c)));
                 if (count >= beams) t = c;
             }
+            // (t is 0 where the wave holds fewer than `beams`: all of them are above it)
             int above = 0;
 #pragma unroll
-            for (int e = 0; e < E; ++e) above += static_cast<int>(__popcll(__ballot(order_key(x[e]) > t && inside(token_of(e)))));
+            for (int e = 0; e < E; ++e) above += static_cast<int>(__popcll(__ballot(k[e] > t)));
             uint32_t last = 0x7FFFFFFFu;  // the lowest bound on the token that keeps beams - above of the equal ones
 #pragma unroll 1
-            for (int bit = 30; bit >= 0; --bit) {
+            for (int bit = 30; t > 0 && bit >= 0; --bit) {
                 const uint32_t c = last & ~(1u << bit);
                 int count = 0;
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    count += static_cast<int>(__popcll(__ballot(order_key(x[e]) == t && inside(token_of(e)) && static_cast<uint32_t>(token_of(e)) <= c)));
+                for (int e = 0; e < E; ++e) count += static_cast<int>(__popcll(__ballot(k[e] == t && static_cast<uint32_t>(token_of(e)) <= c)));
                 if (above + count >= beams) last = c;
             }
             n = 0;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const uint32_t k = order_key(x[e]);
-                n = put(inside(token_of(e)) && (k > t || (k == t && static_cast<uint32_t>(token_of(e)) <= last)), e, n);
-            }
+            for (int e = 0; e < E; ++e) n = put(k[e] > t || (t > 0 && k[e] == t && static_cast<uint32_t>(token_of(e)) <= last), k[e], e, n);
         }
     }
     if (lane == 0) counts[w] = n;
@@ -236,6 +250,9 @@ __global__ __launch_bounds__(kMergeThreads) void select_merge_kernel(const float
     __shared__ int2 r_at[kW];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t first_row = static_cast<int64_t>(blockIdx.x) * beams;
+    const int per_beam = chunks * beams, n = beams * per_beam;
+    const Candidate* cs = cands + first_row * per_beam;
+    const Candidate own = cs[min(tid, n - 1)];  // requested before the sums' chain
     for (int b = w; b < beams; b += kW) {
         const int parts = chunks * kWaves;
         const Sum* sm = sums + (first_row + b) * parts;
@@ -254,10 +271,8 @@ __global__ __launch_bounds__(kMergeThreads) void select_merge_kernel(const float
     }
     if (tid == 0) l_n = 0;
     __syncthreads();
-    const int per_beam = chunks * beams, n = beams * per_beam;
-    const Candidate* cs = cands + first_row * per_beam;
     auto total_of = [&](int i, int& b, int& token) {
-        const Candidate c = cs[i];
+        const Candidate c = i == tid ? own : cs[i];
         b = i / per_beam;
         token = c.token;
         const double t = static_cast<double>(c.x) + offset[b];
