@@ -417,8 +417,10 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
         for (int f = 0; f < kF; ++f) {
             const int d = kFp8 && (f | 1) < kF ? 64 * (f >> 1) + 16 * q + 8 * (f & 1) : 32 * f + 8 * q;
             __builtin_memcpy(&qf[nt][f], __builtin_assume_aligned(qrow + d, 16), 16);
+            if (a.scale_log2 < 0.0f) qf[nt][f] = -qf[nt][f];  // the same scores from -q and the scale's magnitude
         }
     }
+    const float scale = fabsf(a.scale_log2);
     f32x4 o[NT][D / 16];
     float m_run[NT], l_run[NT];  // l_run: of this lane's keys
 #pragma unroll
@@ -428,39 +430,40 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) o[nt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    const C* kbase = static_cast<const C*>(v.c.k) + g * v.c.k_head;
-    const C* vbase = static_cast<const C*>(v.c.v) + g * v.c.v_head;
+    // A block's 16 keys share a page: a scalar address for them and an offset of the lane that never changes.
+    const char* kbase = reinterpret_cast<const char*>(static_cast<const C*>(v.c.k) + g * v.c.k_head);
+    const char* vbase = reinterpret_cast<const char*>(static_cast<const C*>(v.c.v) + g * v.c.v_head);
+    const uint32_t k_off = static_cast<uint32_t>((l * v.c.k_slot + (kFp8 ? 16 : 8) * q) * sizeof(C));
+    const uint32_t v_off = static_cast<uint32_t>((4 * q * v.c.v_slot + D / 16 * l) * sizeof(C));
+    const uint32_t k_last = static_cast<uint32_t>((l * v.c.k_slot + 32 * (kF - 1) + 8 * q) * sizeof(C));  // fp8, an odd count of 32 dims
     for (int from = begin; from < end; from += kWindow) {
     const int until = min(end, from + kWindow), p0 = from >> v.page_shift;
     if (from > begin) __syncthreads();
     stage_pages(v, s.seq, from, until, pages);
     for (int kb = from + 32 * w; kb < until; kb += 32 * kWaves) {
         u32x4 kr[2][kFp8 ? (kF + 1) / 2 : kF];
-        uint8_t vr[8][kVB] __attribute__((aligned(4)));
+        uint32_t vr[8][(kVB + 3) / 4];
         bool ok[2];
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
-            // 16 keys share a page; rows of the page past the sequence's end are read and masked
+            // rows of the page past the sequence's end are read and masked
             const int k0 = kb + 16 * tt;
             const int id = k0 < end ? __builtin_amdgcn_readfirstlane(pages[(k0 >> v.page_shift) - p0]) : -1;
             ok[tt] = id >= 0;
-            const int64_t page = max(id, 0);
-            const int slot = k0 & (v.c.page_size - 1);
-            const C* kp = kbase + page * v.c.k_page + (slot + l) * v.c.k_slot;
-            if constexpr (kFp8) {
+            const int64_t page = max(id, 0), slot = k0 & (v.c.page_size - 1);
+            const char* kp = kbase + (page * v.c.k_page + slot * v.c.k_slot) * static_cast<int64_t>(sizeof(C));
 #pragma unroll
-                for (int f = 0; f < kF / 2; ++f) kr[tt][f] = *reinterpret_cast<const u32x4*>(kp + 64 * f + 16 * q);
-                if constexpr (kF % 2) {
-                    const u32x2 x = *reinterpret_cast<const u32x2*>(kp + 32 * (kF - 1) + 8 * q);
-                    kr[tt][kF / 2] = u32x4{x[0], x[1], 0, 0};
-                }
-            } else {
-#pragma unroll
-                for (int f = 0; f < kF; ++f) kr[tt][f] = *reinterpret_cast<const u32x4*>(kp + 32 * f + 8 * q);
+            for (int f = 0; f < (kFp8 ? kF / 2 : kF); ++f) kr[tt][f] = *reinterpret_cast<const u32x4*>(kp + 64 * f + k_off);
+            if constexpr (kFp8 && kF % 2) {
+                const u32x2 x = *reinterpret_cast<const u32x2*>(kp + k_last);
+                kr[tt][kF / 2] = u32x4{x[0], x[1], 0, 0};
             }
-            const C* vp = vbase + page * v.c.v_page + (slot + 4 * q) * v.c.v_slot + D / 16 * l;
+            const char* vp = vbase + (page * v.c.v_page + slot * v.c.v_slot) * static_cast<int64_t>(sizeof(C));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) __builtin_memcpy(vr[4 * tt + j], __builtin_assume_aligned(vp + j * v.c.v_slot, kVAlign), kVB);
+            for (int j = 0; j < 4; ++j) {
+                vr[4 * tt + j][(kVB + 3) / 4 - 1] = 0;
+                __builtin_memcpy(vr[4 * tt + j], __builtin_assume_aligned(vp + j * v.c.v_slot * static_cast<int64_t>(sizeof(C)) + v_off, kVAlign), kVB);
+            }
         }
         __builtin_amdgcn_sched_barrier(0);  // every load of the block is out before its first product
         const bool full = kb + 32 <= s.ctx && kb + 32 <= end && ok[0] && ok[1];
@@ -477,17 +480,17 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
                     kf[tt][f] = __builtin_bit_cast(v8, kr[tt][f]);
                 }
             }
-        v8 ph[NT], pl[kLo ? NT : 1];
+        float x[NT][8];
+        bool moves = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            float x[8];
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt) {
                 f32x4 sc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int f = 0; f < kF; ++f) sc = F::mma16(kf[tt][f], qf[nt][f], sc);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[4 * tt + i] = sc[i] * a.scale_log2;
+                for (int i = 0; i < 4; ++i) x[nt][4 * tt + i] = sc[i];
             }
             if (!full) {
                 uint32_t vis = visible32(a, s, tok[nt], kb);
@@ -496,25 +499,36 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
                 vis >>= 4 * q;
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (!((vis >> (16 * (i >> 2) + (i & 3))) & 1)) x[i] = -INFINITY;
+                    if (!((vis >> (16 * (i >> 2) + (i & 3))) & 1)) x[nt][i] = -INFINITY;
             }
-            float mx = x[0];
+            float mx = x[nt][0];
 #pragma unroll
-            for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
-            if (__ballot(mx > m_run[nt] + kSlack) != 0) {
+            for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[nt][i]);
+            moves |= mx * scale > m_run[nt] + kSlack;
+        }
+        if (__ballot(moves) != 0) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float mx = x[nt][0];
+#pragma unroll
+                for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[nt][i]);
                 mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
                 mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-                const float mn = fmaxf(m_run[nt], mx);
+                const float mn = fmaxf(m_run[nt], mx * scale);
                 const float f = m_run[nt] == mn ? 1.0f : __builtin_amdgcn_exp2f(m_run[nt] - mn);
                 l_run[nt] *= f;
 #pragma unroll
                 for (int dt = 0; dt < D / 16; ++dt) o[nt][dt] *= f;
                 m_run[nt] = mn;
             }
+        }
+        v8 ph[NT], pl[kLo ? NT : 1];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
             const float base = m_run[nt] == -INFINITY ? 0.0f : m_run[nt] - kShift;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float p = __builtin_amdgcn_exp2f(x[i] - base);
+                const float p = __builtin_amdgcn_exp2f(__fmaf_rn(x[nt][i], scale, -base));
                 l_run[nt] += p;
                 ph[nt][i] = static_cast<T>(p);
                 if constexpr (kLo) pl[nt][i] = static_cast<T>(p - static_cast<float>(ph[nt][i]));
@@ -526,11 +540,7 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
         for (int j = 0; j < 8; ++j) {
             if constexpr (kFp8) {
 #pragma unroll
-                for (int i = 0; i < kVW; ++i) {
-                    uint16_t h;
-                    __builtin_memcpy(&h, vr[j] + 2 * i, 2);
-                    vd[j][i] = F::from_fp8(h);
-                }
+                for (int i = 0; i < kVW; ++i) vd[j][i] = i % 2 ? F::from_fp8_hi(vr[j][i / 2]) : F::from_fp8(vr[j][i / 2]);
             } else {
                 __builtin_memcpy(vd[j], vr[j], kVB);
             }
