@@ -378,18 +378,20 @@ __device__ __forceinline__ bool stage_pages(const View& v, int seq, int begin, i
 // With one row tile the weights enter as hi + lo in the operands' type, two products: 16 bits and more, where memory
 // hides them.  With more tiles the products are a good part of the time and the weights are rounded once, half a
 // step of each weight (as large as the output's own rounding, and of either sign).
-// The 4 waves take every fourth 32-key block of the range and are joined through LDS in wave order.
+// The 4 waves take every fourth 32-key block of the range; above 32 rows two take half of the rows each (RG = 2), their
+// keys from the L1 cache: one wave's 64 rows of head_dim 128 leave no registers for a second wave on the SIMD (an fp8 cache
+// of 57000 rows, 52 rows a kv head: 51 us with four row tiles a wave, 42 us).  Joined through LDS in wave order.
 constexpr int kRowsStep = 128;
 
-template <class T, class C, int D, int NT>
-__global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attention_rows_kernel(View v, AttnArgs a) {
+template <class T, class C, int D, int NT, int RG>
+__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_kernel(View v, AttnArgs a) {
     using F = Frag<T>;
     using v8 = typename F::v8;
     constexpr bool kFp8 = std::is_same_v<C, Fp8>;
     constexpr int kF = D / 32, kVB = D / 16 * static_cast<int>(sizeof(C)), kVW = D / 32;  // fragments; bytes of a value slice; its dwords of T
     constexpr int kVAlign = (kVB & -kVB) < 16 ? kVB & -kVB : 16;
     constexpr bool kLo = NT == 1;
-    constexpr int kRowF = D + 4, kWaves = kThreads / 64;
+    constexpr int kRowF = D + 4, kWaves = kThreads / 64, kKeyWaves = kWaves / RG;
     __shared__ __align__(16) float so[kWaves][16 * kRowF];
     __shared__ float2 sml[kWaves][16];
     __shared__ int pages[kWindowPages];
@@ -402,7 +404,7 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
     const Span s = span_of(v, a, cp.seq);
     const int kps = cp.keys;
     const int begin = range * kps, end = min(s.total, begin + kps);
-    const int n_rows = cp.rows * group;
+    const int n_rows = cp.rows * group, rg = w / kKeyWaves, kw = w % kKeyWaves, rb = 16 * NT * rg;  // the wave's rows from rb on
     if (g == 0 && range == 0 && a.cut && static_cast<int>(threadIdx.x) < cp.rows) a.cut[s.first + threadIdx.x] = cp.cut_of(threadIdx.x);
 
     // queries: rows past the last repeat it
@@ -410,7 +412,7 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
     int tok[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int r = min(16 * nt + l, n_rows - 1);
+        const int r = min(rb + 16 * nt + l, n_rows - 1);
         tok[nt] = r / group;
         const T* qrow = static_cast<const T*>(a.in.q) + static_cast<int64_t>(s.first + tok[nt]) * a.in.q_token + (g * group + r % group) * a.in.q_head;
 #pragma unroll
@@ -440,7 +442,7 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
     const int until = min(end, from + kWindow), p0 = from >> v.page_shift;
     if (from > begin) __syncthreads();
     stage_pages(v, s.seq, from, until, pages);
-    for (int kb = from + 32 * w; kb < until; kb += 32 * kWaves) {
+    for (int kb = from + 32 * kw; kb < until && rb < n_rows; kb += 32 * kKeyWaves) {
         u32x4 kr[2][kFp8 ? (kF + 1) / 2 : kF];
         uint32_t vr[8][(kVB + 3) / 4];
         bool ok[2];
@@ -568,9 +570,10 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
     }
     }
 
-    // Lane (l, q) holds dims D/4 q + D/16 v + dt of row l in o[nt][dt][v].  A row tile at a time, 16 threads a row.
-    constexpr int kPer = D / 16;
-    const int mr = threadIdx.x >> 4, d0 = kPer * (threadIdx.x & 15);
+    // Lane (l, q) holds dims D/4 q + D/16 v + dt of row l in o[nt][dt][v].  A row tile of each row group at a time, its
+    // key waves' threads in equal shares of a row.
+    constexpr int kRowThreads = 4 * kKeyWaves, kPer = D / kRowThreads, kWaveRows = 64 / kRowThreads;
+    const int in_group = threadIdx.x % (64 * kKeyWaves), mr = in_group / kRowThreads, d0 = kPer * (in_group % kRowThreads);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         if (16 * nt >= n_rows) break;
@@ -588,16 +591,14 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
             }
         if (q == 0) sml[w][l] = float2{m_run[nt], lr};
         __syncthreads();
-        const int r = 16 * nt + mr;
+        const int r = rb + 16 * nt + mr;
         const bool live = r < n_rows;
         float mm = -INFINITY, ls = 0.0f;
         float acc[kPer];
 #pragma unroll
         for (int j = 0; j < kPer; ++j) acc[j] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kWaves; ++i) mm = fmaxf(mm, sml[i][mr].x);
-#pragma unroll
-        for (int i = 0; i < kWaves; ++i) {
+        for (int i = rg * kKeyWaves; i < (rg + 1) * kKeyWaves; ++i) mm = fmaxf(mm, sml[i][mr].x);
+        for (int i = rg * kKeyWaves; i < (rg + 1) * kKeyWaves; ++i) {
             const float2 ml = sml[i][mr];
             if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // no key seen
             const float f = ml.x == mm ? 1.0f : __builtin_amdgcn_exp2f(ml.x - mm);
@@ -613,7 +614,8 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
 #pragma unroll
         for (int j = 0; j < kPer; ++j) nan |= acc[j] != acc[j];
         const uint64_t bad = __ballot(nan && live && ls == ls);
-        const bool mine = (bad >> (lane & 48)) & 0xFFFFu;
+        constexpr uint64_t kRowLanes = (uint64_t{1} << kRowThreads) - 1;
+        const bool mine = (bad >> (lane / kRowThreads * kRowThreads)) & kRowLanes;
         if (live && !mine) {
             if (part < 0) {
                 const float inv = ls == 0.0f ? 0.0f : a.v_scale / ls;
@@ -632,9 +634,9 @@ __global__ __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 2 : 1) void attenti
         }
         if (__builtin_expect(bad != 0, 0)) {
 #pragma unroll 1
-            for (int rr = 0; rr < 4; ++rr) {
-                if (!((bad >> (16 * rr)) & 0xFFFFu)) continue;
-                const int br = 16 * nt + 4 * w + rr;
+            for (int rr = 0; rr < kWaveRows; ++rr) {
+                if (!((bad >> (kRowThreads * rr)) & kRowLanes)) continue;
+                const int br = rb + 16 * nt + kWaveRows * kw + rr;
                 const RowState st = scan_row<T, C>(v, a, s, br / group, g * group + br % group, begin, end, lane, lanes_per_key(D), true);
                 write_state<T>(v, a, s.first + br / group, g * group + br % group, cp.part_of(a, range, br / group, g * group + br % group), st, lane);
             }
@@ -991,11 +993,14 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_tile_ker
     }
 }
 
-// Joins the ranges of each row in their order: D / 4 threads a row, 4 ranges requested at once.
-// Block (x, y): token, heads.
+// Joins the ranges of each row: D / 4 threads hold a row's output and `sg` such groups share its ranges, four of
+// them requested at once; the groups are added in order through LDS.  A few rows of many ranges wait for one or two round
+// trips to memory that way (42 tokens of 32 heads, 37 ranges: 10.6 us with one group).  Block (x, y): token, heads.
 template <class T, bool kPlanned>
-__global__ __launch_bounds__(kThreads) void attention_merge_kernel(View v, AttnArgs a) {
-    const int t = blockIdx.x, D = v.c.head_dim, per = D / 4, rows = kThreads / per, lane = threadIdx.x & 63;
+__global__ __launch_bounds__(kThreads) void attention_merge_kernel(View v, AttnArgs a, int sg) {
+    __shared__ f32x4 so[kThreads];
+    __shared__ float2 sml[kThreads];
+    const int t = blockIdx.x, D = v.c.head_dim, per = D / 4, rows = kThreads / per / sg, lane = threadIdx.x & 63;
     int4 cut = {0, 0, 0, 0};
     if constexpr (kPlanned) cut = a.cut[t];  // not written for a token of no sequence, or past max_new
     const int seq = sequence_of(v, t, lane);
@@ -1010,12 +1015,12 @@ __global__ __launch_bounds__(kThreads) void attention_merge_kernel(View v, AttnA
     const int n = cut.x;
     int64_t row = static_cast<int64_t>(cut.y) * a.in.heads;
     const int64_t step = static_cast<int64_t>(cut.z) * a.in.heads;  // between ranges
-    const int slot = threadIdx.x / per, d0 = 4 * (threadIdx.x % per), head = blockIdx.y * rows + slot;
-    if (slot >= rows || head >= a.in.heads) return;
-    row += head;
+    const int slot = threadIdx.x / per, d0 = 4 * (threadIdx.x % per), gi = slot % sg, head = blockIdx.y * rows + slot / sg;
+    const bool live = slot < rows * sg && head < a.in.heads;
+    row += live ? head : 0;
     float m = -INFINITY, l = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int c0 = 0; c0 < n; c0 += 4) {
+    for (int c0 = 4 * gi; live && c0 < n; c0 += 4 * sg) {
         float2 ml[4];
         f32x4 po[4];
 #pragma unroll
@@ -1039,13 +1044,34 @@ __global__ __launch_bounds__(kThreads) void attention_merge_kernel(View v, AttnA
             if (!(w <= 0.0f)) o += po[i] * w;
         }
     }
+    if (sg > 1) {
+        so[threadIdx.x] = o;
+        sml[threadIdx.x] = float2{m, l};
+        __syncthreads();
+        if (gi != 0) return;
+        for (int i = 1; live && i < sg; ++i) {
+            const float2 x = sml[threadIdx.x + i * per];
+            if (x.y == 0.0f) continue;
+            const f32x4 xo = so[threadIdx.x + i * per];
+            const float mn = fmaxf(m, x.x);
+            const float f = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn), w = x.x == mn ? 1.0f : __builtin_amdgcn_exp2f(x.x - mn);
+            l = l * f + x.y * w;
+            if (f > 0.0f) o *= f;
+            else o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (!(w <= 0.0f)) o += xo * w;
+            m = mn;
+        }
+    }
+    if (!live) return;
     T h[4];
     const float inv = a.v_scale / l;
 #pragma unroll
     for (int i = 0; i < 4; ++i) h[i] = static_cast<T>(l == 0.0f ? 0.0f : o[i] * inv);
     T* out = static_cast<T*>(a.in.out) + static_cast<int64_t>(t) * a.in.out_token + head * a.in.out_head + d0;
+    if (kPlanned) __builtin_memcpy(__builtin_assume_aligned(out, 8), h, 8);  // such a call's operands are aligned
+    else
 #pragma unroll
-    for (int i = 0; i < 4; ++i) out[i] = h[i];
+        for (int i = 0; i < 4; ++i) out[i] = h[i];
 }
 
 // ---- host side -------------------------------------------------------------------------------
@@ -1058,6 +1084,7 @@ struct Plan {
     int slots;          // the others: workgroups to cut the call into ..
     int64_t blocks;     // .. and what that makes at most
     bool merge;
+    int64_t most_ranges;  // of a sequence
     int64_t parts;      // partial rows at most
     size_t o_bytes, ml_bytes, bytes;
 };
@@ -1080,10 +1107,10 @@ template <class T, class C, int D, class Fn>
 auto with_matrix_kernel(Kind kind, int row_tiles, Fn f) {
     if (kind == Kind::kTile) return f(attention_tile_kernel<T, C, D>, TileGeom<D>::kLds);
     if constexpr (D <= 128) {
-        if (row_tiles == 2) return f(attention_rows_kernel<T, C, D, 2>, size_t{0});
-        if (row_tiles > 2) return f(attention_rows_kernel<T, C, D, 4>, size_t{0});
+        if (row_tiles == 2) return f(attention_rows_kernel<T, C, D, 2, 1>, size_t{0});
+        if (row_tiles > 2) return f(attention_rows_kernel<T, C, D, 2, 2>, size_t{0});
     }
-    return f(attention_rows_kernel<T, C, D, 1>, size_t{0});
+    return f(attention_rows_kernel<T, C, D, 1, 1>, size_t{0});
 }
 
 template <class Fn>
@@ -1135,6 +1162,7 @@ Plan plan(const View& v, const qmm_paged_query& in) {
         p.kps = static_cast<int>(kps);
         p.splits = static_cast<int>((most + kps - 1) / kps);
         p.merge = p.splits > 1;
+        p.most_ranges = p.splits;
         p.parts = rows * p.splits;
     } else {
         // more row tiles of head_dim 256 do not fit a wave's registers
@@ -1146,7 +1174,7 @@ Plan plan(const View& v, const qmm_paged_query& in) {
         // range, the ranges of all row tiles are at most 2 W / u and one more per row tile (a chain's last tile sees up to
         // twice the mean), and those of sequences with more than one range at most twice that, 4 slots.
         const int64_t least = few ? kRowsStep : kTileKeys * CallPlan<kTileRows, kTileKeys>::kMinSteps;
-        const int64_t most_ranges = (most + least - 1) / least;
+        const int64_t most_ranges = p.most_ranges = (most + least - 1) / least;
         const int64_t seqs = std::min(v.c.batch, in.tokens);
         const int64_t items = kvh * (few ? seqs : seqs + (static_cast<int64_t>(in.tokens) * (in.heads / kvh) + kTileRows - 1) / kTileRows);
         p.blocks = std::min(items * most_ranges, 2 * static_cast<int64_t>(p.slots) + items);
@@ -1228,11 +1256,14 @@ int tree_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, void* work
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return launched(e, "paged attention kernel launch");
     if (p.merge) {
-        const int rows = kThreads / (v.c.head_dim / 4);
+        const int groups = kThreads / (v.c.head_dim / 4);
+        int sg = 1;
+        while (2 * sg <= groups && 4 * sg < p.most_ranges && static_cast<int64_t>(in->tokens) * in->heads * sg < 8192) sg *= 2;
+        const int rows = groups / sg;
         const dim3 mgrid(static_cast<unsigned>(in->tokens), static_cast<unsigned>((in->heads + rows - 1) / rows));
         auto merge = [&](auto tc) {
             using T = decltype(tc);
-            auto go = [&](auto kern) { hipLaunchKernelGGL(kern, mgrid, dim3(kThreads), 0, stream, v, a); };
+            auto go = [&](auto kern) { hipLaunchKernelGGL(kern, mgrid, dim3(kThreads), 0, stream, v, a, sg); };
             if (p.kind == Kind::kLanes) go(attention_merge_kernel<T, false>);
             else go(attention_merge_kernel<T, true>);
         };
