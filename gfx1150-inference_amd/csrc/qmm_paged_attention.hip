@@ -245,6 +245,31 @@ __device__ __forceinline__ uint32_t visible32(const AttnArgs& a, const Span& s, 
     return m & low(e);
 }
 
+// Sums of lanes 0 .. l of the wave (every lane must be active): rows of 16 by shifts, then the rows' last lanes
+// broadcast.
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
+    return x;
+}
+
+__device__ __forceinline__ float wave_total(float x) {
+    auto step = [&](auto ctrl, auto rows) {
+        x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, decltype(rows)::value, 0xF, false));
+    };
+    step(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xF>{});
+    step(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xF>{});
+    step(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xF>{});
+    step(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xF>{});
+    step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});
+    step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+
 // How a call is cut, from its sequences' lengths; the same in every wave of every workgroup.
 //   steps      64 keys of a 128-row tile, or 128 keys of the one tile of few rows, is a step; a chain's row tiles
 //              see fewer keys than the last one does, so their mean counts;
@@ -283,16 +308,11 @@ struct CallPlan {
     // whose roundings are the same everywhere.
     __device__ __forceinline__ bool find(const View& v, const AttnArgs& a, int at, int lane) {
         const int kvh = v.c.kv_heads;
-        // sums over lanes 0 .. batch - 1 (all 64 of a full chunk) meet in lane 0; the lanes past the batch hold 0
-        auto sum = [&](float t) {
-            for (int o = 1; o < 64 && o < v.c.batch; o <<= 1) t += __shfl_xor(t, o, 64);
-            return __shfl(t, 0, 64);
-        };
         float work = 0.0f;
         Lane x{};
         for (int b0 = 0; b0 < v.c.batch; b0 += 64) {
             x = lane_of(v, a, b0 + lane);
-            work += sum(x.work);
+            work += wave_total(x.work);
         }
         // 1e-5 covers the roundings: a length is never below W / slots
         const float shortest = work * static_cast<float>(kvh) / static_cast<float>(a.slots) * 1.00001f;
@@ -307,7 +327,7 @@ struct CallPlan {
         for (int b0 = 0; b0 < v.c.batch; b0 += 64) {
             if (v.c.batch > 64) x = lane_of(v, a, b0 + lane);
 #pragma unroll
-            for (int c = 0; c < kTries; ++c) count[c] += sum(static_cast<float>(ranges_of(x.steps, u[c])) * static_cast<float>(x.tiles));
+            for (int c = 0; c < kTries; ++c) count[c] += wave_total(static_cast<float>(ranges_of(x.steps, u[c])) * static_cast<float>(x.tiles));
         }
         int best = u[0];
 #pragma unroll
@@ -318,14 +338,7 @@ struct CallPlan {
             if (v.c.batch > 64) x = lane_of(v, a, b0 + lane);
             const int n = ranges_of(x.steps, best);
             const int own_blocks = n * x.tiles * kvh, own_parts = n > 1 ? n * x.rows : 0;
-            int sb = own_blocks, sp = own_parts;
-            for (int o = 1; o < 64 && o < v.c.batch; o <<= 1) {
-                const int ub = __shfl_up(sb, o, 64), up = __shfl_up(sp, o, 64);
-                if (lane >= o) {
-                    sb += ub;
-                    sp += up;
-                }
-            }
+            const int sb = wave_scan(own_blocks), sp = wave_scan(own_parts);
             const int here = min(v.c.batch - b0, 64);
             const int hit = static_cast<int>(__popcll(__ballot(lane < here && blocks + sb <= at)));
             if (hit < here) {
