@@ -131,6 +131,30 @@ def test_long_contexts(cuda):
     Case(22, 2, 1, 128, 64, [3000, 10], [9, 20], BF16, mask="tree").check()
 
 
+def test_many_sequences(cuda):
+    """More sequences than a wave's lanes, of every length."""
+    Case(38, 4, 2, 64, 16, [(7 * i) % 97 for i in range(150)], [1 + (i == 9) for i in range(150)], mask=None).check()
+    Case(39, 4, 1, 64, 32, [(11 * i) % 60 for i in range(70)], [(5 * i) % 37 for i in range(70)], BF16, mask="tree").check()
+    Case(40, 2, 2, 128, 16, [0] * 130 + [3], [0] * 129 + [2, 70], mask=None).check()
+
+
+def test_whole_sequences_in_one_range(cuda):
+    """Enough (sequence, kv head) pairs that 9000 keys are one workgroup's: every sequence the same pages and queries."""
+    import paged
+    ctx, heads, D, page, B = 8999, 24, 64, 16, 64
+    g = torch.Generator().manual_seed(41)
+    k, v = (torch.randn(-(-(ctx + 1) // page), heads, page, D, generator=g).half().cuda() for _ in range(2))
+    row = torch.randperm(k.shape[0], generator=g)
+    q1 = torch.randn(1, heads, D, generator=g).half()
+    out = paged.tree_attention(q1.cuda().expand(B, -1, -1), k, v, row.int().cuda()[None].expand(B, -1), _ints(list(range(B + 1))), _ints([ctx] * B),
+                               max_new=1)
+    assert torch.equal(out, out[:1].expand_as(out))
+    kd, vd = (x.double().cpu()[row].transpose(1, 2).reshape(-1, heads, D)[:ctx + 1] for x in (k, v))
+    p = torch.softmax((kd * q1[0].double()).sum(-1) / D ** 0.5, 0)
+    want, spread = (p[..., None] * vd).sum(0), (p[..., None] * vd.abs()).sum(0)
+    assert ((out[0].double().cpu() - want).abs() <= HALF[F16] * (want.abs() + spread) + 4e-5 * spread).all()
+
+
 def test_large_scores(cuda):
     """Scores of a hundred: the running maximum moves through the whole context."""
     c = Case(23, 4, 1, 64, 16, [700], [5], mask="tree", q_scale=12.0)
