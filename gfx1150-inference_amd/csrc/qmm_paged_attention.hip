@@ -772,14 +772,24 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_tile_ker
     const C* kbase = static_cast<const C*>(v.c.k) + g * v.c.k_head;
     const C* vbase = static_cast<const C*>(v.c.v) + g * v.c.v_head;
 
-    // piece 64 j + lane of the wave's 16 rows
-    uint32_t k_off[G::kPieces], v_off[G::kPieces];
+    // Piece 64 j + lane of the wave's 16 rows.  At head_dim 256 (128 of an fp8 cache) the offsets (and the fragments' addresses below) are formed
+    // anew in every step: kept, they are 40 registers that the accumulators then spill.
+    constexpr bool kKeep = D <= (kFp8 ? 96 : 128);
+    auto offset_of = [&](int j, int at, int64_t slot, bool keys) {
+        const int row = (64 * j + at) / G::kChunks, pos = (64 * j + at) % G::kChunks;
+        return static_cast<uint32_t>((row * static_cast<int>(slot) + 8 * (pos ^ (keys ? G::swap_k(row) : G::swap_v(row)))) * static_cast<int>(sizeof(C)));
+    };
+    auto fresh = [](int x) {  // the same value, not to be kept from step to step
+        if constexpr (!kKeep) __asm__("" : "+v"(x));
+        return x;
+    };
+    uint32_t k_off[kKeep ? G::kPieces : 1], v_off[kKeep ? G::kPieces : 1];
+    if constexpr (kKeep)
 #pragma unroll
-    for (int j = 0; j < G::kPieces; ++j) {
-        const int row = (64 * j + lane) / G::kChunks, pos = (64 * j + lane) % G::kChunks;
-        k_off[j] = static_cast<uint32_t>((row * v.c.k_slot + 8 * (pos ^ G::swap_k(row))) * static_cast<int>(sizeof(C)));
-        v_off[j] = static_cast<uint32_t>((row * v.c.v_slot + 8 * (pos ^ G::swap_v(row))) * static_cast<int>(sizeof(C)));
-    }
+        for (int j = 0; j < G::kPieces; ++j) {
+            k_off[j] = offset_of(j, lane, v.c.k_slot, true);
+            v_off[j] = offset_of(j, lane, v.c.v_slot, false);
+        }
     uint16_t* const mine = tile_lds + 16 * w * D;  // of buffer 0's K
     const uint32_t mine_at = __builtin_amdgcn_readfirstlane(reinterpret_cast<uintptr_t>((LdsPtr)mine));
     const int n_tiles = (end - begin + kTileKeys - 1) / kTileKeys;
@@ -801,18 +811,22 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_tile_ker
     u32x2 kr[kFp8 ? G::kPieces : 1], vr[kFp8 ? G::kPieces : 1];
     auto load_k = [&](int t, int id) {
         const C* p = kbase + page(id) * v.c.k_page + (key_of(t) & (v.c.page_size - 1)) * v.c.k_slot;
+        const int at = fresh(lane);
 #pragma unroll
         for (int j = 0; j < G::kPieces; ++j) {
-            if constexpr (kFp8) kr[j] = *reinterpret_cast<const u32x2*>(reinterpret_cast<const char*>(p) + k_off[j]);
-            else copy_to_lds(p, k_off[j], mine_at + 2 * ((t & 1) * G::kBuf) + 1024 * j);
+            const uint32_t off = kKeep ? k_off[kKeep ? j : 0] : offset_of(j, at, v.c.k_slot, true);
+            if constexpr (kFp8) kr[j] = *reinterpret_cast<const u32x2*>(reinterpret_cast<const char*>(p) + off);
+            else copy_to_lds(p, off, mine_at + 2 * ((t & 1) * G::kBuf) + 1024 * j);
         }
     };
     auto load_v = [&](int t, int id) {
         const C* p = vbase + page(id) * v.c.v_page + (key_of(t) & (v.c.page_size - 1)) * v.c.v_slot;
+        const int at = fresh(lane);
 #pragma unroll
         for (int j = 0; j < G::kPieces; ++j) {
-            if constexpr (kFp8) vr[j] = *reinterpret_cast<const u32x2*>(reinterpret_cast<const char*>(p) + v_off[j]);
-            else copy_to_lds(p, v_off[j], mine_at + 2 * ((t & 1) * G::kBuf + G::kTileE) + 1024 * j);
+            const uint32_t off = kKeep ? v_off[kKeep ? j : 0] : offset_of(j, at, v.c.v_slot, false);
+            if constexpr (kFp8) vr[j] = *reinterpret_cast<const u32x2*>(reinterpret_cast<const char*>(p) + off);
+            else copy_to_lds(p, off, mine_at + 2 * ((t & 1) * G::kBuf + G::kTileE) + 1024 * j);
         }
     };
     auto wide = [](u32x2 x) { return u32x4{F::from_fp8(x[0]), F::from_fp8_hi(x[0]), F::from_fp8(x[1]), F::from_fp8_hi(x[1])}; };
@@ -915,12 +929,13 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_tile_ker
             constexpr int kM = D / 8, kPerB = D / 32, kAhead = 4;
             const uint16_t* sk = k_row + ((t + 1) & 1) * G::kBuf;
             const uint16_t* sv = v_row + (t & 1) * G::kBuf;
+            const int kxs = fresh(kx), vxs = fresh(vx);
             v8 kf[kM], vf[kM], pf[4];
             auto read_k = [&](int n) {
-                __builtin_memcpy(&kf[n], __builtin_assume_aligned(sk + 32 * (n & 1) * D + 8 * ((2 * (n >> 1)) ^ kx), 16), 16);
+                __builtin_memcpy(&kf[n], __builtin_assume_aligned(sk + 32 * (n & 1) * D + 8 * ((2 * (n >> 1)) ^ kxs), 16), 16);
             };
             auto read_v = [&](int n) {
-                const uint16_t* at = sv + 16 * (n / kPerB) * D + 8 * ((4 * (n % kPerB)) ^ vx);
+                const uint16_t* at = sv + 16 * (n / kPerB) * D + 8 * ((4 * (n % kPerB)) ^ vxs);
                 const s16x4 f0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
                 const s16x4 f1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 8 * D));
                 vf[n] = __builtin_bit_cast(v8, __builtin_shufflevector(f0, f1, 0, 1, 2, 3, 4, 5, 6, 7));
