@@ -15,6 +15,7 @@
 #include <map>
 #include <mutex>
 #include <type_traits>
+#include <utility>
 
 namespace qmm {
 namespace paged {
@@ -1192,23 +1193,27 @@ auto with_matrix_kernel(const View& v, const qmm_paged_query& in, Kind kind, int
     return fp8 ? types(__bf16{}, Fp8{}) : types(__bf16{}, __bf16{});
 }
 
-// Workgroups of a kernel that run at once, asked for once per kernel (every device is the same chip).
+// Workgroups of a kernel that run at once, asked for once per kernel and device.
 template <class K>
 int kernel_slots(K kern, size_t lds) {
     static std::mutex mu;
-    static std::map<const void*, int> known;
-    const void* key = reinterpret_cast<const void*>(kern);
-    std::lock_guard<std::mutex> lock(mu);
-    const auto it = known.find(key);
-    if (it != known.end()) return it->second;
+    static std::map<std::pair<const void*, int>, int> known;
+    const void* fn = reinterpret_cast<const void*>(kern);
     int per_cu = 0, dev = 0, cus = 0;
-    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
-        (lds > 65536 && hipFuncSetAttribute(key, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)) != hipSuccess) ||
-        hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kern, kThreads, lds) != hipSuccess || per_cu < 1 || cus < 1) {
+    if (hipGetDevice(&dev) != hipSuccess) {
         (void)hipGetLastError();
         return 256;  // without a device: argument checks only
     }
-    return known[key] = per_cu * cus;
+    std::lock_guard<std::mutex> lock(mu);
+    const auto it = known.find({fn, dev});
+    if (it != known.end()) return it->second;
+    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
+        (lds > 65536 && hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)) != hipSuccess) ||
+        hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kern, kThreads, lds) != hipSuccess || per_cu < 1 || cus < 1) {
+        (void)hipGetLastError();
+        return 256;
+    }
+    return known[{fn, dev}] = per_cu * cus;
 }
 
 Plan plan(const View& v, const qmm_paged_query& in) {
