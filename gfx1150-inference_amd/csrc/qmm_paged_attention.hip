@@ -703,7 +703,9 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
 // copied straight into LDS (global_load_lds; an fp8 cache goes through registers, converted on the way).  Both K
 // and V lie as they are in memory, with the 16-byte pieces of a row exchanged by its number (TileGeom) so that neither the
 // key fragments (16 rows, one piece) nor V's transposing reads (ds_read_b64_tr_b16: 4 rows, two pieces) meet on a bank.
-// Bound by the vector work of the weights beside the products.  The kv heads come fastest in the grid: with 8 of them
+// Bound by the vector work of the weights beside the products, and in short calls by the start (plan, queries, first tile: 10 us)
+// and the partial results.  63-node trees of eight users, 64 heads of 128 over up to 8191 keys (66 GFLOP): 91 us; chunks of up to 500
+// tokens, 32 heads of 64 (16 GFLOP): 44 us.  The kv heads come fastest in the grid: with 8 of them
 // (or 16, ..) the row tiles of one meet on one XCD and its keys in one L2.
 constexpr int kTileRows = 128, kTileKeys = 64;
 
@@ -1138,7 +1140,10 @@ __global__ __launch_bounds__(kThreads) void attention_merge_kernel(View v, AttnA
 }
 
 // ---- host side -------------------------------------------------------------------------------
-// Which kernel serves a call, by the rows (tokens x query heads) that share a kv head, and how its keys are cut.
+// Which kernel serves a call, by the rows (tokens x query heads) that share a kv head, and how its keys are cut.  Up to 64 rows go
+// straight into registers: an fp8 cache is then converted where it is used (52 rows, 57000 keys: 48.5 us, 55.0 through LDS),
+// short calls start sooner (64 rows, 900 keys: 16.1 / 18.1; 28 rows: 14.0 / 16.7), the others are even (52 rows, f16: 38.1 / 38.7)
+// but for many sequences (16 of 64 rows and 2000 keys: 36.5 / 32.7).
 enum class Kind { kLanes, kRows, kTile };
 struct Plan {
     Kind kind;
