@@ -405,8 +405,8 @@ __device__ __forceinline__ void load_row_bytes(uint32_t* dst, const char* src) {
 
 // ---- few rows: keys straight into registers ------------------------------------------------------
 // Up to 64 rows (tokens x query heads of one kv head) against one kv head's keys: decoding, small trees.  Bound by
-// reading K and V from HBM, each once (1.32 GB of 32 users in 221 us, 6.0 TB/s; 238 us with loads that keep the lines).  A wave takes 32 keys at a time, no LDS on the way, and every
-// row tile of 16 uses them:
+// reading K and V from HBM, each once (1.32 GB of 32 users in 220 us, 6.0 TB/s; 238 us with loads that keep the lines).  A wave
+// takes 32 keys at a time, no LDS on the way, and every row tile of 16 uses them:
 //   * S^T = K Q^T on 16x16x32: lane (l, q) = (lane % 16, lane / 16) loads key l's dims 8 q.. of every 32 (fp8: 16 bytes of
 //     every 64, the queries' dims in the same order) and receives the scores of row l with keys 4q .. 4q + 3 of
 //     each 16;
@@ -477,143 +477,143 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
     const uint32_t v_off = static_cast<uint32_t>((4 * q * v.c.v_slot + D / 16 * l) * sizeof(C));
     const uint32_t k_last = static_cast<uint32_t>((l * v.c.k_slot + 32 * (kF - 1) + 8 * q) * sizeof(C));  // fp8, an odd count of 32 dims
     for (int from = begin; from < end; from += kWindow) {
-    const int until = min(end, from + kWindow), p0 = from >> v.page_shift;
-    if (from > begin) __syncthreads();
-    stage_pages(v, s.seq, from, until, pages);
-    for (int kb = from + 32 * kw; kb < until && rb < n_rows; kb += 32 * kKeyWaves) {
-        u32x4 kr[2][kFp8 ? (kF + 1) / 2 : kF];
-        uint32_t vr[8][(kVB + 3) / 4];
-        bool ok[2];
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
-            // rows of the page past the sequence's end are read and masked
-            const int k0 = kb + 16 * tt;
-            const int id = k0 < end ? __builtin_amdgcn_readfirstlane(pages[(k0 >> v.page_shift) - p0]) : -1;
-            ok[tt] = id >= 0;
-            const int64_t page = max(id, 0), slot = k0 & (v.c.page_size - 1);
-            const char* kp = kbase + (page * v.c.k_page + slot * v.c.k_slot) * static_cast<int64_t>(sizeof(C));
-#pragma unroll
-            for (int f = 0; f < (kFp8 ? kF / 2 : kF); ++f) {
-                uint32_t x[4];
-                load_row_bytes<16, 16, RG == 1>(x, kp + 64 * f + k_off);
-                kr[tt][f] = u32x4{x[0], x[1], x[2], x[3]};
-            }
-            if constexpr (kFp8 && kF % 2) {
-                const u32x2 x = *reinterpret_cast<const u32x2*>(kp + k_last);
-                kr[tt][kF / 2] = u32x4{x[0], x[1], 0, 0};
-            }
-            const char* vp = vbase + (page * v.c.v_page + slot * v.c.v_slot) * static_cast<int64_t>(sizeof(C));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                vr[4 * tt + j][(kVB + 3) / 4 - 1] = 0;
-                load_row_bytes<kVB, kVAlign, RG == 1>(vr[4 * tt + j], vp + j * v.c.v_slot * static_cast<int64_t>(sizeof(C)) + v_off);
-            }
-        }
-        __builtin_amdgcn_sched_barrier(0);  // every load of the block is out before its first product
-        const bool full = kb + 32 <= s.ctx && kb + 32 <= end && ok[0] && ok[1];
-        v8 kf[2][kF];
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-            for (int f = 0; f < kF; ++f) {
-                if constexpr (kFp8) {
-                    const uint32_t x = kr[tt][f >> 1][2 * (f & 1)], y = kr[tt][f >> 1][2 * (f & 1) + 1];
-                    const u32x4 t = {F::from_fp8(x), F::from_fp8_hi(x), F::from_fp8(y), F::from_fp8_hi(y)};
-                    kf[tt][f] = __builtin_bit_cast(v8, t);
-                } else {
-                    kf[tt][f] = __builtin_bit_cast(v8, kr[tt][f]);
-                }
-            }
-        float x[NT][8];
-        bool moves = false;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+        const int until = min(end, from + kWindow), p0 = from >> v.page_shift;
+        if (from > begin) __syncthreads();
+        stage_pages(v, s.seq, from, until, pages);
+        for (int kb = from + 32 * kw; kb < until && rb < n_rows; kb += 32 * kKeyWaves) {
+            u32x4 kr[2][kFp8 ? (kF + 1) / 2 : kF];
+            uint32_t vr[8][(kVB + 3) / 4];
+            bool ok[2];
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt) {
-                f32x4 sc = {0.0f, 0.0f, 0.0f, 0.0f};
+                // rows of the page past the sequence's end are read and masked
+                const int k0 = kb + 16 * tt;
+                const int id = k0 < end ? __builtin_amdgcn_readfirstlane(pages[(k0 >> v.page_shift) - p0]) : -1;
+                ok[tt] = id >= 0;
+                const int64_t page = max(id, 0), slot = k0 & (v.c.page_size - 1);
+                const char* kp = kbase + (page * v.c.k_page + slot * v.c.k_slot) * static_cast<int64_t>(sizeof(C));
 #pragma unroll
-                for (int f = 0; f < kF; ++f) sc = F::mma16(kf[tt][f], qf[nt][f], sc);
+                for (int f = 0; f < (kFp8 ? kF / 2 : kF); ++f) {
+                    uint32_t x[4];
+                    load_row_bytes<16, 16, RG == 1>(x, kp + 64 * f + k_off);
+                    kr[tt][f] = u32x4{x[0], x[1], x[2], x[3]};
+                }
+                if constexpr (kFp8 && kF % 2) {
+                    const u32x2 x = *reinterpret_cast<const u32x2*>(kp + k_last);
+                    kr[tt][kF / 2] = u32x4{x[0], x[1], 0, 0};
+                }
+                const char* vp = vbase + (page * v.c.v_page + slot * v.c.v_slot) * static_cast<int64_t>(sizeof(C));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[nt][4 * tt + i] = sc[i];
+                for (int j = 0; j < 4; ++j) {
+                    vr[4 * tt + j][(kVB + 3) / 4 - 1] = 0;
+                    load_row_bytes<kVB, kVAlign, RG == 1>(vr[4 * tt + j], vp + j * v.c.v_slot * static_cast<int64_t>(sizeof(C)) + v_off);
+                }
             }
-            if (!full) {
-                uint32_t vis = visible32(a, s, tok[nt], kb);
-                if (!ok[0]) vis &= 0xFFFF0000u;
-                if (!ok[1]) vis &= 0x0000FFFFu;
-                vis >>= 4 * q;
+            __builtin_amdgcn_sched_barrier(0);  // every load of the block is out before its first product
+            const bool full = kb + 32 <= s.ctx && kb + 32 <= end && ok[0] && ok[1];
+            v8 kf[2][kF];
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (!((vis >> (16 * (i >> 2) + (i & 3))) & 1)) x[nt][i] = -INFINITY;
-            }
-            float mx = x[nt][0];
+            for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-            for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[nt][i]);
-            moves |= mx * scale > m_run[nt] + kSlack;
-        }
-        if (__ballot(moves) != 0) {
+                for (int f = 0; f < kF; ++f) {
+                    if constexpr (kFp8) {
+                        const uint32_t x = kr[tt][f >> 1][2 * (f & 1)], y = kr[tt][f >> 1][2 * (f & 1) + 1];
+                        const u32x4 t = {F::from_fp8(x), F::from_fp8_hi(x), F::from_fp8(y), F::from_fp8_hi(y)};
+                        kf[tt][f] = __builtin_bit_cast(v8, t);
+                    } else {
+                        kf[tt][f] = __builtin_bit_cast(v8, kr[tt][f]);
+                    }
+                }
+            float x[NT][8];
+            bool moves = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt) {
+                    f32x4 sc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int f = 0; f < kF; ++f) sc = F::mma16(kf[tt][f], qf[nt][f], sc);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[nt][4 * tt + i] = sc[i];
+                }
+                if (!full) {
+                    uint32_t vis = visible32(a, s, tok[nt], kb);
+                    if (!ok[0]) vis &= 0xFFFF0000u;
+                    if (!ok[1]) vis &= 0x0000FFFFu;
+                    vis >>= 4 * q;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (!((vis >> (16 * (i >> 2) + (i & 3))) & 1)) x[nt][i] = -INFINITY;
+                }
                 float mx = x[nt][0];
 #pragma unroll
                 for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[nt][i]);
-                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-                const float mn = fmaxf(m_run[nt], mx * scale);
-                const float f = m_run[nt] == mn ? 1.0f : __builtin_amdgcn_exp2f(m_run[nt] - mn);
-                l_run[nt] *= f;
-#pragma unroll
-                for (int dt = 0; dt < D / 16; ++dt) o[nt][dt] *= f;
-                m_run[nt] = mn;
+                moves |= mx * scale > m_run[nt] + kSlack;
             }
-        }
-        v8 ph[NT], pl[kLo ? NT : 1];
+            if (__ballot(moves) != 0) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const float base = m_run[nt] == -INFINITY ? 0.0f : m_run[nt] - kShift;
+                for (int nt = 0; nt < NT; ++nt) {
+                    float mx = x[nt][0];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float p = __builtin_amdgcn_exp2f(__fmaf_rn(x[nt][i], scale, -base));
-                ph[nt][i] = static_cast<T>(p);
-                if constexpr (kLo) {
-                    l_run[nt] += p;
-                    pl[nt][i] = static_cast<T>(p - static_cast<float>(ph[nt][i]));
-                } else if (i & 1) {
-                    l_run[nt] = F::add2(ph[nt], i - 1, l_run[nt]);
+                    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[nt][i]);
+                    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                    const float mn = fmaxf(m_run[nt], mx * scale);
+                    const float f = m_run[nt] == mn ? 1.0f : __builtin_amdgcn_exp2f(m_run[nt] - mn);
+                    l_run[nt] *= f;
+#pragma unroll
+                    for (int dt = 0; dt < D / 16; ++dt) o[nt][dt] *= f;
+                    m_run[nt] = mn;
+                }
+            }
+            v8 ph[NT], pl[kLo ? NT : 1];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float base = m_run[nt] == -INFINITY ? 0.0f : m_run[nt] - kShift;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float p = __builtin_amdgcn_exp2f(__fmaf_rn(x[nt][i], scale, -base));
+                    ph[nt][i] = static_cast<T>(p);
+                    if constexpr (kLo) {
+                        l_run[nt] += p;
+                        pl[nt][i] = static_cast<T>(p - static_cast<float>(ph[nt][i]));
+                    } else if (i & 1) {
+                        l_run[nt] = F::add2(ph[nt], i - 1, l_run[nt]);
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);  // and V's transposition waits for V alone
+            uint32_t vd[8][kVW];  // the value slices as pairs of T
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if constexpr (kFp8) {
+#pragma unroll
+                    for (int i = 0; i < kVW; ++i) vd[j][i] = i % 2 ? F::from_fp8_hi(vr[j][i / 2]) : F::from_fp8(vr[j][i / 2]);
+                } else {
+                    __builtin_memcpy(vd[j], vr[j], kVB);
+                }
+            }
+            if (!full) {  // rows that nobody sees may hold anything
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (!(ok[j >> 2] && kb + 16 * (j >> 2) + 4 * q + (j & 3) < s.total))
+#pragma unroll
+                        for (int i = 0; i < kVW; ++i) vd[j][i] = 0;
+            }
+#pragma unroll
+            for (int dt = 0; dt < D / 16; ++dt) {  // operand row l is dim D/16 l + dt of the lane's 8 keys
+                u32x4 t;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    t[i] = __builtin_amdgcn_perm(vd[2 * i + 1][dt >> 1], vd[2 * i][dt >> 1], (dt & 1) ? 0x07060302u : 0x05040100u);
+                const v8 vf = __builtin_bit_cast(v8, t);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    o[nt][dt] = F::mma16(vf, ph[nt], o[nt][dt]);
+                    if constexpr (kLo) o[nt][dt] = F::mma16(vf, pl[nt], o[nt][dt]);
                 }
             }
         }
-        __builtin_amdgcn_sched_barrier(0);  // and V's transposition waits for V alone
-        uint32_t vd[8][kVW];  // the value slices as pairs of T
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if constexpr (kFp8) {
-#pragma unroll
-                for (int i = 0; i < kVW; ++i) vd[j][i] = i % 2 ? F::from_fp8_hi(vr[j][i / 2]) : F::from_fp8(vr[j][i / 2]);
-            } else {
-                __builtin_memcpy(vd[j], vr[j], kVB);
-            }
-        }
-        if (!full) {  // rows that nobody sees may hold anything
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (!(ok[j >> 2] && kb + 16 * (j >> 2) + 4 * q + (j & 3) < s.total))
-#pragma unroll
-                    for (int i = 0; i < kVW; ++i) vd[j][i] = 0;
-        }
-#pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) {  // operand row l is dim D/16 l + dt of the lane's 8 keys
-            u32x4 t;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                t[i] = __builtin_amdgcn_perm(vd[2 * i + 1][dt >> 1], vd[2 * i][dt >> 1], (dt & 1) ? 0x07060302u : 0x05040100u);
-            const v8 vf = __builtin_bit_cast(v8, t);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                o[nt][dt] = F::mma16(vf, ph[nt], o[nt][dt]);
-                if constexpr (kLo) o[nt][dt] = F::mma16(vf, pl[nt], o[nt][dt]);
-            }
-        }
-    }
     }
 
     // Lane (l, q) holds dims D/4 q + D/16 v + dt of row l in o[nt][dt][v].  A row tile of each row group at a time, its
@@ -691,13 +691,14 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
 }
 
 // ---- many rows: keys through LDS -----------------------------------------------------------------
-// A workgroup of 4 waves owns 128 RT rows (tokens x query heads of one kv head), 32 RT a wave, and walks the keys in
-// tiles of 64, staged through LDS (two buffers, one barrier a tile) and taken 32 at a time:
-//   * S^T = K Q^T on 32x32x16, the wave's queries in registers: a lane holds one row (lane % 32) and 16 of the 32
+// A workgroup of 4 waves owns 128 rows (tokens x query heads of one kv head), 32 a wave, and walks the keys in tiles of 64,
+// staged through LDS (two buffers, one barrier a tile):
+//   * S^T = K Q^T on 32x32x16, the wave's queries in registers: a lane holds one row (lane % 32) and 16 of every 32
 //     keys, the partner lane (lane ^ 32) the others;
 //   * the weights go from the S registers into O^T += V^T P^T without leaving the lane (the k order of each 16-key
 //     block is the order the lane holds its keys in).  Weights are rounded to the operands' type once, half a step, of
-//     either sign;
+//     either sign, and their sum is of the rounded ones;
+//   * the next tile's scores are formed beside this tile's weights, so keys are copied two tiles ahead, values one;
 //   * the lanes keep sums of their own; maxima are exchanged only when the running one moves (kSlack).
 // Wave w stages keys 16 w .. 16 w + 15 of a tile, which share a page: a scalar address and lane offsets that never change,
 // copied straight into LDS (global_load_lds; an fp8 cache goes through registers, converted on the way).  Both K
