@@ -6,8 +6,8 @@
 //           of exp(x - max).
 //   Pass 2: one block per sentence joins the chunks' sums into each beam's logarithm, in 64 bits, and
 //           ranks the chunks' candidates by (total in 64 bits, beam, token).
-// 128 rows of 128256 f16 logits (33 MB): 19.8 us of pass 1, bound by its vector work (10 instructions a logit) at three waves a
-// SIMD, and 8.4 us of pass 2, whose sixteen blocks wait for loads and a 64-bit exponential and logarithm.
+// 128 rows of 128256 f16 logits (33 MB): 14.8 us of pass 1, bound by its vector work (a dozen instructions a logit), and 8.6 us
+// of pass 2, whose sixteen blocks wait for loads and a 64-bit exponential and logarithm.
 // The order of equal totals and every sum are fixed by the sizes alone, so equal beams give equal totals.
 #include "qmm_paged.h"
 
@@ -109,35 +109,46 @@ __global__ __launch_bounds__(kThreads) void select_chunk_kernel(const T* __restr
     const int row = blockIdx.y, chunk = blockIdx.x;
     const T* base = logits + (row / beams) * sentence_stride + (row % beams) * beam_stride;
     const int first = chunk * (E * kThreads);  // token of the chunk's first element
-    float x[E];
+    // The logits stay as they came, 16 bytes a piece, and are converted where they are used: 64 of them as floats left
+    // three waves a SIMD (19.8 us, where it is 14.8).
+    using P = typename Piece<T>::type;
+    P raw[kN];
 #pragma unroll
     for (int j = 0; j < kN; ++j) {
         const int at = first + (j * kThreads + tid) * kP;
         if (at + kP <= vocab) {
-            typename Piece<T>::type p;
-            __builtin_memcpy(&p, base + at, 16);
-#pragma unroll
-            for (int e = 0; e < kP; ++e) x[j * kP + e] = static_cast<float>(p[e]);
+            __builtin_memcpy(&raw[j], base + at, 16);
         } else {
 #pragma unroll
-            for (int e = 0; e < kP; ++e) x[j * kP + e] = at + e < vocab ? static_cast<float>(base[at + e]) : -INFINITY;
+            for (int e = 0; e < kP; ++e) raw[j][e] = at + e < vocab ? base[at + e] : static_cast<T>(-INFINITY);
         }
     }
+    auto unkept = [&] {  // what was converted before is not kept beyond this point
+#pragma unroll
+        for (int j = 0; j < kN; ++j) {
+            u32x4 t = __builtin_bit_cast(u32x4, raw[j]);
+            __asm__("" : "+v"(t));
+            raw[j] = __builtin_bit_cast(P, t);
+        }
+    };
+    auto x = [&](int e) { return static_cast<float>(raw[e / kP][e % kP]); };
     // the wave's maximum and sum
     float piece_best[kN], m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < kN; ++j) {
-        piece_best[j] = x[j * kP];
+        piece_best[j] = x(j * kP);
 #pragma unroll
-        for (int e = 1; e < kP; ++e) piece_best[j] = fmaxf(piece_best[j], x[j * kP + e]);
+        for (int e = 1; e < kP; ++e) piece_best[j] = fmaxf(piece_best[j], x(j * kP + e));
         m = fmaxf(m, piece_best[j]);
     }
     const float lane_best = m;
     m = wave_max(m);
     const float ref = m == -INFINITY ? 0.0f : m;  // nothing but -inf: every term is 0
     float s = 0.0f;
+    unkept();
 #pragma unroll
-    for (int e = 0; e < E; ++e) s += exp_of(x[e] - ref);
+    for (int e = 0; e < E; ++e) s += exp_of(x(e) - ref);
+    unkept();
     const double ws = wave_add(static_cast<double>(s));
     if (lane == 0) sums[(static_cast<int64_t>(row) * gridDim.x + chunk) * kWaves + w] = Sum{static_cast<double>(m), ws};
 
@@ -168,38 +179,44 @@ __global__ __launch_bounds__(kThreads) void select_chunk_kernel(const T* __restr
             for (int j = 0; j < kN; ++j) {
                 if (__ballot(piece_best[j] >= least) == 0) continue;
 #pragma unroll
-                for (int e = 0; e < kP; ++e) n = put(x[j * kP + e] >= least, order_key(x[j * kP + e]), j * kP + e, n);
+                for (int e = 0; e < kP; ++e) n = put(x(j * kP + e) >= least, order_key(x(j * kP + e)), j * kP + e, n);
             }
         }
         if (n > kWaveList || !(least > -INFINITY)) {
             // many equal logits: the exact bound, then the lowest tokens of those that equal it
-            uint32_t k[E], t = 0;
-#pragma unroll
-            for (int e = 0; e < E; ++e) k[e] = inside(token_of(e)) ? order_key(x[e]) : 0;  // 0: below every key
+            auto key = [&](int e) { return inside(token_of(e)) ? order_key(x(e)) : 0; };  // 0: below every key
+            uint32_t t = 0;
 #pragma unroll 1
             for (int bit = 31; bit >= 0; --bit) {
                 const uint32_t c = t | (1u << bit);
                 int count = 0;
+                unkept();
 #pragma unroll
-                for (int e = 0; e < E; ++e) count += static_cast<int>(__popcll(__ballot(k[e] >= c)));
+                for (int e = 0; e < E; ++e) count += static_cast<int>(__popcll(__ballot(key(e) >= c)));
                 if (count >= beams) t = c;
             }
             // (t is 0 where the wave holds fewer than `beams`: all of them are above it)
             int above = 0;
+            unkept();
 #pragma unroll
-            for (int e = 0; e < E; ++e) above += static_cast<int>(__popcll(__ballot(k[e] > t)));
+            for (int e = 0; e < E; ++e) above += static_cast<int>(__popcll(__ballot(key(e) > t)));
             uint32_t last = 0x7FFFFFFFu;  // the lowest bound on the token that keeps beams - above of the equal ones
 #pragma unroll 1
             for (int bit = 30; t > 0 && bit >= 0; --bit) {
                 const uint32_t c = last & ~(1u << bit);
                 int count = 0;
+                unkept();
 #pragma unroll
-                for (int e = 0; e < E; ++e) count += static_cast<int>(__popcll(__ballot(k[e] == t && static_cast<uint32_t>(token_of(e)) <= c)));
+                for (int e = 0; e < E; ++e) count += static_cast<int>(__popcll(__ballot(key(e) == t && static_cast<uint32_t>(token_of(e)) <= c)));
                 if (above + count >= beams) last = c;
             }
             n = 0;
+            unkept();
 #pragma unroll
-            for (int e = 0; e < E; ++e) n = put(k[e] > t || (t > 0 && k[e] == t && static_cast<uint32_t>(token_of(e)) <= last), k[e], e, n);
+            for (int e = 0; e < E; ++e) {
+                const uint32_t k = key(e);
+                n = put(k > t || (t > 0 && k == t && static_cast<uint32_t>(token_of(e)) <= last), k, e, n);
+            }
         }
     }
     if (lane == 0) counts[w] = n;
@@ -363,7 +380,7 @@ __global__ __launch_bounds__(kMergeThreads) void select_merge_kernel(const float
 
 // ---- host side -------------------------------------------------------------------------------
 // Logits a thread: as few as leave 512 chunks, so that small calls use the chip's width and large ones read up to 64 logits a
-// thread at once and leave few candidates (128 rows of 128256: 19.8 + 8.8 us at 64, 16.7 + 12.3 at 32).
+// thread at once and leave few candidates (128 rows of 128256: 14.8 + 8.6 us at 64, 15.0 + 12.5 at 32).
 int per_thread(int64_t rows, int vocab) {
     int e = 8;
     while (e < 64 && rows * ((vocab + 2 * e * kThreads - 1) / (2 * e * kThreads)) >= 512) e *= 2;
