@@ -703,7 +703,8 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
 // Wave w stages keys 16 w .. 16 w + 15 of a tile, which share a page: a scalar address and lane offsets that never change,
 // copied straight into LDS (global_load_lds; an fp8 cache goes through registers, converted on the way).  Both K
 // and V lie as they are in memory, with the 16-byte pieces of a row exchanged by its number (TileGeom) so that neither the
-// key fragments (16 rows, one piece) nor V's transposing reads (ds_read_b64_tr_b16: 4 rows, two pieces) meet on a bank.
+// key fragments (16 rows, one piece) nor V's transposing reads (ds_read_b64_tr_b16: half a wave takes four pieces of 4
+// rows) meet on a bank.
 // Bound by the vector work of the weights beside the products, and in short calls by the start (plan, queries, first tile: 10 us)
 // and the partial results.  63-node trees of eight users, 64 heads of 128 over up to 8191 keys (66 GFLOP): 91 us; chunks of up to 500
 // tokens, 32 heads of 64 (16 GFLOP): 44 us.  The kv heads come fastest in the grid: with 8 of them
@@ -718,7 +719,7 @@ struct TileGeom {
     static constexpr int kChunks = D / 8, kPieces = D / 32;  // 16-byte pieces of a row; of 16 rows, per lane
     // what the piece number is XORed with
     static __device__ __forceinline__ int swap_k(int row) { return D == 64 ? (row >> 1) & 7 : D == 96 ? (row >> 2) & 3 : row & 15; }
-    static __device__ __forceinline__ int swap_v(int row) { return D == 64 ? ((row >> 1) & 3) << 1 : D == 96 ? 0 : (row & 7) << 1; }
+    static __device__ __forceinline__ int swap_v(int row) { return D == 64 ? ((row >> 1) & 1) << 2 : D == 96 ? 0 : (row & 3) << 2; }
 };
 
 extern __shared__ __align__(16) uint16_t tile_lds[];
