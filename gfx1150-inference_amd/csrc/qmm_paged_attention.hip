@@ -31,6 +31,7 @@ struct AttnArgs {
     int slots;         // workgroups that a plan cuts the call into: those that run at once
     float* part_o;     // [partial row][D]
     float2* part_ml;   // [partial row]: maximum, sum
+    int64_t parts;     // tokens that the partial rows have room for
     int4* cut;         // [token]: ranges, its first partial row and the rows between ranges, in tokens
 };
 
@@ -322,13 +323,13 @@ struct CallPlan {
             x = lane_of(v, a, b0 + lane);
             work += wave_total(x.work);
         }
-        // 1e-5 covers the roundings: a length is never below W / slots
+        // 1e-5 covers the roundings: a length is never below W / slots, or it is 2^25 steps, which no sequence passes
         const float shortest = work * static_cast<float>(kvh) / static_cast<float>(a.slots) * 1.00001f;
         int u[kTries];
         float count[kTries];
 #pragma unroll
         for (int c = 0; c < kTries; ++c) {
-            u[c] = max(static_cast<int>(fminf(ceilf(shortest * (1.0f + 0.25f * static_cast<float>(c))), 8388608.0f)), kMinSteps);
+            u[c] = max(static_cast<int>(fminf(ceilf(shortest * (1.0f + 0.25f * static_cast<float>(c))), 33554432.0f)), kMinSteps);
             count[c] = 0.0f;
         }
         auto ranges_of = [&](int steps, int len) { return static_cast<int>((static_cast<uint32_t>(steps) + len - 1) / static_cast<uint32_t>(len)); };
@@ -358,7 +359,8 @@ struct CallPlan {
                 keys = (of(x.steps) + ranges - 1) / ranges * kStep;
                 block = at - (blocks + of(sb - own_blocks));
                 first_part = parts + of(sp - own_parts);
-                return true;
+                // room is short only where cu descends and sequences overlap
+                return ranges == 1 || first_part + static_cast<int64_t>(ranges) * rows <= a.parts;
             }
             blocks += __builtin_amdgcn_readlane(sb, here - 1);
             parts += __builtin_amdgcn_readlane(sp, here - 1);
@@ -1079,6 +1081,7 @@ __global__ __launch_bounds__(kThreads) void attention_merge_kernel(View v, AttnA
         cut = int4{(s.total + a.kps - 1) / a.kps, t, a.in.tokens, 0};
     }
     if (cut.x <= 1) return;  // written by the range itself
+    if (kPlanned && (cut.y < 0 || cut.z < 1 || cut.y + static_cast<int64_t>(cut.x - 1) * cut.z >= a.parts)) return;  // nor where cu descends
     const int n = cut.x;
     int64_t row = static_cast<int64_t>(cut.y) * a.in.heads;
     const int64_t step = static_cast<int64_t>(cut.z) * a.in.heads;  // between ranges
@@ -1310,6 +1313,7 @@ int tree_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, void* work
     a.kps = p.kps;
     a.slots = p.slots;
     a.part_o = static_cast<float*>(workspace);
+    a.parts = p.parts / in->heads;
     if (p.merge) {
         a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + p.o_bytes);
         a.cut = reinterpret_cast<int4*>(static_cast<char*>(workspace) + p.o_bytes + p.ml_bytes);

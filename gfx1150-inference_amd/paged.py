@@ -5,8 +5,8 @@ For batches of sequences whose rows live in pages of one pool.  The caller owns 
 * a layer's cache is a K and a V tensor ``[pages, kv_heads, page_size, head_dim]`` (float16, bfloat16 or
   float8_e4m3fn; any strides with ``head_dim`` contiguous, so that K and V may share one tensor);
 * ``table`` ``[batch, width]`` int32 holds each sequence's page ids, ``ctx`` ``[batch]`` int32 the rows it has;
-* ``cu`` ``[batch + 1]`` int32 delimits the new tokens, which are concatenated: sequence b has tokens
-  ``cu[b]`` to ``cu[b + 1] - 1``, and they take its rows ``ctx[b]``, ``ctx[b] + 1``, ...
+* ``cu`` ``[batch + 1]`` int32, not descending, delimits the new tokens, which are concatenated: sequence b has
+  tokens ``cu[b]`` to ``cu[b + 1] - 1``, and they take its rows ``ctx[b]``, ``ctx[b] + 1``, ...
 
 A decoding step of a model calls, per layer, ``append`` and ``tree_attention``; a step with drafted
 tokens ends with one ``commit_path`` over all layers.  Every call is asynchronous on ``stream`` (the

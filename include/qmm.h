@@ -350,9 +350,9 @@ int qmm_forward_layer_host(const qmm_layer_config* cfg, const qmm_layer_weights*
  * strides given in elements; num_layers of them layer_stride apart for the calls that touch every
  * layer), page_size a power of two.  Row i of sequence b is slot i % page_size of page
  * table[b][i / page_size].  Sequence b holds ctx[b] rows and has the new tokens
- * cu[b] .. cu[b + 1] - 1 of the call's `tokens` (concatenated; a sequence may have none); they
- * take the rows ctx[b], ctx[b] + 1, ...  table, cu and ctx are read on the device: a row whose page is
- * outside the table or the pool is not written, copied or seen.
+ * cu[b] .. cu[b + 1] - 1 of the call's `tokens` (concatenated; a sequence may have none; cu does not
+ * descend); they take the rows ctx[b], ctx[b] + 1, ...  table, cu and ctx are read on the device: a row
+ * whose page is outside the table or the pool is not written, copied or seen.
  * --------------------------------------------------------------------------------- */
 typedef struct qmm_paged_kv {
     void* k;
