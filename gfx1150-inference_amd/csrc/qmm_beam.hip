@@ -6,8 +6,9 @@
 //           of exp(x - max).
 //   Pass 2: one block per sentence joins the chunks' sums into each beam's logarithm, in 64 bits, and
 //           ranks the chunks' candidates by (total in 64 bits, beam, token).
-// 128 rows of 128256 f16 logits (33 MB): 14.8 us of pass 1, bound by its vector work (a dozen instructions a logit), and 8.6 us
-// of pass 2, whose sixteen blocks wait for loads and a 64-bit exponential and logarithm.
+// 128 rows of 128256 f16 logits (33 MB): 14.7 us of pass 1, whose blocks all run at once, so that its parts follow each
+// other (7.3 us of reading and maxima, 3 of exponentials, 4 of finding the candidates), and 8.0 us of pass 2, whose sixteen
+// blocks wait for loads and a 64-bit exponential and logarithm.
 // The order of equal totals and every sum are fixed by the sizes alone, so equal beams give equal totals.
 #include "qmm_paged.h"
 
@@ -40,16 +41,48 @@ __device__ __forceinline__ uint32_t order_key(float x) {
     return x != x ? 0x007FFFFFu : k;
 }
 
-__device__ __forceinline__ double wave_add(double x) {
+// x joined over the wave, the result in every lane (all of them must be active): neighbours, pairs and halves of 16 lanes
+// by DPP, rows of 16 and halves of the wave by swaps.  4 beams of 32000 f32 logits: 5.0 + 5.0 us, 5.3 + 5.8 with shuffles
+// through LDS (and the partial sums read twice).
+template <class V, class Join>
+__device__ __forceinline__ V wave_join(V x, Join join) {
+    constexpr int kWords = sizeof(V) / 4;
+    struct Words {
+        uint32_t w[kWords];
+    };
+    auto dpp = [&](auto ctrl) {
+        Words t = __builtin_bit_cast(Words, x);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
+        for (int i = 0; i < kWords; ++i)
+            t.w[i] = static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(t.w[i]), decltype(ctrl)::value, 0xF, 0xF, false));
+        x = join(x, __builtin_bit_cast(V, t));
+    };
+    dpp(std::integral_constant<int, 0xB1>{});   // quad_perm [1, 0, 3, 2]
+    dpp(std::integral_constant<int, 0x4E>{});   // quad_perm [2, 3, 0, 1]
+    dpp(std::integral_constant<int, 0x141>{});  // row_half_mirror
+    dpp(std::integral_constant<int, 0x140>{});  // row_mirror
+    auto swap = [&](auto f) {  // of a value with itself: what the lower and the upper rows hold, in all of them
+        const Words t = __builtin_bit_cast(Words, x);
+        Words a, b;
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            const auto y = f(t.w[i]);
+            a.w[i] = y[0];
+            b.w[i] = y[1];
+        }
+        x = join(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b));
+    };
+    swap([](uint32_t v) { return __builtin_amdgcn_permlane16_swap(v, v, false, false); });
+    swap([](uint32_t v) { return __builtin_amdgcn_permlane32_swap(v, v, false, false); });
     return x;
 }
 
+__device__ __forceinline__ double wave_add(double x) {
+    return wave_join(x, [](double a, double b) { return a + b; });
+}
+
 __device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
-    return x;
+    return wave_join(x, [](float a, float b) { return fmaxf(a, b); });
 }
 
 // The largest t, of sign, exponent and 11 bits of the float, that at least n of the wave's keys reach (n <= 64), one
@@ -275,17 +308,19 @@ __global__ __launch_bounds__(kMergeThreads) void select_merge_kernel(const float
     for (int b = w; b < beams; b += kW) {
         const int parts = chunks * kWaves;
         const Sum* sm = sums + (first_row + b) * parts;
-        double m = -INFINITY;
-        for (int i = lane; i < parts; i += 64) m = fmax(m, sm[i].m);
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) m = fmax(m, __shfl_xor(m, o, 64));
+        const float score = scores[first_row + b];
+        const Sum p0 = lane < parts ? sm[lane] : Sum{-INFINITY, 0.0};
+        float best = static_cast<float>(p0.m);  // an fp32 value
+        for (int i = lane + 64; i < parts; i += 64) best = fmaxf(best, static_cast<float>(sm[i].m));
+        const double m = static_cast<double>(wave_max(best));
         double s = 0.0;
-        for (int i = lane; i < parts; i += 64) {
-            const Sum p = sm[i];
+        auto add = [&](const Sum& p) {
             if (p.m > -INFINITY || p.s != p.s) s += p.s * exp(p.m - m);
-        }
+        };
+        add(p0);
+        for (int i = lane + 64; i < parts; i += 64) add(sm[i]);
         s = wave_add(s);
-        const double at = static_cast<double>(scores[first_row + b]) - (m + log(s));
+        const double at = static_cast<double>(score) - (m + log(s));
         if (lane == 0) offset[b] = at == at ? at : -INFINITY;
     }
     if (tid == 0) l_n = 0;
@@ -380,7 +415,7 @@ __global__ __launch_bounds__(kMergeThreads) void select_merge_kernel(const float
 
 // ---- host side -------------------------------------------------------------------------------
 // Logits a thread: as few as leave 512 chunks, so that small calls use the chip's width and large ones read up to 64 logits a
-// thread at once and leave few candidates (128 rows of 128256: 14.8 + 8.6 us at 64, 15.0 + 12.5 at 32).
+// thread at once and leave few candidates (128 rows of 128256: 14.8 + 8.6 us at 64, 15.0 + 12.5 at 32, with sums joined through LDS).
 int per_thread(int64_t rows, int vocab) {
     int e = 8;
     while (e < 64 && rows * ((vocab + 2 * e * kThreads - 1) / (2 * e * kThreads)) >= 512) e *= 2;
