@@ -187,7 +187,8 @@ __global__ __launch_bounds__(kThreads) void attention_lanes_kernel(View v, AttnA
     const int begin = split * a.kps;
     if (begin >= s.total && split > 0) return;  // the first range of a sequence without rows writes zeros
     const int lpk = lanes_per_key(v.c.head_dim);
-    const RowState r = scan_row<T, C>(v, a, s, t - s.first, head, begin, min(s.total, begin + a.kps), lane, lpk, aligned != 0);
+    const int end = begin + min(s.total - begin, a.kps);  // kps may be INT32_MAX
+    const RowState r = scan_row<T, C>(v, a, s, t - s.first, head, begin, end, lane, lpk, aligned != 0);
     const int64_t part = s.total <= a.kps ? -1 : (static_cast<int64_t>(split) * a.in.tokens + t) * a.in.heads + head;
     write_state<T>(v, a, t, head, part, r, lane);
 }
@@ -1078,7 +1079,7 @@ __global__ __launch_bounds__(kThreads) void attention_merge_kernel(View v, AttnA
         if (t - max(v.c.cu[seq], 0) >= a.in.max_new) return;
     } else {
         const Span s = span_of(v, a, seq);
-        cut = int4{(s.total + a.kps - 1) / a.kps, t, a.in.tokens, 0};
+        cut = int4{s.total > 0 ? (s.total - 1) / a.kps + 1 : 0, t, a.in.tokens, 0};
     }
     if (cut.x <= 1) return;  // written by the range itself
     if (kPlanned && (cut.y < 0 || cut.z < 1 || cut.y + static_cast<int64_t>(cut.x - 1) * cut.z >= a.parts)) return;  // nor where cu descends
@@ -1236,7 +1237,8 @@ Plan plan(const View& v, const qmm_paged_query& in) {
         p.kind = Kind::kLanes;
         int64_t kps = 64;
         while (kps < most && (rows * ((most + kps - 1) / kps) > 16384 || (most + kps - 1) / kps > 1024)) kps *= 2;
-        p.kps = static_cast<int>(kps);
+        // a length that no longer fits its 32 bits is past `most`: one range takes everything
+        p.kps = static_cast<int>(std::min<int64_t>(kps, INT32_MAX));
         p.splits = static_cast<int>((most + kps - 1) / kps);
         p.merge = p.splits > 1;
         p.most_ranges = p.splits;
