@@ -34,9 +34,9 @@ struct Candidate {
     int32_t token;  // -1: none
 };
 
-// A monotone image of the float order; NaN (of either sign) as -inf.
+// A monotone image of the float order; both zeros alike, NaN (of either sign) as -inf.
 __device__ __forceinline__ uint32_t order_key(float x) {
-    const uint32_t u = __float_as_uint(x);
+    const uint32_t u = __float_as_uint(x + 0.0f);  // -0 becomes +0
     const uint32_t k = u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
     return x != x ? 0x007FFFFFu : k;
 }

@@ -1,0 +1,49 @@
+"""GPU tests of beam.select's order of equal totals: lower beam first, then the lower token, for zeros of either sign."""
+
+import pytest
+import torch
+
+import paged_reference as R
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+INF = float("inf")
+
+
+def _order(logits, scores):
+    """The call's parents and tokens, and the definition's."""
+    import beam
+    want = R.select(logits.double().cpu(), scores.double().cpu())
+    got = beam.select(logits, scores)
+    fin = want[0] > -INF
+    assert torch.equal(got[0].cpu() > -INF, fin)
+    assert ((got[0].double().cpu() - want[0]).abs()[fin] <= 2.0 ** -23 * want[0].abs()[fin] + 1e-6).all()
+    assert got[1].tolist() == want[1].tolist()
+    assert got[2].tolist() == want[2].tolist()
+
+
+def _signs(seed, shape):
+    g = torch.Generator().manual_seed(seed)
+    return torch.where(torch.rand(shape, generator=g) < 0.5, -torch.zeros(shape), torch.zeros(shape))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_zeros_of_either_sign_are_equal(cuda, dtype):
+    _order(torch.tensor([[[-0.0, 0.0]]], device="cuda").to(dtype), torch.zeros(1, 1, device="cuda"))
+    for V, W in ((40, 3), (5000, 1), (5000, 8), (70001, 4)):
+        x = -1.0 - torch.rand(2, W, V, generator=torch.Generator().manual_seed(V))
+        at = torch.randperm(V, generator=torch.Generator().manual_seed(W))[:min(V, 30)]
+        x[:, :, at] = _signs(V + W, (2, W, len(at)))  # the maximum, in many places
+        _order(x.to(dtype).cuda(), torch.zeros(2, W, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [33, 5000])
+def test_zeros_of_either_sign_at_the_cut(cuda, dtype, V):
+    """Nothing but zeros, and zeros below a few larger logits: which ones stay is the lowest tokens' matter."""
+    x = _signs(V, (2, 6, V))
+    _order(x.to(dtype).cuda(), torch.zeros(2, 6, device="cuda"))
+    x[:, :, V - 3:] = 1.0
+    x[0, 2, V // 2] = 2.0
+    _order(x.to(dtype).cuda(), torch.zeros(2, 6, device="cuda"))
