@@ -5,7 +5,8 @@
 //           as the logits, so the chunk's best `beams` logits are found there, beside its maximum and its sum
 //           of exp(x - max).
 //   Pass 2: one block per sentence joins the chunks' sums into each beam's logarithm, in 64 bits, and
-//           ranks the chunks' candidates by (total in 64 bits, beam, token).
+//           ranks the chunks' candidates by (total in 64 bits, beam, token).  A beam that is out (all of its totals count as
+//           -inf: its score or a logit is NaN, its score is -inf or a logit +inf) has its lowest tokens as candidates.
 // 128 rows of 128256 f16 logits (33 MB): 14.7 us of pass 1, whose blocks all run at once, so that its parts follow each
 // other (7.3 us of reading and maxima, 3 of exponentials, 4 of finding the candidates), and 8.0 us of pass 2, whose sixteen
 // blocks wait for loads and a 64-bit exponential and logarithm.
@@ -197,13 +198,7 @@ __global__ __launch_bounds__(kThreads) void select_chunk_kernel(const T* __restr
         return n + static_cast<int>(__popcll(mask));
     };
     int n = 0;
-    const bool dead = !(scores[row] > -INFINITY);  // every total is -inf: the lowest tokens stand for the rest
-    if (dead) {
-        if (w == 0) {
-            n = min(beams, vocab - first);  // a chunk holds at least 2048
-            if (lane < n) mine[lane] = static_cast<uint32_t>(~(first + lane));
-        }
-    } else {
+    if (scores[row] > -INFINITY) {  // the beam is out otherwise, and pass 2 needs no candidates of it
         // (a piece at a time: few hold one).  What lies past the vocabulary is -inf, and NaN reaches nothing, so a bound
         // of -inf takes the other way too.
         const float least = key_value(wave_threshold(order_key(lane_best), beams));
@@ -289,8 +284,8 @@ __device__ __forceinline__ bool better(double ta, int ba, int ja, double tb, int
 }
 
 __global__ __launch_bounds__(kMergeThreads) void select_merge_kernel(const float* __restrict__ scores, const Sum* __restrict__ sums,
-                                                                     const Candidate* __restrict__ cands, int beams, int chunks,
-                                                                     float* __restrict__ out_scores, int32_t* __restrict__ out_parents,
+                                                                     const Candidate* __restrict__ cands, int beams, int vocab,
+                                                                     int chunks, float* __restrict__ out_scores, int32_t* __restrict__ out_parents,
                                                                      int32_t* __restrict__ out_tokens) {
     constexpr int kW = kMergeThreads / 64;
     __shared__ double offset[kMaxBeams];  // score - logarithm; -inf: the beam is out
@@ -328,8 +323,14 @@ __global__ __launch_bounds__(kMergeThreads) void select_merge_kernel(const float
     auto total_of = [&](int i, int& b, int& token) {
         const Candidate c = i == tid ? own : cs[i];
         b = i / per_beam;
+        const double off = offset[b];
+        if (off == -INFINITY) {  // the beam is out: its lowest tokens
+            const int at = i - b * per_beam;
+            token = at < min(beams, vocab) ? at : -1;
+            return off;
+        }
         token = c.token;
-        const double t = static_cast<double>(c.x) + offset[b];
+        const double t = static_cast<double>(c.x) + off;
         return t == t ? t : -INFINITY;
     };
     // a bound that at least `beams` candidates of some wave reach: totals rounded to fp32 keep their order
@@ -484,7 +485,7 @@ int select(const void* logits, int dtype, int64_t sentence_stride, int64_t beam_
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return launched(e, "beam select kernel launch");
     hipLaunchKernelGGL(select_merge_kernel, dim3(static_cast<unsigned>(sentences)), dim3(kMergeThreads), 0, stream, scores, sums, cands,
-                       beams, p.chunks, out_scores, out_parents, out_tokens);
+                       beams, vocab, p.chunks, out_scores, out_parents, out_tokens);
     return launched(hipGetLastError(), "beam select merge kernel launch");
 }
 

@@ -1,4 +1,5 @@
-"""GPU tests of beam.select's order of equal totals: lower beam first, then the lower token, for zeros of either sign."""
+"""GPU tests of beam.select's order of equal totals: lower beam first, then the lower token, for zeros of either sign and for
+beams that are out."""
 
 import pytest
 import torch
@@ -47,3 +48,24 @@ def test_zeros_of_either_sign_at_the_cut(cuda, dtype, V):
     x[:, :, V - 3:] = 1.0
     x[0, 2, V // 2] = 2.0
     _order(x.to(dtype).cuda(), torch.zeros(2, 6, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bad", [float("nan"), INF])
+def test_a_beam_that_is_out_stands_for_its_lowest_tokens(cuda, dtype, bad):
+    """One logit that is NaN or infinite puts its beam out: all of its totals are -inf, and equal."""
+    g = torch.Generator().manual_seed(3)
+    for W, V in ((1, 7), (1, 5000), (3, 40000), (8, 5), (64, 2100)):
+        x = torch.randn(2, W, V, generator=g)
+        x[:, :, V // 2] = bad
+        _order(x.to(dtype).cuda(), torch.zeros(2, W, device="cuda"))
+    # a sentence with too few finite totals: the beam that is out fills up in order with the masked tokens of the others
+    x = torch.randn(1, 5, 6000, generator=g)
+    x[0, 1, 4000] = bad
+    x[0, 0, 2:] = x[0, 2:, 1:] = -INF
+    s = torch.tensor([[0.5, 0.0, -INF, -INF, float("nan")]], device="cuda")
+    _order(x.to(dtype).cuda(), s)
+
+
+def test_nothing_but_nan(cuda):
+    _order(torch.full((2, 3, 4000), float("nan"), device="cuda"), torch.zeros(2, 3, device="cuda"))
