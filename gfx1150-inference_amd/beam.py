@@ -14,11 +14,12 @@ import paged_module as _ops
 def select(logits, scores, stream=None):
     """``(scores, parents, tokens)``, each ``[sentences, beams]`` (float32, int32, int32), of the best
     ``beams`` totals ``scores[s, w] + log_softmax(logits[s, w])`` of each sentence in descending order; equal
-    totals go to the lower beam, then the lower token.
+    totals go to the lower beam, then the lower token.  Totals are formed in 64 bits; where a score's size makes
+    those of a beam's different logits equal (-1e30), the larger logit is the better one.
 
     ``logits`` ``[sentences, beams, vocab]`` float32, float16 or bfloat16 (vocab contiguous), ``scores``
     ``[sentences, beams]`` float32.  The first step of a search gives all beams but one a score of -inf.  A
-    total that is not a number counts as -inf."""
+    total that is not a number counts as -inf: all of a beam's where a logit is NaN or +inf."""
     return paged._on(stream, _ops.beam_select, logits, scores)
 
 

@@ -5,7 +5,8 @@
 //           as the logits, so the chunk's best `beams` logits are found there, beside its maximum and its sum
 //           of exp(x - max).
 //   Pass 2: one block per sentence joins the chunks' sums into each beam's logarithm, in 64 bits, and
-//           ranks the chunks' candidates by (total in 64 bits, beam, token).  A beam that is out (all of its totals count as
+//           ranks the chunks' candidates by (total in 64 bits, beam, logit, token): where a score's size leaves totals of
+//           different logits equal, a beam keeps the order of its logits, as pass 1 does.  A beam that is out (all of its totals count as
 //           -inf: its score or a logit is NaN, its score is -inf or a logit +inf) has its lowest tokens as candidates.
 // 128 rows of 128256 f16 logits (33 MB): 14.7 us of pass 1, whose blocks all run at once, so that its parts follow each
 // other (7.3 us of reading and maxima, 3 of exponentials, 4 of finding the candidates), and 8.0 us of pass 2, whose sixteen
@@ -279,8 +280,15 @@ __global__ __launch_bounds__(kThreads) void select_chunk_kernel(const T* __restr
     for (int i = total + tid; i < beams; i += kThreads) dst[i] = Candidate{0.0f, -1};
 }
 
-__device__ __forceinline__ bool better(double ta, int ba, int ja, double tb, int bb, int jb) {
-    return ta > tb || (ta == tb && (ba < bb || (ba == bb && ja < jb)));
+struct Entry {  // a candidate's beam, and its place there: the logit's order and then the lower token are larger
+    double total;
+    uint64_t place;
+    int beam;
+    __device__ __forceinline__ int token() const { return static_cast<int>(~static_cast<uint32_t>(place)); }
+};
+
+__device__ __forceinline__ bool better(const Entry& a, const Entry& b) {
+    return a.total > b.total || (a.total == b.total && (a.beam < b.beam || (a.beam == b.beam && a.place > b.place)));
 }
 
 __global__ __launch_bounds__(kMergeThreads) void select_merge_kernel(const float* __restrict__ scores, const Sum* __restrict__ sums,
@@ -290,11 +298,8 @@ __global__ __launch_bounds__(kMergeThreads) void select_merge_kernel(const float
     constexpr int kW = kMergeThreads / 64;
     __shared__ double offset[kMaxBeams];  // score - logarithm; -inf: the beam is out
     __shared__ uint32_t bounds[kW];
-    __shared__ double l_total[kMergeList];
-    __shared__ int2 l_at[kMergeList];
+    __shared__ Entry list[kMergeList], waves[kW];
     __shared__ int l_n;
-    __shared__ double r_total[kW];
-    __shared__ int2 r_at[kW];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t first_row = static_cast<int64_t>(blockIdx.x) * beams;
     const int per_beam = chunks * beams, n = beams * per_beam;
@@ -320,25 +325,26 @@ __global__ __launch_bounds__(kMergeThreads) void select_merge_kernel(const float
     }
     if (tid == 0) l_n = 0;
     __syncthreads();
-    auto total_of = [&](int i, int& b, int& token) {
+    auto entry_of = [&](int i, Entry& x) {  // false: there is none
         const Candidate c = i == tid ? own : cs[i];
-        b = i / per_beam;
-        const double off = offset[b];
+        x.beam = i / per_beam;
+        const double off = offset[x.beam];
         if (off == -INFINITY) {  // the beam is out: its lowest tokens
-            const int at = i - b * per_beam;
-            token = at < min(beams, vocab) ? at : -1;
-            return off;
+            const int at = i - x.beam * per_beam;
+            x.total = off;
+            x.place = static_cast<uint32_t>(~at);
+            return at < min(beams, vocab);
         }
-        token = c.token;
         const double t = static_cast<double>(c.x) + off;
-        return t == t ? t : -INFINITY;
+        x.total = t == t ? t : -INFINITY;
+        x.place = (static_cast<uint64_t>(order_key(c.x)) << 32) | static_cast<uint32_t>(~c.token);
+        return c.token >= 0;
     };
     // a bound that at least `beams` candidates of some wave reach: totals rounded to fp32 keep their order
     uint32_t best = 0;
     for (int i = tid; i < n; i += kMergeThreads) {
-        int b, token;
-        const double t = total_of(i, b, token);
-        if (token >= 0) best = max(best, order_key(static_cast<float>(t)));
+        Entry x;
+        if (entry_of(i, x)) best = max(best, order_key(static_cast<float>(x.total)));
     }
     const uint32_t t_wave = wave_threshold(best, beams);
     if (lane == 0) bounds[w] = t_wave;
@@ -346,70 +352,47 @@ __global__ __launch_bounds__(kMergeThreads) void select_merge_kernel(const float
     uint32_t bound = 0;
     for (int i = 0; i < kW; ++i) bound = max(bound, bounds[i]);
     for (int i = tid; i < n; i += kMergeThreads) {
-        int b, token;
-        const double t = total_of(i, b, token);
-        if (token >= 0 && order_key(static_cast<float>(t)) >= bound) {
+        Entry x;
+        if (entry_of(i, x) && order_key(static_cast<float>(x.total)) >= bound) {
             const int at = atomicAdd(&l_n, 1);
-            if (at < kMergeList) {
-                l_total[at] = t;
-                l_at[at] = int2{b, token};
-            }
+            if (at < kMergeList) list[at] = x;
         }
     }
     __syncthreads();
-    auto write = [&](int rank, double t, int2 at) {
-        out_scores[first_row + rank] = static_cast<float>(t);
-        out_parents[first_row + rank] = at.x;
-        out_tokens[first_row + rank] = at.y;
+    auto write = [&](int rank, const Entry& x) {
+        out_scores[first_row + rank] = static_cast<float>(x.total);
+        out_parents[first_row + rank] = x.beam;
+        out_tokens[first_row + rank] = x.token();
     };
     const int listed = l_n;
     if (listed <= kMergeList) {
         if (tid < listed) {
-            const double t = l_total[tid];
-            const int2 at = l_at[tid];
+            const Entry x = list[tid];
             int rank = 0;
-            for (int i = 0; i < listed; ++i) rank += better(l_total[i], l_at[i].x, l_at[i].y, t, at.x, at.y);
-            if (rank < beams) write(rank, t, at);
+            for (int i = 0; i < listed; ++i) rank += better(list[i], x);
+            if (rank < beams) write(rank, x);
         }
         return;
     }
     // Many equal totals: one after the other, each the best of those after the last one in order.
-    double last_t = INFINITY;
-    int2 last{-1, -1};
+    Entry last{INFINITY, 0, -1};
     for (int r = 0; r < beams; ++r) {
-        double bt = -INFINITY;
-        int2 ba{INT32_MAX, INT32_MAX};
+        Entry top{-INFINITY, 0, INT32_MAX};
         for (int i = tid; i < n; i += kMergeThreads) {
-            int b, token;
-            const double t = total_of(i, b, token);
-            if (token >= 0 && better(last_t, last.x, last.y, t, b, token) && better(t, b, token, bt, ba.x, ba.y)) {
-                bt = t;
-                ba = int2{b, token};
-            }
+            Entry x;
+            if (entry_of(i, x) && better(last, x) && better(x, top)) top = x;
         }
         for (int o = 32; o > 0; o >>= 1) {
-            const double ot = __shfl_xor(bt, o, 64);
-            const int2 oa{__shfl_xor(ba.x, o, 64), __shfl_xor(ba.y, o, 64)};
-            if (better(ot, oa.x, oa.y, bt, ba.x, ba.y)) {
-                bt = ot;
-                ba = oa;
-            }
+            const Entry x{__shfl_xor(top.total, o, 64), __shfl_xor(top.place, o, 64), __shfl_xor(top.beam, o, 64)};
+            if (better(x, top)) top = x;
         }
-        if (lane == 0) {
-            r_total[w] = bt;
-            r_at[w] = ba;
-        }
+        if (lane == 0) waves[w] = top;
         __syncthreads();
-        bt = r_total[0];
-        ba = r_at[0];
+        top = waves[0];
         for (int i = 1; i < kW; ++i)
-            if (better(r_total[i], r_at[i].x, r_at[i].y, bt, ba.x, ba.y)) {
-                bt = r_total[i];
-                ba = r_at[i];
-            }
-        last_t = bt;
-        last = ba;
-        if (tid == 0) write(r, bt, ba);
+            if (better(waves[i], top)) top = waves[i];
+        last = top;
+        if (tid == 0) write(r, top);
         __syncthreads();
     }
 }

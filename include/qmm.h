@@ -424,7 +424,9 @@ int qmm_paged_commit_path(const qmm_paged_kv* kv, const int32_t* path, int64_t p
 /* One step of beam search over logits [sentences][beams][vocab] (F32, F16 or BF16; strides in
  * elements, vocab contiguous): the `beams` best totals scores[s][w] + log_softmax(logits[s][w]) of each
  * sentence in descending order, with their beams and tokens; equal totals go to the lower beam, then
- * the lower token.  A beam whose total is not a number counts as -inf.  beams <= 64.  scores and the
+ * the lower token.  Totals are formed in 64 bits; where a score's size makes those of a beam's different
+ * logits equal, the larger logit is the better one.  A total that is not a number counts as -inf (all of a
+ * beam's where a logit is NaN or +inf).  beams <= 64.  scores and the
  * outputs are contiguous [sentences][beams].  `workspace`: qmm_beam_select_workspace() bytes, 16-byte
  * aligned, or NULL as above. */
 size_t qmm_beam_select_workspace(int dtype, int sentences, int beams, int vocab);

@@ -1,5 +1,5 @@
 """GPU tests of beam.select's order of equal totals: lower beam first, then the lower token, for zeros of either sign and for
-beams that are out."""
+beams that are out; where the totals of different logits round to one number, the larger logit."""
 
 import pytest
 import torch
@@ -69,3 +69,14 @@ def test_a_beam_that_is_out_stands_for_its_lowest_tokens(cuda, dtype, bad):
 
 def test_nothing_but_nan(cuda):
     _order(torch.full((2, 3, 4000), float("nan"), device="cuda"), torch.zeros(2, 3, device="cuda"))
+
+
+@pytest.mark.parametrize("score", [-1e30, 1e30, INF])
+def test_totals_that_round_to_one_number(cuda, score):
+    """A score beside which the logits vanish: within a beam the larger logit is still the better one."""
+    import beam
+    x = torch.randn(1, 3, 9000, generator=torch.Generator().manual_seed(4))
+    x[0, 0, [5, 8000]] = 9.0  # equal logits: the lower token
+    s, p, t = beam.select(x.cuda(), torch.full((1, 3), score, device="cuda"))
+    assert (s == score).all() and p.tolist() == [[0, 0, 0]]
+    assert t[0].tolist() == torch.sort(x[0, 0], descending=True, stable=True).indices[:3].tolist()
