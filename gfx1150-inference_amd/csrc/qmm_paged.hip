@@ -270,9 +270,9 @@ struct Strides {  // in units
 };
 
 // Commit of a path: block (x, b) takes 256 of the (layer, K or V, head, piece) columns of sequence b; a
-// thread moves its column of every step, eight loads in flight.  Step j reads row path[j] >= j and
-// writes row j, so in ascending order no step reads what an earlier batch of steps has overwritten, and
-// within a batch the loads come first.  The steps that move something are listed in LDS first.  48 sequences, up to 6 rows
+// thread moves its column of every step, eight loads in flight.  The j-th node that is taken, path's j-th entry or a
+// later one, is at least j where the path ascends, and its row becomes row j: in that order no step reads what an earlier
+// batch of steps has overwritten, and within a batch the loads come first.  The steps that move something are listed in LDS first.  48 sequences, up to 6 rows
 // in 32 layers (38 MB read and written): 8.2 us, of which 4 are the launch and the chain of loads before the first row.
 constexpr int kSteps = 64, kInFlight = 8;
 
@@ -301,18 +301,20 @@ __global__ __launch_bounds__(kThreads) void commit_kernel(View v, Strides st, co
             const int j = j0 + lane;
             const int node = j < path_len ? path[b * path_stride + j] : -1;
             const bool live = node >= 0 && node < n_new;
+            const uint64_t below = (uint64_t{1} << lane) - 1, lives = __ballot(live);
+            const int to = taken + static_cast<int>(__popcll(lives & below));
             int4 m{-1, 0, -1, 0};
-            if (live && node != j) {
+            if (live && node != to) {
                 m.x = page_of(v, b, ctx + node);
                 m.y = (ctx + node) & (v.c.page_size - 1);
-                m.z = page_of(v, b, ctx + j);
-                m.w = (ctx + j) & (v.c.page_size - 1);
+                m.z = page_of(v, b, ctx + to);
+                m.w = (ctx + to) & (v.c.page_size - 1);
             }
             const bool moves_row = m.x >= 0 && m.z >= 0;
             const uint64_t mask = __ballot(moves_row);
-            if (moves_row) moves[__popcll(mask & ((uint64_t{1} << lane) - 1))] = m;
+            if (moves_row) moves[__popcll(mask & below)] = m;
             if (lane == 0) n_moves = __popcll(mask);
-            taken += __popcll(__ballot(live));
+            taken += __popcll(lives);
         }
         __syncthreads();
         const int n = n_moves;

@@ -59,8 +59,8 @@ def tree_attention(q, k_cache, v_cache, table, cu, ctx, mask=None, max_new=None,
 
 
 def commit_path(k_cache, v_cache, table, cu, ctx, path, stream=None):
-    """Keeps the accepted path of each sequence's drafted tree: row ``ctx[b] + path[b, j]`` becomes row
+    """Keeps the accepted path of each sequence's drafted tree: row ``ctx[b] + node`` of the path's j-th node becomes row
     ``ctx[b] + j`` in every layer of ``k_cache`` and ``v_cache`` ``[layers, pages, kv_heads, page_size, head_dim]``.
-    ``path`` ``[batch, steps]`` int32 holds ascending nodes, padded with -1.  Returns the sequences' new lengths,
-    ``ctx`` plus the path's nodes."""
+    ``path`` ``[batch, steps]`` int32 holds ascending nodes; entries that are none of the sequence's new tokens, as the
+    -1 of padding, are passed over.  Returns the sequences' new lengths, ``ctx`` plus the path's nodes."""
     return _on(stream, _ops.commit_path, k_cache, v_cache, table, cu, ctx, path)

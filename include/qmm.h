@@ -414,9 +414,9 @@ size_t qmm_paged_attention_workspace(const qmm_paged_kv* kv, const qmm_paged_que
 int qmm_paged_tree_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, void* workspace, size_t workspace_bytes,
                              void* stream);
 
-/* After a drafted tree was verified: row ctx[b] + j of sequence b becomes its row ctx[b] + path[b][j],
- * in every layer, for each entry of path ([batch][path_len], rows path_stride apart; entries outside
- * the sequence's new tokens, -1 among them, are skipped), and lens[b] = ctx[b] + the entries taken.
+/* After a drafted tree was verified: in every layer, row ctx[b] + node of sequence b becomes its row
+ * ctx[b] + j for the j-th node of path ([batch][path_len], rows path_stride apart; entries outside the
+ * sequence's new tokens, -1 among them, are no nodes and not counted), and lens[b] = ctx[b] + the nodes.
  * A path ascends, as the nodes of a tree do whose parents come first. */
 int qmm_paged_commit_path(const qmm_paged_kv* kv, const int32_t* path, int64_t path_stride, int path_len, int32_t* lens,
                           void* stream);

@@ -1,4 +1,7 @@
-"""GPU tests of the paged calls' far ends: tables with room for more rows than 32 bits count."""
+"""GPU tests of the paged calls' far ends: tables with room for more rows than 32 bits count, paths with entries that
+are no nodes."""
+
+import random
 
 import pytest
 import torch
@@ -26,3 +29,42 @@ def test_attention_with_a_table_of_more_than_2_to_the_30_rows(cuda, n):
     want, spread = R.attention(q.double(), k.double(), v.double(), [table[0][:1]], [0, n], [ctx], page)
     # the output's rounding, and fp32 scores and sums
     assert ((got - want).abs() <= 2.0 ** -11 * want.abs() + 4e-5 * spread + 1e-7).all()
+
+
+@pytest.mark.parametrize("path", [[0, 2, 20, -5, 4, 18], [-1] + list(range(12)), [-1, -1, 3, 5, 9, -7, 11, 99, 12, 13, 14, 15, 19],
+                                  [-1] * 70 + [1, 4, 6, -1, 7] + [-1] * 60 + [8, 15]], ids=lambda p: str(len(p)))
+def test_commit_path_closes_up_over_skipped_entries(cuda, path):
+    """The k-th entry that is a node becomes row ctx + k, so that `lens` counts the rows that were kept."""
+    import paged
+    ctx, n, page = 13, 20, 16
+    table = [2, 0, 1]
+    k, v = (torch.randn(2, 3, 2, page, 64, device="cuda").half() for _ in range(2))
+    want = [k.clone(), v.clone()]
+    nodes = [p for p in path if 0 <= p < n]
+    for w, src in zip(want, (k.clone(), v.clone())):
+        for j, node in enumerate(nodes):
+            d, s = ctx + j, ctx + node
+            w[:, table[d // page], :, d % page] = src[:, table[s // page], :, s % page]
+    lens = paged.commit_path(k, v, _ints([table]), _ints([0, n]), _ints([ctx]), _ints([path]))
+    assert lens.tolist() == [ctx + len(nodes)]
+    assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+
+
+def test_commit_path_of_many_skipped_entries(cuda):
+    import paged
+    rng = random.Random(5)
+    B, n, page = 6, 200, 32
+    k = torch.randn(1, 8 * B, 1, page, 64, device="cuda").half()
+    table = [list(range(8 * b, 8 * b + 8)) for b in range(B)]
+    ctx = [rng.randint(0, 50) for _ in range(B)]
+    paths = [[x for node in sorted(rng.sample(range(n), 90)) for x in ([node] if rng.random() < 0.6 else [-1, node])][:100] for _ in range(B)]
+    paths = [p + [-1] * (100 - len(p)) for p in paths]
+    want = k.clone()
+    for b, p in enumerate(paths):
+        for j, node in enumerate(x for x in p if x >= 0):
+            d, s = ctx[b] + j, ctx[b] + node
+            want[:, table[b][d // page], :, d % page] = k[:, table[b][s // page], :, s % page]
+    v = k.clone()
+    lens = paged.commit_path(k, v, _ints(table), _ints([n * b for b in range(B + 1)]), _ints(ctx), _ints(paths))
+    assert lens.tolist() == [c + sum(x >= 0 for x in p) for c, p in zip(ctx, paths)]
+    assert torch.equal(k, want) and torch.equal(v, want)
