@@ -200,8 +200,8 @@ Tensor tree_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_ca
     in.max_new = int_of(max_new.value_or(tokens), "max_new");
     in.heads = int_of(q.size(1), "heads");
     in.dtype = code_of(dtype);
-    require(!scale || *scale != 0.0, "scale must not be 0");
-    in.scale = static_cast<float>(scale.value_or(0.0));
+    in.scale = static_cast<float>(scale.value_or(0.0));  // 0: the default
+    require(!scale || in.scale != 0.0f, "scale must not be 0 in 32 bits");
     void* stream = stream_of(k_cache.device());
     const size_t need = qmm_paged_attention_workspace(&kv, &in);
     Tensor space;  // the allocator's: safe to capture

@@ -1,5 +1,5 @@
 """GPU tests of the paged calls' far ends: tables with room for more rows than 32 bits count, paths with entries that
-are no nodes."""
+are no nodes, arguments that vanish in 32 bits."""
 
 import random
 
@@ -68,3 +68,18 @@ def test_commit_path_of_many_skipped_entries(cuda):
     lens = paged.commit_path(k, v, _ints(table), _ints([n * b for b in range(B + 1)]), _ints(ctx), _ints(paths))
     assert lens.tolist() == [c + sum(x >= 0 for x in p) for c, p in zip(ctx, paths)]
     assert torch.equal(k, want) and torch.equal(v, want)
+
+
+def _small(**kw):
+    args = dict(q=torch.ones(1, 2, 64, device="cuda").half(), k_cache=torch.ones(2, 1, 16, 64, device="cuda").half(),
+                v_cache=torch.ones(2, 1, 16, 64, device="cuda").half(), table=_ints([[0, 1]]), cu=_ints([0, 1]), ctx=_ints([17]))
+    args.update(kw)
+    return args
+
+
+@pytest.mark.parametrize("scale", [1e-50, -1e-60])
+def test_a_scale_that_fp32_has_as_zero_is_refused(cuda, scale):
+    """It must not become the default of 1 / sqrt(head_dim)."""
+    import paged
+    with pytest.raises(ValueError, match="scale"):
+        paged.tree_attention(**_small(scale=scale))
