@@ -51,9 +51,9 @@ std::string shape_of(const Tensor& t) {
     return s.str();
 }
 
-// An int32 index tensor, its last dimension contiguous; sizes of -1 are free.
+// An int32 index tensor, its last dimension contiguous (one entry always is); sizes of -1 are free.
 void check_ints(const Tensor& t, const char* name, std::initializer_list<int64_t> sizes, c10::Device device) {
-    if (t.scalar_type() != at::kInt || t.device() != device || t.dim() != static_cast<int64_t>(sizes.size()) || (t.numel() > 0 && t.stride(-1) != 1))
+    if (t.scalar_type() != at::kInt || t.device() != device || t.dim() != static_cast<int64_t>(sizes.size()) || (t.numel() > 0 && t.size(-1) > 1 && t.stride(-1) != 1))
         throw py::value_error(std::string(name) + " must be an int32 tensor of " + std::to_string(sizes.size()) +
                               " dimension(s) on the cache's device, its last one contiguous");
     int64_t d = 0;

@@ -1,5 +1,5 @@
 """GPU tests of the paged calls' far ends: tables with room for more rows than 32 bits count, paths with entries that
-are no nodes, arguments that vanish in 32 bits."""
+are no nodes, arguments that vanish in 32 bits or look strided."""
 
 import random
 
@@ -83,3 +83,18 @@ def test_a_scale_that_fp32_has_as_zero_is_refused(cuda, scale):
     import paged
     with pytest.raises(ValueError, match="scale"):
         paged.tree_attention(**_small(scale=scale))
+
+
+def test_single_entries_of_wider_tensors(cuda):
+    """One entry is contiguous whatever its stride says."""
+    import paged
+    a = _small()
+    want = paged.tree_attention(**a)
+    wide = torch.zeros(1, 7, dtype=torch.int32, device="cuda")
+    wide[0, 3] = 17
+    assert wide[:, 3].stride(0) != 1
+    assert torch.equal(paged.tree_attention(**_small(ctx=wide[:, 3])), want)
+    narrow = torch.zeros(1, 2, 5, dtype=torch.int32, device="cuda")[:, :1, 4]
+    assert narrow.shape == (1, 1) and narrow.stride(1) != 1
+    one = paged.tree_attention(**_small(ctx=_ints([3]), table=_ints([[0]])))
+    assert torch.equal(paged.tree_attention(**_small(ctx=_ints([3]), table=narrow)), one)
