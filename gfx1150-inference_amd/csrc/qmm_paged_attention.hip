@@ -1269,6 +1269,12 @@ Plan plan(const View& v, const qmm_paged_query& in) {
     return p;
 }
 
+// What a score in base 2 is of the product with the stored key.
+float score_scale(const View& v, const qmm_paged_query& in) {
+    const float scale = in.scale != 0.0f ? in.scale : 1.0f / std::sqrt(static_cast<float>(v.c.head_dim));
+    return scale * v.c.k_scale * 1.4426950408889634f;
+}
+
 int check_query(const qmm_paged_kv* kv, const qmm_paged_query* in, View* v) {
     const int rc = check_view(kv, true, v);
     if (rc != QMM_OK) return rc;
@@ -1278,6 +1284,7 @@ int check_query(const qmm_paged_kv* kv, const qmm_paged_query* in, View* v) {
     if (in->heads <= 0 || in->heads % v->c.kv_heads != 0) return bad("heads must be divisible by kv_heads.");
     if (in->tokens < 0 || in->max_new < 0 || in->mask_words < 0) return bad("tokens, max_new and mask_words must be non-negative.");
     if (!std::isfinite(in->scale)) return bad("scale must be finite.");
+    if (!std::isnormal(score_scale(*v, *in))) return bad("scale * k_scale is out of fp32's range.");
     if (in->tokens > 0 && v->c.batch > 0 && (!in->q || !in->out)) return bad("q and out must be non-null.");
     if ((reinterpret_cast<uintptr_t>(in->q) | reinterpret_cast<uintptr_t>(in->out)) % 2 != 0) return bad("q and out must be aligned to their elements.");
     if (in->heads > 65535) return bad("too many heads.");
@@ -1309,8 +1316,7 @@ int tree_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, void* work
     }
     AttnArgs a{};
     a.in = *in;
-    const float scale = in->scale != 0.0f ? in->scale : 1.0f / std::sqrt(static_cast<float>(v.c.head_dim));
-    a.scale_log2 = scale * v.c.k_scale * 1.4426950408889634f;
+    a.scale_log2 = score_scale(v, *in);
     a.v_scale = v.c.v_scale;
     a.kps = p.kps;
     a.slots = p.slots;
