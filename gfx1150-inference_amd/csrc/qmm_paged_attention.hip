@@ -318,13 +318,14 @@ struct CallPlan {
     // whose roundings are the same everywhere.
     __device__ __forceinline__ bool find(const View& v, const AttnArgs& a, int at, int lane) {
         const int kvh = v.c.kv_heads;
-        float work = 0.0f;
+        double own_work = 0.0;  // of this lane's sequences, up to a thousand: no rounding, whatever the batch
         Lane x{};
         for (int b0 = 0; b0 < v.c.batch; b0 += 64) {
             x = lane_of(v, a, b0 + lane);
-            work += wave_total(x.work);
+            own_work += static_cast<double>(x.work);
         }
-        // 1e-5 covers the roundings: a length is never below W / slots, or it is 2^25 steps, which no sequence passes
+        const float work = wave_total(static_cast<float>(own_work));
+        // 1e-5 covers the ten roundings from here on (and one in a lane's work): a length is never below W / slots, or it is 2^25 steps, which no sequence passes
         const float shortest = work * static_cast<float>(kvh) / static_cast<float>(a.slots) * 1.00001f;
         int u[kTries];
         float count[kTries];
