@@ -83,6 +83,10 @@ def ints(x):
     return torch.tensor(x, dtype=torch.int32, device="cuda")
 
 
+def pages_of(table):
+    return {p for row in table.tolist() for p in row if p >= 0}
+
+
 def starts(counts):
     cu = [0]
     for n in counts:
@@ -173,6 +177,7 @@ def beams(model, cache, prompt, steps, width):
     if len(tables[0]) > full:
         for p in open_pages:
             cache.k[:, p], cache.v[:, p] = cache.k[:, tables[0][full]], cache.v[:, tables[0][full]]
+        cache.free += tables[0][full:]
     room = -(-(ctx[0] + steps) // cache.page_size) + 1
     table = ints([tables[0][:full] + [p] + [-1] * (room - full - 1) for p in open_pages])
     lens = ints([ctx[0]] * width)
@@ -187,10 +192,10 @@ def beams(model, cache, prompt, steps, width):
         if step + 1 == steps:
             break
         spare = [cache.free.pop() for _ in range(width)]
-        old = table
+        before = pages_of(table)
         table, lens = beam.reorder(cache.k, cache.v, table, lens, parents, ints([spare]))
-        # the open pages of before are free again (none where the last one was just filled)
-        cache.free += [p for p in (int(old[w, int(n) // cache.page_size]) for w, n in enumerate(lens)) if p >= 0]
+        # what no hypothesis holds any more is free again: the open pages of before, and full ones of dropped hypotheses
+        cache.free += before - pages_of(table)
         logits = model.forward(chosen[0].long(), cache, table, one, lens, max_new=1).view(1, width, -1)
         lens = lens + 1
     return scores[0].tolist(), tokens
