@@ -298,7 +298,10 @@ __global__ __launch_bounds__(kMergeThreads) void select_merge_kernel(const float
     constexpr int kW = kMergeThreads / 64;
     __shared__ double offset[kMaxBeams];  // score - logarithm; -inf: the beam is out
     __shared__ uint32_t bounds[kW];
-    __shared__ Entry list[kMergeList], waves[kW];
+    __shared__ double l_total[kMergeList];
+    __shared__ uint64_t l_place[kMergeList];
+    __shared__ int l_beam[kMergeList];
+    __shared__ Entry waves[kW];
     __shared__ int l_n;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t first_row = static_cast<int64_t>(blockIdx.x) * beams;
@@ -355,7 +358,11 @@ __global__ __launch_bounds__(kMergeThreads) void select_merge_kernel(const float
         Entry x;
         if (entry_of(i, x) && order_key(static_cast<float>(x.total)) >= bound) {
             const int at = atomicAdd(&l_n, 1);
-            if (at < kMergeList) list[at] = x;
+            if (at < kMergeList) {
+                l_total[at] = x.total;
+                l_place[at] = x.place;
+                l_beam[at] = x.beam;
+            }
         }
     }
     __syncthreads();
@@ -367,9 +374,15 @@ __global__ __launch_bounds__(kMergeThreads) void select_merge_kernel(const float
     const int listed = l_n;
     if (listed <= kMergeList) {
         if (tid < listed) {
-            const Entry x = list[tid];
-            int rank = 0;
-            for (int i = 0; i < listed; ++i) rank += better(list[i], x);
+            const Entry x{l_total[tid], l_place[tid], l_beam[tid]};
+            int rank = 0, equal = 0;
+            for (int i = 0; i < listed; ++i) {
+                const double t = l_total[i];
+                rank += t > x.total;
+                equal += t == x.total;
+            }
+            if (equal > 1)  // few: the places of these alone
+                for (int i = 0; i < listed; ++i) rank += l_total[i] == x.total && better(Entry{x.total, l_place[i], l_beam[i]}, x);
             if (rank < beams) write(rank, x);
         }
         return;
