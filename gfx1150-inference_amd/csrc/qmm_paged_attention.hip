@@ -5,7 +5,8 @@
 //
 // The keys of a sequence are cut into ranges, one workgroup each, where the rows alone leave the chip idle; a
 // range's maximum (base 2), sum and unnormalised output are joined by a second kernel in the order of the ranges,
-// so a result depends on the call's lengths alone.  How long a range is, every workgroup works out from all
+// so a call repeats itself to the bit.  Its bits go by what chooses the kernel and the cut: all sequences' lengths,
+// max_new, alignment, the workgroups that the device runs at once, and, on the vector ALUs, the table's width.  How long a range is, every workgroup works out from all
 // sequences' lengths, which only the device knows (plan_call): the host sees no more than the width of the table.
 #include "qmm_device.h"
 #include "qmm_paged.h"
@@ -419,7 +420,8 @@ __device__ __forceinline__ void load_row_bytes(uint32_t* dst, const char* src) {
 //     row) and v_perm transposes them in registers.
 // With one row tile the weights enter as hi + lo in the operands' type, two products: 16 bits and more, where memory
 // hides them.  With more tiles the products are a good part of the time and the weights are rounded once, half a
-// step of each weight (as large as the output's own rounding, and of either sign).
+// step of each weight (as large as the output's own rounding, and of either sign): f16 outputs of 13-node trees are
+// 2.8e-4 off in the 2-norm, 2.1e-4 with hi + lo, which is their own rounding; the kernel takes 42 us, 49 with hi + lo.
 // The 4 waves take every fourth 32-key block of the range; above 32 rows two take half of the rows each (RG = 2), their
 // keys from the L1 cache: one wave's 64 rows of head_dim 128 leave no registers for a second wave on the SIMD (an fp8 cache
 // of 57000 rows, 52 rows a kv head: 51 us with four row tiles a wave, 42 us).  Joined through LDS in wave order.
@@ -701,7 +703,8 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
 //     keys, the partner lane (lane ^ 32) the others;
 //   * the weights go from the S registers into O^T += V^T P^T without leaving the lane (the k order of each 16-key
 //     block is the order the lane holds its keys in).  Weights are rounded to the operands' type once, half a step, of
-//     either sign, and their sum is of the rounded ones;
+//     either sign, and their sum, in fp32, is of the rounded ones.  As hi + lo they would bring the 2-norm of f16 outputs'
+//     errors from 2.8e-4 to the outputs' own rounding, 2.1e-4, and 63-node trees from 91 to 122 us (500 tokens: 44 to 57);
 //   * the next tile's scores are formed beside this tile's weights, so keys are copied two tiles ahead, values one;
 //   * the lanes keep sums of their own; maxima are exchanged only when the running one moves (kSlack).
 // Wave w stages keys 16 w .. 16 w + 15 of a tile, which share a page: a scalar address and lane offsets that never change,
@@ -709,9 +712,10 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
 // and V lie as they are in memory, with the 16-byte pieces of a row exchanged by its number (TileGeom) so that neither the
 // key fragments (16 rows, one piece) nor V's transposing reads (ds_read_b64_tr_b16: half a wave takes four pieces of 4
 // rows) meet on a bank.
-// Bound by the vector work of the weights beside the products, and in short calls by the start (plan, queries, first tile: 10 us)
-// and the partial results.  63-node trees of eight users, 64 heads of 128 over up to 8191 keys (66 GFLOP): 91 us; chunks of up to 500
-// tokens, 32 heads of 64 (16 GFLOP): 44 us.  The kv heads come fastest in the grid: with 8 of them
+// Bound by what one or two waves a SIMD can have under way, and in short calls by the start (plan, queries, first tile: 10 us)
+// and the partial results.  63-node trees of eight users, 64 heads of 128 over up to 8191 keys (66 GFLOP): 91-93 us, matrix
+// cores busy for 33 % of the SIMDs' cycles and vector ALUs for 35 %; chunks of up to 500 tokens, 32 heads of 64 (16 GFLOP):
+// 44 us, 14 and 34 % with 1.2 waves a SIMD in the mean (the same buffers in every pass, without the join).  The kv heads come fastest in the grid: with 8 of them
 // (or 16, ..) the row tiles of one meet on one XCD and its keys in one L2.
 constexpr int kTileRows = 128, kTileKeys = 64;
 

@@ -11,7 +11,8 @@ For batches of sequences whose rows live in pages of one pool.  The caller owns 
 A decoding step of a model calls, per layer, ``append`` and ``tree_attention``; a step with drafted
 tokens ends with one ``commit_path`` over all layers.  Every call is asynchronous on ``stream`` (the
 current one by default) and can be captured into a graph.  The indices are read on the device: a row whose
-page is outside the table or the pool is not written, copied or seen.
+page is outside the table or the pool is not written, copied or seen, and a token that ``cu`` gives to no sequence
+(padding) is passed over: its row of ``q_out`` or ``out`` is left as it was, uninitialised in a new tensor.
 """
 
 from __future__ import annotations
@@ -54,7 +55,8 @@ def tree_attention(q, k_cache, v_cache, table, cu, ctx, mask=None, max_new=None,
     ancestors and itself), or those up to itself without a mask: one token is a decoding step, many
     a chunk of a prompt.  A token that sees nothing gets zeros, and a row that it does not see has no effect
     on it, NaN or not.  Query head h reads kv head ``h // (heads // kv_heads)``.  ``max_new`` bounds the
-    new tokens of any one sequence (``tokens`` by default); knowing it, a call starts fewer workgroups."""
+    new tokens of any one sequence (``tokens`` by default); tokens past it may be left out.  Give it where it is known:
+    without it a batch of many single tokens is taken for one long sequence and runs in tiles of 128 rows."""
     return _on(stream, _ops.tree_attention, q, k_cache, v_cache, table, cu, ctx, mask, max_new, scale, k_scale, v_scale, out)
 
 

@@ -352,7 +352,8 @@ int qmm_forward_layer_host(const qmm_layer_config* cfg, const qmm_layer_weights*
  * table[b][i / page_size].  Sequence b holds ctx[b] rows and has the new tokens
  * cu[b] .. cu[b + 1] - 1 of the call's `tokens` (concatenated; a sequence may have none; cu does not
  * descend); they take the rows ctx[b], ctx[b] + 1, ...  table, cu and ctx are read on the device: a row
- * whose page is outside the table or the pool is not written, copied or seen.
+ * whose page is outside the table or the pool is not written, copied or seen, and the outputs of a token
+ * that cu gives to no sequence are not written.
  * --------------------------------------------------------------------------------- */
 typedef struct qmm_paged_kv {
     void* k;
@@ -395,7 +396,7 @@ int qmm_paged_append(const qmm_paged_kv* kv, const qmm_paged_new* in, void* stre
  * unless that is E4M3).  New token i of a sequence sees its ctx cached rows and, of the sequence's
  * new rows j, those whose bit j % 32 of mask[token][j / 32] is set (words past mask_words: not
  * seen), or j <= i when mask is NULL.  scale 0 means 1 / sqrt(head_dim).  No sequence has more than
- * max_new new tokens (tokens past that are not computed). */
+ * max_new new tokens (tokens past that may be left out). */
 typedef struct qmm_paged_query {
     const void* q;
     void* out;
