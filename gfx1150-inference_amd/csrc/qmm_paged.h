@@ -33,12 +33,17 @@ struct View {
     int page_shift;
 };
 
-// Page id of row `row` of sequence `seq`, -1 where the table or the pool has no such page.
+// Page id of row `row` of sequence `seq`, -1 where the table or the pool has no such page (a row past 2^31 is negative).
 __device__ __forceinline__ int page_of(const View& v, int seq, int row) {
     const int p = row >> v.page_shift;
-    if (p >= v.c.table_width) return -1;
+    if (static_cast<uint32_t>(p) >= static_cast<uint32_t>(v.c.table_width)) return -1;
     const int id = v.c.table[static_cast<int64_t>(seq) * v.c.table_stride + p];
     return static_cast<uint32_t>(id) < static_cast<uint32_t>(v.c.num_pages) ? id : -1;
+}
+
+// Row `i` behind the cached ones; past 2^31 it is negative, and on no page.
+__device__ __forceinline__ int row_of(const View& v, int seq, int i) {
+    return static_cast<int>(static_cast<uint32_t>(min(max(v.c.ctx[seq], 0), 1 << 30)) + static_cast<uint32_t>(i));
 }
 
 // The sequence of token t: the count of ends cu[1..batch] at or below it (every lane of the wave must be

@@ -1,5 +1,6 @@
 """GPU tests of the paged calls' far ends: tables with room for more rows than 32 bits count, paths with entries that
-are no nodes, arguments that vanish in 32 bits or look strided."""
+are no nodes, arguments that vanish in 32 bits or look strided,
+indices out of every range."""
 
 import random
 
@@ -98,3 +99,28 @@ def test_single_entries_of_wider_tensors(cuda):
     assert narrow.shape == (1, 1) and narrow.stride(1) != 1
     one = paged.tree_attention(**_small(ctx=_ints([3]), table=_ints([[0]])))
     assert torch.equal(paged.tree_attention(**_small(ctx=_ints([3]), table=narrow)), one)
+
+
+@pytest.mark.parametrize("first,last", [(-2 ** 31, 3), (-5, 3), (-2 ** 31, -2 ** 31), (2 ** 31 - 1, 2 ** 31 - 1), (0, 2 ** 31 - 1)])
+@pytest.mark.parametrize("ctx", [2 ** 31 - 1, -2 ** 31, 14])
+def test_indices_of_any_value_stay_within_table_and_pool(cuda, first, last, ctx):
+    """Ends of the new tokens and lengths that no call should have: what is written is a token's own row, or nothing."""
+    import beam
+    import paged
+    page, D = 16, 64
+    kc, vc = (torch.full((3, 1, page, D), 7.0, device="cuda").half() for _ in range(2))
+    table, cu, c = _ints([[2, 0]]), _ints([first, last]), _ints([ctx])
+    x = torch.arange(1, 4, device="cuda").half()[:, None, None].expand(3, 1, D).contiguous()
+    paged.append(x, x, kc, vc, table, cu, c, rotary_dim=0)
+    want = torch.full((3, 1, page, D), 7.0).half()
+    if first <= 0 < last and ctx <= 14:
+        for i in range(3):
+            row = max(ctx, 0) + i
+            want[[2, 0][row // page], 0, row % page] = i + 1
+    assert torch.equal(kc.cpu(), want) and torch.equal(vc.cpu(), want)
+    paged.tree_attention(x, kc, vc, table, cu, c)
+    before = kc.clone()
+    lens = paged.commit_path(kc[None], vc[None], table, cu, c, _ints([[2 ** 31 - 2, 2 ** 30, -7]]))
+    assert torch.equal(kc, before) and torch.equal(vc, before) and lens.shape == (1,)
+    beam.reorder(kc[None], vc[None], table, c, _ints([[-2 ** 31]]), _ints([[2 ** 31 - 1]]))
+    assert torch.equal(kc, before) and torch.equal(vc, before)
