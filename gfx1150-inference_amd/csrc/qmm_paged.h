@@ -41,9 +41,12 @@ __device__ __forceinline__ int page_of(const View& v, int seq, int row) {
     return static_cast<uint32_t>(id) < static_cast<uint32_t>(v.c.num_pages) ? id : -1;
 }
 
-// Row `i` behind the cached ones; past 2^31 it is negative, and on no page.
-__device__ __forceinline__ int row_of(const View& v, int seq, int i) {
-    return static_cast<int>(static_cast<uint32_t>(min(max(v.c.ctx[seq], 0), 1 << 30)) + static_cast<uint32_t>(i));
+// Cached rows of a sequence, as every call takes them.
+__device__ __forceinline__ int cached_rows(const View& v, int seq) { return min(max(v.c.ctx[seq], 0), 1 << 30); }
+
+// Row `i` behind `cached` ones; past 2^31 it is negative, and on no page.
+__device__ __forceinline__ int row_behind(int cached, int i) {
+    return static_cast<int>(static_cast<uint32_t>(cached) + static_cast<uint32_t>(i));
 }
 
 // The sequence of token t: the count of ends cu[1..batch] at or below it (every lane of the wave must be

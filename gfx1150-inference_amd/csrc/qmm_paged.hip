@@ -127,7 +127,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(View v, AppendArgs a, 
     }
     const int seq = sequence_of(v, t, tid & 63);
     if (seq >= v.c.batch || t < v.c.cu[seq]) return;  // a token of no sequence (the same in every wave)
-    const int row = row_of(v, seq, t - max(v.c.cu[seq], 0));
+    const int row = row_behind(cached_rows(v, seq), t - max(v.c.cu[seq], 0));
     const int page = page_of(v, seq, row), slot = row & (v.c.page_size - 1);
     if (half > 0) {
         const int pos = a.in.positions ? a.in.positions[t] : row;
@@ -195,7 +195,7 @@ __global__ __launch_bounds__(kThreads) void append_scalar_kernel(View v, AppendA
     const int D = v.c.head_dim, heads = a.in.q ? a.in.heads : 0, kvh = v.c.kv_heads, half = a.in.rotary_dim / 2;
     const int seq = sequence_of(v, t, tid & 63);
     if (seq >= v.c.batch || t < v.c.cu[seq]) return;
-    const int row = row_of(v, seq, t - max(v.c.cu[seq], 0));
+    const int row = row_behind(cached_rows(v, seq), t - max(v.c.cu[seq], 0));
     const int page = page_of(v, seq, row), slot = row & (v.c.page_size - 1);
     if (half > 0) {
         const int pos = a.in.positions ? a.in.positions[t] : row;
@@ -283,7 +283,7 @@ __global__ __launch_bounds__(kThreads) void commit_kernel(View v, Strides st, co
     __shared__ int4 moves[kSteps];  // source page, slot; target page, slot
     __shared__ int n_moves;
     const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
-    const int ctx = min(max(v.c.ctx[b], 0), 1 << 30), n_new = max(v.c.cu[b + 1], 0) - max(v.c.cu[b], 0);
+    const int ctx = cached_rows(v, b), n_new = max(v.c.cu[b + 1], 0) - max(v.c.cu[b], 0);
     const int64_t columns = static_cast<int64_t>(v.c.num_layers) * 2 * v.c.kv_heads * st.per_row;
     const int64_t col = static_cast<int64_t>(blockIdx.x) * kThreads + tid;
     const int piece = static_cast<int>(col % st.per_row);
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(kThreads) void commit_kernel(View v, Strides st, co
             const int to = taken + static_cast<int>(__popcll(lives & below));
             int4 m{-1, 0, -1, 0};
             if (live && node != to) {
-                const int from_row = row_of(v, b, node), to_row = row_of(v, b, to);
+                const int from_row = row_behind(ctx, node), to_row = row_behind(ctx, to);
                 m.x = page_of(v, b, from_row);
                 m.y = from_row & (v.c.page_size - 1);
                 m.z = page_of(v, b, to_row);

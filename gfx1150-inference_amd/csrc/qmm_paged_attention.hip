@@ -46,7 +46,7 @@ __device__ __forceinline__ Span span_of(const View& v, const AttnArgs& a, int se
     s.seq = seq;
     s.first = max(v.c.cu[seq], 0);
     s.n = max(min(max(v.c.cu[seq + 1], 0), a.in.tokens) - s.first, 0);
-    s.ctx = min(max(v.c.ctx[seq], 0), 1 << 30);
+    s.ctx = cached_rows(v, seq);
     s.total = static_cast<int>(min(static_cast<int64_t>(s.ctx) + s.n, static_cast<int64_t>(v.c.table_width) << v.page_shift));
     return s;
 }
