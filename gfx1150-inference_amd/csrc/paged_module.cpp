@@ -11,6 +11,7 @@
 #include <optional>
 #include <sstream>
 #include <string>
+#include <vector>
 
 #include "qmm.h"
 
@@ -124,11 +125,13 @@ void* stream_of(c10::Device device) {
     return c10::hip::getCurrentHIPStream(device.index()).stream();
 }
 
+// A new int32 tensor.
 Tensor ints(at::IntArrayRef sizes, c10::Device device) { return at::empty(sizes, at::TensorOptions().dtype(at::kInt).device(device)); }
 
 OptTensor append(const Tensor& k, const Tensor& v, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& cu,
                  const Tensor& ctx, const OptTensor& q, OptTensor q_out, const OptTensor& positions, double freq_base,
-                 std::optional<int64_t> rotary_dim, bool neox, double k_scale, double v_scale) {
+                 std::optional<int64_t> rotary_dim, bool neox, double k_scale, double v_scale, const OptTensor& q_norm, const OptTensor& k_norm,
+                 double norm_eps, const std::optional<std::vector<int64_t>>& axes) {
     require(k.is_cuda(), "k must be on a GPU");
     const qmm_paged_kv kv = cache_of(k_cache, v_cache, table, &cu, ctx, k_scale, v_scale, false);
     const auto dtype = k.scalar_type();
@@ -144,7 +147,11 @@ OptTensor append(const Tensor& k, const Tensor& v, const Tensor& k_cache, const 
     in.k_head = k.stride(1);
     in.v_token = v.stride(0);
     in.v_head = v.stride(1);
-    if (positions) {
+    if (axes) {
+        require(positions.has_value(), "axes need positions");
+        check_ints(*positions, "positions", {-1, tokens}, k_cache.device());
+        in.positions = static_cast<const int32_t*>(positions->data_ptr());
+    } else if (positions) {
         check_ints(*positions, "positions", {tokens}, k_cache.device());
         in.positions = static_cast<const int32_t*>(positions->data_ptr());
     }
@@ -167,15 +174,42 @@ OptTensor append(const Tensor& k, const Tensor& v, const Tensor& k_cache, const 
     in.rotary_dim = int_of(rotary_dim.value_or(kv.head_dim), "rotary_dim");
     in.neox = neox ? 1 : 0;
     in.freq_base = static_cast<float>(freq_base);
-    check(qmm_paged_append(&kv, &in, stream_of(k_cache.device())));
+    if (!q_norm && !k_norm && !axes) {
+        check(qmm_paged_append(&kv, &in, stream_of(k_cache.device())));
+        return q_out;
+    }
+    qmm_paged_norm norm{};
+    norm.weight_dtype = in.dtype;
+    norm.eps = static_cast<float>(norm_eps);
+    require(!q_norm || q, "q_norm needs q");
+    for (const OptTensor* w : {&q_norm, &k_norm}) {
+        if (!*w) continue;
+        const Tensor& t = **w;
+        require(t.dim() == 1 && t.size(0) == kv.head_dim && (t.size(0) == 1 || t.stride(0) == 1) && t.device() == k_cache.device(),
+                "q_norm and k_norm must be contiguous [head_dim] tensors on the cache's device");
+        norm.weight_dtype = code_of(t.scalar_type());
+    }
+    require(!q_norm || !k_norm || q_norm->scalar_type() == k_norm->scalar_type(), "q_norm and k_norm must be of one type");
+    if (q_norm) norm.q_weight = q_norm->data_ptr();
+    if (k_norm) norm.k_weight = k_norm->data_ptr();
+    uint8_t axis[128];
+    if (axes) {
+        require(in.rotary_dim >= 0 && in.rotary_dim <= 256 && static_cast<int64_t>(axes->size()) == in.rotary_dim / 2, "axes must hold one axis for each rotated pair");
+        for (size_t i = 0; i < axes->size(); ++i) {
+            require((*axes)[i] >= 0 && (*axes)[i] < positions->size(0) && (*axes)[i] < 256, "axes must be rows of positions");
+            axis[i] = static_cast<uint8_t>((*axes)[i]);
+        }
+        norm.axes = axis;
+        norm.axis_stride = positions->stride(0);
+        norm.num_axes = static_cast<int32_t>(std::min<int64_t>(positions->size(0), 256));
+    }
+    check(qmm_paged_append_normed(&kv, &in, &norm, stream_of(k_cache.device())));
     return q_out;
 }
 
-Tensor tree_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& cu, const Tensor& ctx,
-                      const OptTensor& mask, std::optional<int64_t> max_new, std::optional<double> scale, double k_scale, double v_scale,
-                      OptTensor out) {
-    require(q.is_cuda(), "q must be on a GPU");
-    const qmm_paged_kv kv = cache_of(k_cache, v_cache, table, &cu, ctx, k_scale, v_scale, false);
+// The queries of checked arguments; `out` becomes a new tensor where there is none.
+qmm_paged_query query_of(const Tensor& q, const Tensor& k_cache, const OptTensor& mask, std::optional<int64_t> max_new, std::optional<double> scale,
+                         OptTensor& out) {
     const auto dtype = q.scalar_type();
     require(dtype == at::kHalf || dtype == at::kBFloat16, "q must be float16 or bfloat16");
     check_rows(q, "q", -1, -1, k_cache, dtype);
@@ -202,12 +236,107 @@ Tensor tree_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_ca
     in.dtype = code_of(dtype);
     in.scale = static_cast<float>(scale.value_or(0.0));  // 0: the default
     require(!scale || in.scale != 0.0f, "scale must not be 0 in 32 bits");
+    return in;
+}
+
+// Device memory for a call: the allocator's, safe to capture.
+struct Space {
+    Tensor t;
+    size_t bytes;
+    Space(size_t need, c10::Device device) : bytes(need) {
+        if (need) t = at::empty({static_cast<int64_t>(need)}, at::TensorOptions().dtype(at::kByte).device(device));
+    }
+    void* data() const { return bytes ? t.data_ptr() : nullptr; }
+};
+
+Tensor tree_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& cu, const Tensor& ctx,
+                      const OptTensor& mask, std::optional<int64_t> max_new, std::optional<double> scale, double k_scale, double v_scale,
+                      OptTensor out) {
+    require(q.is_cuda(), "q must be on a GPU");
+    const qmm_paged_kv kv = cache_of(k_cache, v_cache, table, &cu, ctx, k_scale, v_scale, false);
+    const qmm_paged_query in = query_of(q, k_cache, mask, max_new, scale, out);
     void* stream = stream_of(k_cache.device());
-    const size_t need = qmm_paged_attention_workspace(&kv, &in);
-    Tensor space;  // the allocator's: safe to capture
-    if (need) space = at::empty({static_cast<int64_t>(need)}, at::TensorOptions().dtype(at::kByte).device(q.device()));
-    check(qmm_paged_tree_attention(&kv, &in, need ? space.data_ptr() : nullptr, need, stream));
+    const Space space(qmm_paged_attention_workspace(&kv, &in), q.device());
+    check(qmm_paged_tree_attention(&kv, &in, space.data(), space.bytes, stream));
     return *out;
+}
+
+Tensor shared_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& cu, const Tensor& ctx,
+                        const Tensor& groups, const Tensor& shared, const OptTensor& mask, std::optional<int64_t> max_new,
+                        std::optional<double> scale, double k_scale, double v_scale, OptTensor out) {
+    require(q.is_cuda(), "q must be on a GPU");
+    const qmm_paged_kv kv = cache_of(k_cache, v_cache, table, &cu, ctx, k_scale, v_scale, false);
+    const qmm_paged_query in = query_of(q, k_cache, mask, max_new, scale, out);
+    check_ints(shared, "shared", {-1}, k_cache.device());
+    check_ints(groups, "groups", {shared.size(0) + 1}, k_cache.device());
+    const qmm_paged_groups g{static_cast<const int32_t*>(groups.data_ptr()), static_cast<const int32_t*>(shared.data_ptr()),
+                             int_of(shared.size(0), "the count of groups")};
+    void* stream = stream_of(k_cache.device());
+    const Space space(qmm_paged_shared_workspace(&kv, &in, &g), q.device());
+    check(qmm_paged_shared_attention(&kv, &in, &g, space.data(), space.bytes, stream));
+    return *out;
+}
+
+// Sums of weights: float32, the rows contiguous.
+void check_sums(const Tensor& t, const char* name, std::initializer_list<int64_t> sizes, c10::Device device) {
+    bool fits = t.scalar_type() == at::kFloat && t.device() == device && t.dim() == static_cast<int64_t>(sizes.size()) &&
+                (t.numel() == 0 || t.size(-1) <= 1 || t.stride(-1) == 1);
+    int64_t d = 0;
+    for (int64_t want : sizes) {
+        fits = fits && (want < 0 || t.size(d) == want);
+        ++d;
+    }
+    if (!fits) throw py::value_error(std::string(name) + " must be a float32 tensor of " + std::to_string(sizes.size()) + " dimensions that fits the call, on the cache's device, its rows contiguous");
+}
+
+std::tuple<Tensor, Tensor> weighted_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& cu,
+                                              const Tensor& ctx, const Tensor& weights, OptTensor weights_out, const OptTensor& mask,
+                                              std::optional<int64_t> max_new, std::optional<double> scale, double k_scale, double v_scale,
+                                              OptTensor out) {
+    require(q.is_cuda(), "q must be on a GPU");
+    const qmm_paged_kv kv = cache_of(k_cache, v_cache, table, &cu, ctx, k_scale, v_scale, false);
+    const qmm_paged_query in = query_of(q, k_cache, mask, max_new, scale, out);
+    if (!weights_out) weights_out = weights;
+    check_sums(weights, "weights", {kv.batch, kv.kv_heads, -1}, k_cache.device());
+    check_sums(*weights_out, "weights_out", {kv.batch, kv.kv_heads, weights.size(2)}, k_cache.device());
+    qmm_paged_weights w{static_cast<const float*>(weights.data_ptr()), static_cast<float*>(weights_out->data_ptr()), weights.stride(0),
+                        weights.stride(1), weights_out->stride(0), weights_out->stride(1), int_of(weights.size(2), "the count of rows")};
+    void* stream = stream_of(k_cache.device());
+    const Space space(qmm_paged_weighted_workspace(&kv, &in, &w), q.device());
+    check(qmm_paged_weighted_attention(&kv, &in, &w, space.data(), space.bytes, stream));
+    return {*out, *weights_out};
+}
+
+std::tuple<Tensor, Tensor, Tensor> evict(const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& ctx,
+                                         const Tensor& weights, const Tensor& fresh, int64_t keep, int64_t recent, int64_t sinks) {
+    require(k_cache.is_cuda(), "k_cache must be on a GPU");
+    const qmm_paged_kv kv = cache_of(k_cache, v_cache, table, nullptr, ctx, 1.0, 1.0, true);
+    const c10::Device device = k_cache.device();
+    check_sums(weights, "weights", {kv.num_layers, kv.batch, kv.kv_heads, -1}, device);
+    check_ints(fresh, "fresh", {kv.batch, -1}, device);
+    Tensor new_table = ints(table.sizes(), device), lens = ints(ctx.sizes(), device), kept = at::empty(weights.sizes(), weights.options());
+    qmm_paged_evict_args e{};
+    e.weights = static_cast<const float*>(weights.data_ptr());
+    e.weights_out = static_cast<float*>(kept.data_ptr());
+    e.fresh = static_cast<const int32_t*>(fresh.data_ptr());
+    e.table_out = static_cast<int32_t*>(new_table.data_ptr());
+    e.lens_out = static_cast<int32_t*>(lens.data_ptr());
+    e.w_layer = weights.stride(0);
+    e.w_batch = weights.stride(1);
+    e.w_head = weights.stride(2);
+    e.wo_layer = kept.stride(0);
+    e.wo_batch = kept.stride(1);
+    e.wo_head = kept.stride(2);
+    e.fresh_stride = fresh.stride(0);
+    e.rows = int_of(weights.size(3), "the count of rows");
+    e.fresh_width = int_of(fresh.size(1), "fresh's width");
+    e.keep = int_of(keep, "keep");
+    e.recent = int_of(recent, "recent");
+    e.sinks = int_of(sinks, "sinks");
+    void* stream = stream_of(device);
+    const Space space(qmm_paged_evict_workspace(&kv, &e), device);
+    check(qmm_paged_evict(&kv, &e, space.data(), space.bytes, stream));
+    return {new_table, lens, kept};
 }
 
 Tensor commit_path(const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& cu, const Tensor& ctx, const Tensor& path) {
@@ -264,6 +393,9 @@ PYBIND11_MODULE(paged_module, m) {
     m.doc() = "Paged key/value cache and beam search on torch tensors (see paged.py and beam.py)";
     m.def("append", &append);
     m.def("tree_attention", &tree_attention);
+    m.def("shared_attention", &shared_attention);
+    m.def("weighted_attention", &weighted_attention);
+    m.def("evict", &evict);
     m.def("commit_path", &commit_path);
     m.def("beam_select", &beam_select);
     m.def("beam_reorder", &beam_reorder);

@@ -76,6 +76,27 @@ __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d
     return static_cast<uint32_t>(w);
 }
 
+// Rows are copied in units of U bytes, the largest that every address is a multiple of.
+template <int B>
+struct Unit;
+template <>
+struct Unit<16> {
+    using type = u32x4;
+};
+template <>
+struct Unit<4> {
+    using type = uint32_t;
+};
+template <>
+struct Unit<1> {
+    using type = uint8_t;
+};
+
+struct Strides {  // in units
+    int64_t k_layer, k_page, k_head, k_slot, v_layer, v_page, v_head, v_slot;
+    int per_row;
+};
+
 // ---- host side -------------------------------------------------------------------------------
 
 inline int elem_bytes(int dtype) { return dtype == QMM_DTYPE_E4M3 ? 1 : dtype == QMM_DTYPE_F32 ? 4 : 2; }
@@ -89,6 +110,18 @@ inline int launched(hipError_t e, const char* what) {
 
 // Checks a cache description; fills `out`.  need_cu: the call reads cu.
 int check_view(const qmm_paged_kv* kv, bool need_cu, View* out);
+
+// The largest unit of 16, 4 and 1 bytes that divides every address of the cache's rows; strides in it.
+inline int copy_unit(const qmm_paged_kv& c, Strides* st) {
+    const int64_t eb = elem_bytes(c.dtype);
+    const int64_t s[8] = {c.k_layer, c.k_page, c.k_head, c.k_slot, c.v_layer, c.v_page, c.v_head, c.v_slot};
+    uint64_t all = reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v) | static_cast<uint64_t>(c.head_dim * eb);
+    for (int64_t x : s) all |= static_cast<uint64_t>(x * eb);
+    const int unit = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
+    *st = {s[0] * eb / unit, s[1] * eb / unit, s[2] * eb / unit, s[3] * eb / unit, s[4] * eb / unit, s[5] * eb / unit,
+           s[6] * eb / unit, s[7] * eb / unit, static_cast<int>(c.head_dim * eb / unit)};
+    return unit;
+}
 
 // Runs the body of a C entry point: no exception leaves it.
 template <class Body>

@@ -247,28 +247,87 @@ __global__ __launch_bounds__(kThreads) void append_scalar_kernel(View v, AppendA
     }
 }
 
+// ---- append with norms and axes ------------------------------------------------------------------
+// y = x rsqrt(mean(x^2) + eps) w for each query and key head, then the rotation, pair i by the position on its axis.
+// Squares, their sum and the products are fp32, and the result is rounded once.
+struct NormArgs {
+    const void *qw, *kw;
+    int64_t axis_stride;
+    int w_f32;
+    float eps;
+    uint8_t axis[kMaxPairs];
+};
+
+template <class T>
+__device__ __forceinline__ float norm_weight(const NormArgs& n, const void* w, int d) {
+    return n.w_f32 ? static_cast<const float*>(w)[d] : to_float(static_cast<const T*>(w)[d]);
+}
+
+// Every alignment, rotation and head size: one wave per head of a token, its dimensions through LDS for the partner of
+// each rotated one.  Block (x, y): token, four heads (queries, keys, then values).
+template <class T, bool kFp8>
+__global__ __launch_bounds__(kThreads) void append_normed_scalar_kernel(View v, AppendArgs a, NormArgs nm, RopeTurns fr) {
+    __shared__ float2 cs[kMaxPairs];
+    __shared__ float row[4][2 * kMaxPairs];
+    const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int D = v.c.head_dim, heads = a.in.q ? a.in.heads : 0, kvh = v.c.kv_heads, half = a.in.rotary_dim / 2;
+    const int seq = sequence_of(v, t, lane);
+    if (seq >= v.c.batch || t < v.c.cu[seq]) return;
+    const int r = row_behind(cached_rows(v, seq), t - max(v.c.cu[seq], 0));
+    const int page = page_of(v, seq, r), slot = r & (v.c.page_size - 1);
+    if (tid < half) cs[tid] = cos_sin(fr.turn[tid], a.in.positions ? a.in.positions[nm.axis[tid] * nm.axis_stride + t] : r);
+    const int64_t tt = t;
+    const int head = blockIdx.y * 4 + w;
+    const bool is_q = head < heads, is_k = !is_q && head < heads + kvh, is_v = !is_q && !is_k && head < heads + 2 * kvh;
+    const int h = is_q ? head : is_k ? head - heads : head - heads - kvh;
+    const T* src = is_q   ? static_cast<const T*>(a.in.q) + tt * a.in.q_token + h * a.in.q_head
+                   : is_k ? static_cast<const T*>(a.in.k) + tt * a.in.k_token + h * a.in.k_head
+                          : static_cast<const T*>(a.in.v) + tt * a.in.v_token + h * a.in.v_head;
+    const void* weight = is_q ? nm.qw : is_k ? nm.kw : nullptr;
+    float x[4], squares = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int d = lane + 64 * i;
+        x[i] = d < D && (is_q || is_k || is_v) ? to_float(src[d]) : 0.0f;
+        squares += x[i] * x[i];
+    }
+    for (int o = 32; o > 0; o >>= 1) squares += __shfl_xor(squares, o, 64);
+    const float f = weight ? 1.0f / sqrtf(squares / static_cast<float>(D) + nm.eps) : 1.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int d = lane + 64 * i;
+        if (d < D) row[w][d] = weight ? x[i] * f * norm_weight<T>(nm, weight, d) : x[i];
+    }
+    __syncthreads();
+    if (!(is_q || is_k || is_v) || (!is_q && page < 0)) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int d = lane + 64 * i;
+        if (d >= D) break;
+        float y = row[w][d];
+        if (!is_v && d < 2 * half) {
+            const int pair = a.in.neox ? (d < half ? d : d - half) : d >> 1;
+            const bool first = a.in.neox ? d < half : !(d & 1);
+            const int other = a.in.neox ? (first ? d + half : d - half) : d ^ 1;
+            const float2 c = cs[pair];
+            y = first ? y * c.x - row[w][other] * c.y : row[w][other] * c.y + y * c.x;
+        }
+        if (is_q) {
+            static_cast<T*>(a.in.q_out)[tt * a.in.qo_token + h * a.in.qo_head + d] = static_cast<T>(y);
+        } else {
+            const int64_t at = is_k ? page * v.c.k_page + slot * v.c.k_slot + h * v.c.k_head + d : page * v.c.v_page + slot * v.c.v_slot + h * v.c.v_head + d;
+            void* base = is_k ? v.c.k : v.c.v;
+            if constexpr (kFp8) {
+                const float z = is_k ? (a.k_exact ? y * a.k_mul : y / a.k_div) : (a.v_exact ? y * a.v_mul : y / a.v_div);
+                static_cast<uint8_t*>(base)[at] = static_cast<uint8_t>(pack_e4m3(clamp_e4m3(z), 0.0f, 0.0f, 0.0f));
+            } else {
+                static_cast<T*>(base)[at] = static_cast<T>(y);
+            }
+        }
+    }
+}
+
 // ---- moving rows ---------------------------------------------------------------------------------
-// Rows are copied in units of U bytes, the largest that every address is a multiple of.
-template <int B>
-struct Unit;
-template <>
-struct Unit<16> {
-    using type = u32x4;
-};
-template <>
-struct Unit<4> {
-    using type = uint32_t;
-};
-template <>
-struct Unit<1> {
-    using type = uint8_t;
-};
-
-struct Strides {  // in units
-    int64_t k_layer, k_page, k_head, k_slot, v_layer, v_page, v_head, v_slot;
-    int per_row;
-};
-
 // Commit of a path: block (x, b) takes 256 of the (layer, K or V, head, piece) columns of sequence b; a
 // thread moves its column of every step, eight loads in flight.  The j-th node that is taken, path's j-th entry or a
 // later one, is at least j where the path ascends, and its row becomes row j: in that order no step reads what an earlier
@@ -400,18 +459,6 @@ bool power_of_two(float x) {
     return std::isfinite(x) && x > 0.0f && std::frexp(x, &e) == 0.5f && std::isfinite(1.0f / x) && 1.0f / x >= 0x1p-126f;
 }
 
-// The largest unit of 16, 4 and 1 bytes that divides every address of the cache's rows; strides in it.
-int copy_unit(const qmm_paged_kv& c, Strides* st) {
-    const int64_t eb = elem_bytes(c.dtype);
-    const int64_t s[8] = {c.k_layer, c.k_page, c.k_head, c.k_slot, c.v_layer, c.v_page, c.v_head, c.v_slot};
-    uint64_t all = reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v) | static_cast<uint64_t>(c.head_dim * eb);
-    for (int64_t x : s) all |= static_cast<uint64_t>(x * eb);
-    const int unit = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
-    *st = {s[0] * eb / unit, s[1] * eb / unit, s[2] * eb / unit, s[3] * eb / unit, s[4] * eb / unit, s[5] * eb / unit,
-           s[6] * eb / unit, s[7] * eb / unit, static_cast<int>(c.head_dim * eb / unit)};
-    return unit;
-}
-
 // Turns per position of each pair, 2^64 a turn.  A program's layers share one base, so a thread's last table is kept.
 const RopeTurns& rope_turns(float base, int rotary_dim) {
     thread_local RopeTurns turns{};
@@ -460,7 +507,8 @@ int check_view(const qmm_paged_kv* kv, bool need_cu, View* out) {
 
 namespace {
 
-int append(const qmm_paged_kv* kv, const qmm_paged_new* in, hipStream_t stream) {
+// norm: NULL, or what qmm_paged_append_normed adds.
+int append(const qmm_paged_kv* kv, const qmm_paged_new* in, const qmm_paged_norm* norm, hipStream_t stream) {
     View v;
     int rc = check_view(kv, true, &v);
     if (rc != QMM_OK) return rc;
@@ -473,6 +521,28 @@ int append(const qmm_paged_kv* kv, const qmm_paged_new* in, hipStream_t stream) 
     if (in->tokens < 0 || in->heads < 0) return bad("tokens and heads must be non-negative.");
     if (rot < 0 || rot % 2 != 0 || rot > D) return bad("rotary_dim must be even, between 0 and head_dim.");
     if (rot > 0 && !(in->freq_base > 0.0f && std::isfinite(in->freq_base))) return bad("freq_base must be positive and finite.");
+    NormArgs nm{};
+    if (norm) {
+        const bool weighs = norm->q_weight || norm->k_weight;
+        if (weighs && norm->weight_dtype != in->dtype && norm->weight_dtype != QMM_DTYPE_F32) return bad("the norms' weights must be F32 or of the new tokens' dtype.");
+        const uintptr_t align = norm->weight_dtype == QMM_DTYPE_F32 ? 4 : 2;
+        if ((reinterpret_cast<uintptr_t>(norm->q_weight) | reinterpret_cast<uintptr_t>(norm->k_weight)) % align != 0)
+            return bad("the norms' weights must be aligned to their elements.");
+        if (weighs && !(norm->eps >= 0.0f && std::isfinite(norm->eps))) return bad("eps must be finite and not negative.");
+        if (norm->axes) {
+            if (norm->num_axes < 1 || norm->num_axes > 256) return bad("num_axes must be between 1 and 256.");
+            if (!in->positions) return bad("axes need positions.");
+            for (int i = 0; i < rot / 2; ++i) {
+                if (norm->axes[i] >= norm->num_axes) return bad("axes must be below num_axes.");
+                nm.axis[i] = norm->axes[i];
+            }
+            nm.axis_stride = norm->axis_stride;
+        }
+        nm.qw = norm->q_weight;
+        nm.kw = norm->k_weight;
+        nm.w_f32 = norm->weight_dtype == QMM_DTYPE_F32;
+        nm.eps = norm->eps;
+    }
     if (in->tokens == 0 || v.c.batch == 0) return QMM_OK;
     if (!in->k || !in->v) return bad("k and v of the new tokens must be non-null.");
     if (in->q && (!in->q_out || in->heads == 0)) return bad("q needs q_out and a positive count of heads.");
@@ -509,6 +579,13 @@ int append(const qmm_paged_kv* kv, const qmm_paged_new* in, hipStream_t stream) 
     if (grid.y > 65535) return bad("too many heads.");
     static const RopeTurns none{};
     const RopeTurns& fr = rot > 0 ? rope_turns(in->freq_base, rot) : none;
+    if (norm && (norm->axes || norm->q_weight || norm->k_weight)) {
+        const dim3 by_head(static_cast<unsigned>(in->tokens), static_cast<unsigned>((heads + 2 * v.c.kv_heads + 3) / 4));
+        auto scalar = [&](auto kern) { hipLaunchKernelGGL(kern, by_head, dim3(kThreads), 0, stream, v, a, nm, fr); };
+        if (in->dtype == QMM_DTYPE_F16) fp8 ? scalar(append_normed_scalar_kernel<_Float16, true>) : scalar(append_normed_scalar_kernel<_Float16, false>);
+        else fp8 ? scalar(append_normed_scalar_kernel<__bf16, true>) : scalar(append_normed_scalar_kernel<__bf16, false>);
+        return launched(hipGetLastError(), "paged append kernel launch");
+    }
     auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, stream, v, a, fr); };
     auto pick = [&](auto tc, auto f8) {
         using T = decltype(tc);
@@ -567,7 +644,13 @@ int reorder(const qmm_paged_kv* kv, const int32_t* parents, const int32_t* fresh
 extern "C" {
 
 int qmm_paged_append(const qmm_paged_kv* kv, const qmm_paged_new* in, void* stream) {
-    return qmm::paged::entry([&] { return qmm::paged::append(kv, in, static_cast<hipStream_t>(stream)); });
+    return qmm::paged::entry([&] { return qmm::paged::append(kv, in, nullptr, static_cast<hipStream_t>(stream)); });
+}
+
+int qmm_paged_append_normed(const qmm_paged_kv* kv, const qmm_paged_new* in, const qmm_paged_norm* norm, void* stream) {
+    return qmm::paged::entry([&] {
+        return norm ? qmm::paged::append(kv, in, norm, static_cast<hipStream_t>(stream)) : qmm::paged::bad("norm must be non-null.");
+    });
 }
 
 int qmm_paged_commit_path(const qmm_paged_kv* kv, const int32_t* path, int64_t path_stride, int path_len, int32_t* lens, void* stream) {

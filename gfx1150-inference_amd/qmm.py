@@ -123,6 +123,34 @@ class PagedQuery(ctypes.Structure):
                 ("mask_words", _i), ("scale", ctypes.c_float)]
 
 
+class PagedNorm(ctypes.Structure):
+    """Mirror of qmm_paged_norm (include/qmm.h)."""
+
+    _fields_ = [("q_weight", _vp), ("k_weight", _vp), ("axes", _vp), ("axis_stride", _i64), ("weight_dtype", _i), ("num_axes", _i),
+                ("eps", ctypes.c_float)]
+
+
+class PagedGroups(ctypes.Structure):
+    """Mirror of qmm_paged_groups (include/qmm.h)."""
+
+    _fields_ = [("first", _vp), ("shared", _vp), ("count", _i)]
+
+
+class PagedWeights(ctypes.Structure):
+    """Mirror of qmm_paged_weights (include/qmm.h)."""
+
+    _fields_ = [("old_sums", _vp), ("new_sums", _vp), ("old_batch", _i64), ("old_head", _i64), ("new_batch", _i64), ("new_head", _i64),
+                ("rows", _i)]
+
+
+class PagedEvict(ctypes.Structure):
+    """Mirror of qmm_paged_evict_args (include/qmm.h)."""
+
+    _fields_ = [("weights", _vp), ("weights_out", _vp), ("fresh", _vp), ("table_out", _vp), ("lens_out", _vp),
+                ("w_layer", _i64), ("w_batch", _i64), ("w_head", _i64), ("wo_layer", _i64), ("wo_batch", _i64), ("wo_head", _i64),
+                ("fresh_stride", _i64), ("rows", _i), ("fresh_width", _i), ("keep", _i), ("recent", _i), ("sinks", _i)]
+
+
 _SIGNATURES = {
     "qmm_last_error": (ctypes.c_char_p, []),
     "qmm_version": (_i, []),
@@ -153,6 +181,13 @@ _SIGNATURES = {
     "qmm_paged_append": (_i, [_vp, _vp, _vp]),
     "qmm_paged_attention_workspace": (ctypes.c_size_t, [_vp, _vp]),
     "qmm_paged_tree_attention": (_i, [_vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "qmm_paged_append_normed": (_i, [_vp, _vp, _vp, _vp]),
+    "qmm_paged_shared_workspace": (ctypes.c_size_t, [_vp, _vp, _vp]),
+    "qmm_paged_shared_attention": (_i, [_vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "qmm_paged_weighted_workspace": (ctypes.c_size_t, [_vp, _vp, _vp]),
+    "qmm_paged_weighted_attention": (_i, [_vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "qmm_paged_evict_workspace": (ctypes.c_size_t, [_vp, _vp]),
+    "qmm_paged_evict": (_i, [_vp, _vp, _vp, ctypes.c_size_t, _vp]),
     "qmm_paged_commit_path": (_i, [_vp, _vp, _i64, _i, _vp, _vp]),
     "qmm_beam_select_workspace": (ctypes.c_size_t, [_i, _i, _i, _i]),
     "qmm_beam_select": (_i, [_vp, _i, _i64, _i64, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),

@@ -359,7 +359,7 @@ typedef struct qmm_paged_kv {
     void* k;
     void* v;
     const int32_t* table; /* [batch][table_width], rows table_stride apart */
-    const int32_t* cu;    /* [batch + 1]; not read by qmm_beam_reorder */
+    const int32_t* cu;    /* [batch + 1]; not read by qmm_beam_reorder and qmm_paged_evict */
     const int32_t* ctx;   /* [batch] */
     int64_t table_stride;
     int64_t k_layer, k_page, k_head, k_slot; /* strides in elements */
@@ -392,6 +392,21 @@ typedef struct qmm_paged_new {
  * tokens of one call must not share a cache row. */
 int qmm_paged_append(const qmm_paged_kv* kv, const qmm_paged_new* in, void* stream);
 
+/* What qmm_paged_append_normed does besides: every query and key head x becomes
+ * x * rsqrt(mean(x^2) + eps) * weight ahead of its rotation (fp32, not rounded in between), and pair i
+ * of the rotated dimensions turns by the position on axis axes[i]. */
+typedef struct qmm_paged_norm {
+    const void* q_weight; /* [head_dim] of the new tokens' dtype or F32; NULL: queries are not normed */
+    const void* k_weight; /* alike, for the keys */
+    const uint8_t* axes;  /* host memory, rotary_dim / 2 axes below num_axes; NULL: one axis for all */
+    int64_t axis_stride;  /* positions of axis a begin at in->positions + a * axis_stride */
+    int32_t weight_dtype, num_axes;
+    float eps;
+} qmm_paged_norm;
+
+/* qmm_paged_append with norms and axes; `axes` needs positions.  axes is read before the call returns. */
+int qmm_paged_append_normed(const qmm_paged_kv* kv, const qmm_paged_new* in, const qmm_paged_norm* norm, void* stream);
+
 /* Queries q [tokens][heads][head_dim] of the new tokens, out alike (16-bit float, the cache's type
  * unless that is E4M3).  New token i of a sequence sees its ctx cached rows and, of the sequence's
  * new rows j, those whose bit j % 32 of mask[token][j / 32] is set (words past mask_words: not
@@ -414,6 +429,55 @@ typedef struct qmm_paged_query {
 size_t qmm_paged_attention_workspace(const qmm_paged_kv* kv, const qmm_paged_query* in);
 int qmm_paged_tree_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, void* workspace, size_t workspace_bytes,
                              void* stream);
+
+/* Groups of consecutive sequences that begin with the same rows: group g is the sequences first[g] ..
+ * first[g + 1] - 1 (first does not descend; sequences outside every group share nothing), whose tables begin with the
+ * same pages for at least shared[g] rows that each of them has in its cache.  Device memory. */
+typedef struct qmm_paged_groups {
+    const int32_t* first;  /* [count + 1] */
+    const int32_t* shared; /* [count] */
+    int32_t count;
+} qmm_paged_groups;
+
+/* qmm_paged_tree_attention, the rows that a group shares being read once for the group.  A shared row is read through the
+ * table of any of the group's sequences. */
+size_t qmm_paged_shared_workspace(const qmm_paged_kv* kv, const qmm_paged_query* in, const qmm_paged_groups* groups);
+int qmm_paged_shared_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, const qmm_paged_groups* groups, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/* Sums of softmax weights, fp32 [batch][kv_heads][rows] (strides in elements, rows contiguous): new_sums[b][g][j] = what row j
+ * of sequence b gets from kv head g's query heads and the call's new tokens, on top of old_sums[b][g][j] where j < ctx[b].  A
+ * new row's sum starts at 0.  Entries behind a sequence's last new row are left as they are, and rows that `rows`
+ * has no place for are not summed.  new_sums may be old_sums (the same strides), and must not overlap it otherwise. */
+typedef struct qmm_paged_weights {
+    const float* old_sums;
+    float* new_sums;
+    int64_t old_batch, old_head, new_batch, new_head;
+    int32_t rows;
+} qmm_paged_weights;
+
+/* qmm_paged_tree_attention, and the weights' sums. */
+size_t qmm_paged_weighted_workspace(const qmm_paged_kv* kv, const qmm_paged_query* in, const qmm_paged_weights* weights);
+int qmm_paged_weighted_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, const qmm_paged_weights* weights, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
+/* Which rows of a sequence stay: of each layer and kv head the first `sinks`, the last `recent` and, of the others, those
+ * of the largest weights [num_layers][batch][kv_heads][rows] (fp32; equal ones go to the lower row; NaN, and a row that
+ * `rows` has no place for, count as -inf), `keep` rows in all.  A sequence of at most `keep` rows (that its table has
+ * places for) stays as it is.  Of the others the kept rows are copied in their order to rows 0 .. keep - 1 of the pages
+ * fresh[b][0 .. fresh_width - 1], which no sequence of the table uses. */
+typedef struct qmm_paged_evict_args {
+    const float* weights;
+    float* weights_out;   /* alike, not overlapping: the kept rows' weights, 0 behind them */
+    const int32_t* fresh; /* [batch][fresh_width], rows fresh_stride apart */
+    int32_t* table_out;   /* [batch][table_width], contiguous: fresh pages and -1 behind them, or the table's row */
+    int32_t* lens_out;    /* [batch]: the new lengths */
+    int64_t w_layer, w_batch, w_head, wo_layer, wo_batch, wo_head, fresh_stride;
+    int32_t rows, fresh_width, keep, recent, sinks;
+} qmm_paged_evict_args;
+
+size_t qmm_paged_evict_workspace(const qmm_paged_kv* kv, const qmm_paged_evict_args* args);
+int qmm_paged_evict(const qmm_paged_kv* kv, const qmm_paged_evict_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /* After a drafted tree was verified: in every layer, row ctx[b] + node of sequence b becomes its row
  * ctx[b] + j for the j-th node of path ([batch][path_len], rows path_stride apart; entries outside the
