@@ -263,6 +263,147 @@ __device__ __forceinline__ float norm_weight(const NormArgs& n, const void* w, i
     return n.w_f32 ? static_cast<const float*>(w)[d] : to_float(static_cast<const T*>(w)[d]);
 }
 
+// The sum over 2^shift neighbouring lanes (shift 2 to 5), in all of them.
+__device__ __forceinline__ float group_sum(float x, int shift) {
+    auto step = [&](auto ctrl) { x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xF, 0xF, false)); };
+    step(std::integral_constant<int, 0xB1>{});   // lane ^ 1
+    step(std::integral_constant<int, 0x4E>{});   // lane ^ 2
+    if (shift > 2) step(std::integral_constant<int, 0x141>{});  // the mirrored lane of 8
+    if (shift > 3) step(std::integral_constant<int, 0x140>{});  // .. and of 16
+    if (shift > 4) x += __shfl_xor(x, 16, 64);
+    return x;
+}
+
+// As append_kernel, with 2^lane_shift lanes for each query and key head, of which the first units_rot hold a unit: the squares' sum
+// is one over neighbouring lanes.  What turns and weighs a lane's dimensions waits in LDS, the same for every head.
+template <class T, bool kFp8, bool kNeox>
+__global__ __launch_bounds__(kThreads) void append_normed_kernel(View v, AppendArgs a, NormArgs nm, RopeTurns fr, int lane_shift) {
+    __shared__ float2 cs[kMaxPairs];
+    __shared__ __align__(16) float weights[2][2 * kMaxPairs];
+    const int t = blockIdx.x, tid = threadIdx.x, D = v.c.head_dim;
+    const int heads = a.in.q ? a.in.heads : 0, kvh = v.c.kv_heads, half = a.in.rotary_dim / 2;
+    const int rot_total = (heads + kvh) << lane_shift;
+    int u = blockIdx.y * a.per_block + tid;
+    const int u_end = min(a.units, static_cast<int>(blockIdx.y + 1) * a.per_block);
+
+    struct Unit {
+        int kind, head, d0;  // kind 0 query, 1 key, 2 value
+        bool paired, live;   // d0 + half goes with it; the lane holds a unit
+    };
+    auto decode = [&](int i) {
+        Unit n;
+        if (i < rot_total) {
+            const int c = i & ((1 << lane_shift) - 1);
+            n.head = i >> lane_shift;
+            n.live = c < a.units_rot;
+            n.kind = n.head < heads ? 0 : 1;
+            if (n.kind) n.head -= heads;
+            n.paired = kNeox && 8 * c < half;
+            n.d0 = kNeox && !n.paired ? 8 * c + half : 8 * c;
+        } else {
+            const int j = i - rot_total;
+            n.kind = 2;
+            n.head = j / a.units_v;
+            n.d0 = 8 * (j % a.units_v);
+            n.paired = false;
+            n.live = true;
+        }
+        return n;
+    };
+    float x[8], y[8];
+    auto request = [&](const Unit& n) {
+        const int64_t tt = t;
+        const T* src = n.kind == 0   ? static_cast<const T*>(a.in.q) + tt * a.in.q_token + n.head * a.in.q_head
+                       : n.kind == 1 ? static_cast<const T*>(a.in.k) + tt * a.in.k_token + n.head * a.in.k_head
+                                     : static_cast<const T*>(a.in.v) + tt * a.in.v_token + n.head * a.in.v_head;
+        if (n.live) load8(src + n.d0, x);
+        if (n.live && n.paired) load8(src + n.d0 + half, y);
+    };
+    Unit n{};
+    if (u < u_end) {
+        n = decode(u);
+        request(n);
+    }
+    for (int d = tid; d < D; d += kThreads) {
+        weights[0][d] = nm.qw ? norm_weight<T>(nm, nm.qw, d) : 1.0f;
+        weights[1][d] = nm.kw ? norm_weight<T>(nm, nm.kw, d) : 1.0f;
+    }
+    const int seq = sequence_of(v, t, tid & 63);
+    if (seq >= v.c.batch || t < v.c.cu[seq]) return;  // a token of no sequence (the same in every wave)
+    const int row = row_behind(cached_rows(v, seq), t - max(v.c.cu[seq], 0));
+    const int page = page_of(v, seq, row), slot = row & (v.c.page_size - 1);
+    if (tid < half) cs[tid] = cos_sin(fr.turn[tid], a.in.positions ? a.in.positions[nm.axis[tid] * nm.axis_stride + t] : row);
+    __syncthreads();
+    const int64_t k_at = page * v.c.k_page + slot * v.c.k_slot, v_at = page * v.c.v_page + slot * v.c.v_slot;
+    const float mean = 1.0f / static_cast<float>(D);
+    while (u < u_end) {
+        const Unit cur = n;
+        float p[8], r[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            p[e] = x[e];
+            r[e] = y[e];
+        }
+        u += kThreads;
+        if (u < u_end) {  // the next unit's loads are out before this one's stores
+            n = decode(u);
+            request(n);
+        }
+        if (cur.kind != 2) {
+            if (cur.kind == 0 ? nm.qw != nullptr : nm.kw != nullptr) {
+                float squares = 0.0f;
+                if (cur.live)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) squares += p[e] * p[e];
+                if (cur.live && cur.paired)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) squares += r[e] * r[e];
+                const float f = rsqrtf(group_sum(squares, lane_shift) * mean + nm.eps);
+                const float* w = weights[cur.kind] + cur.d0;
+                if (cur.live)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) p[e] *= f * w[e];
+                if (cur.live && cur.paired)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) r[e] *= f * w[half + e];
+            }
+            if (!cur.live) continue;
+            if constexpr (kNeox) {
+                if (cur.paired) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float2 w = cs[cur.d0 + e];
+                        const float f = p[e], g = r[e];
+                        p[e] = f * w.x - g * w.y;
+                        r[e] = f * w.y + g * w.x;
+                    }
+                }
+            } else if (cur.d0 < 2 * half) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 w = cs[cur.d0 / 2 + e];
+                    const float f = p[2 * e], g = p[2 * e + 1];
+                    p[2 * e] = f * w.x - g * w.y;
+                    p[2 * e + 1] = f * w.y + g * w.x;
+                }
+            }
+        }
+        if (cur.kind == 0) {
+            const int64_t at = static_cast<int64_t>(t) * a.in.qo_token + cur.head * a.in.qo_head + cur.d0;
+            store8<T, false>(a.in.q_out, at, p, 1.0f, 1.0f, 1);
+            if (cur.paired) store8<T, false>(a.in.q_out, at + half, r, 1.0f, 1.0f, 1);
+        } else if (page >= 0) {
+            if (cur.kind == 1) {
+                const int64_t at = k_at + cur.head * v.c.k_head + cur.d0;
+                store8<T, kFp8>(v.c.k, at, p, a.k_div, a.k_mul, a.k_exact);
+                if (cur.paired) store8<T, kFp8>(v.c.k, at + half, r, a.k_div, a.k_mul, a.k_exact);
+            } else {
+                store8<T, kFp8>(v.c.v, v_at + cur.head * v.c.v_head + cur.d0, p, a.v_div, a.v_mul, a.v_exact);
+            }
+        }
+    }
+}
+
 // Every alignment, rotation and head size: one wave per head of a token, its dimensions through LDS for the partner of
 // each rotated one.  Block (x, y): token, four heads (queries, keys, then values).
 template <class T, bool kFp8>
@@ -568,7 +709,10 @@ int append(const qmm_paged_kv* kv, const qmm_paged_new* in, const qmm_paged_norm
     // interleaved pairs lie within 8 dimensions
     a.units_rot = vec && !in->neox ? D / 8 : (D - rot / 2) / step;
     a.units_v = D / step;
-    const int64_t units = static_cast<int64_t>(heads + v.c.kv_heads) * a.units_rot + static_cast<int64_t>(v.c.kv_heads) * a.units_v;
+    const bool normed = norm && (norm->axes || norm->q_weight || norm->k_weight);
+    int lane_shift = 2;  // of a head's lanes, where its dimensions' squares are summed up
+    while (1 << lane_shift < a.units_rot) ++lane_shift;
+    const int64_t units = static_cast<int64_t>(heads + v.c.kv_heads) * (normed && vec ? 1 << lane_shift : a.units_rot) + static_cast<int64_t>(v.c.kv_heads) * a.units_v;
     if (units > (1 << 30)) return bad("too many heads.");
     a.units = static_cast<int>(units);
     // A block takes a whole token where that leaves a thousand blocks, as its angles then serve all heads (6818 tokens of 80
@@ -579,7 +723,18 @@ int append(const qmm_paged_kv* kv, const qmm_paged_new* in, const qmm_paged_norm
     if (grid.y > 65535) return bad("too many heads.");
     static const RopeTurns none{};
     const RopeTurns& fr = rot > 0 ? rope_turns(in->freq_base, rot) : none;
-    if (norm && (norm->axes || norm->q_weight || norm->k_weight)) {
+    if (normed && vec) {
+        auto vector = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, stream, v, a, nm, fr, lane_shift); };
+        auto pick = [&](auto tc, auto f8) {
+            using T = decltype(tc);
+            constexpr bool F = decltype(f8)::value;
+            in->neox ? vector(append_normed_kernel<T, F, true>) : vector(append_normed_kernel<T, F, false>);
+        };
+        if (in->dtype == QMM_DTYPE_F16) fp8 ? pick(_Float16{}, std::true_type{}) : pick(_Float16{}, std::false_type{});
+        else fp8 ? pick(__bf16{}, std::true_type{}) : pick(__bf16{}, std::false_type{});
+        return launched(hipGetLastError(), "paged append kernel launch");
+    }
+    if (normed) {
         const dim3 by_head(static_cast<unsigned>(in->tokens), static_cast<unsigned>((heads + 2 * v.c.kv_heads + 3) / 4));
         auto scalar = [&](auto kern) { hipLaunchKernelGGL(kern, by_head, dim3(kThreads), 0, stream, v, a, nm, fr); };
         if (in->dtype == QMM_DTYPE_F16) fp8 ? scalar(append_normed_scalar_kernel<_Float16, true>) : scalar(append_normed_scalar_kernel<_Float16, false>);
