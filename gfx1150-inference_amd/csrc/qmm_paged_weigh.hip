@@ -14,6 +14,16 @@ struct WeighArgs {
     int blocks;  // along the rows
 };
 
+// The sum over the 16 lanes of a row of lanes, in all of them.
+__device__ __forceinline__ float row_sum(float x) {
+    auto step = [&](auto ctrl) { x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xF, 0xF, false)); };
+    step(std::integral_constant<int, 0xB1>{});   // lane ^ 1
+    step(std::integral_constant<int, 0x4E>{});   // lane ^ 2
+    step(std::integral_constant<int, 0x141>{});  // the mirrored lane of 8
+    step(std::integral_constant<int, 0x140>{});  // .. and of 16
+    return x;
+}
+
 // The rows of a sequence that have a sum.
 __device__ __forceinline__ int summed_rows(const WeighArgs& wa, const Span& s) {
     return static_cast<int>(min(static_cast<int64_t>(s.ctx) + s.n, static_cast<int64_t>(wa.w.rows)));
@@ -54,6 +64,277 @@ __global__ __launch_bounds__(kThreads) void weigh_lanes_kernel(View v, AttnArgs 
     }
 }
 
+// ---- matrix-core kernels ---------------------------------------------------------------------------
+// A workgroup takes a share of the call's steps of kStep keys, in the order sequence, kv head, key: every sum is one
+// workgroup's, and no sequence's length leaves the others waiting.
+template <int kStep>
+struct Steps {
+    int seq, g, step, left;  // where a share begins; the sequence's steps from there on
+
+    static __device__ __forceinline__ int of(const View& v, const AttnArgs& a, const WeighArgs& wa, int b) {
+        if (b >= v.c.batch) return 0;
+        return (summed_rows(wa, span_of<Lse>(v, a, b)) + kStep - 1) / kStep;
+    }
+    // every lane of the wave must be active
+    static __device__ __forceinline__ int count(const View& v, const AttnArgs& a, const WeighArgs& wa, int lane) {
+        int n = 0;
+        for (int b0 = 0; b0 < v.c.batch; b0 += 64) n += __builtin_amdgcn_readlane(wave_scan(of(v, a, wa, b0 + lane)), 63);
+        return n * v.c.kv_heads;
+    }
+    // Finds step `at` of them, which is below the count.
+    __device__ __forceinline__ void find(const View& v, const AttnArgs& a, const WeighArgs& wa, int at, int lane) {
+        int before = 0;
+        for (int b0 = 0; b0 < v.c.batch; b0 += 64) {
+            const int own = of(v, a, wa, b0 + lane) * v.c.kv_heads, upto = wave_scan(own);
+            const int here = min(v.c.batch - b0, 64);
+            const int hit = static_cast<int>(__popcll(__ballot(lane < here && before + upto <= at)));
+            if (hit < here) {
+                const int steps = __builtin_amdgcn_readlane(own, hit), rest = at - (before + __builtin_amdgcn_readlane(upto - own, hit));
+                const int each = steps / v.c.kv_heads;
+                seq = b0 + hit;
+                g = rest / each;
+                step = rest % each;
+                left = each - step;
+                return;
+            }
+            before += __builtin_amdgcn_readlane(upto, here - 1);
+        }
+    }
+};
+
+// Up to 16 NT rows (tokens x query heads of one kv head): decoding, small trees.  As in the attention over them a wave takes 32 keys
+// at a time, straight into registers, and lane (l, q) = (lane % 16, lane / 16) receives the scores of row l with keys 4q ..
+// 4q + 3 of each 16; their weights are added up over the 16 lanes.
+constexpr int kRowsKeys = 128;
+
+template <class T, class C, int D, int NT>
+__global__ __launch_bounds__(kThreads) void weigh_rows_kernel(View v, AttnArgs a, WeighArgs wa) {
+    using F = Frag<T>;
+    using v8 = typename F::v8;
+    constexpr bool kFp8 = std::is_same_v<C, Fp8>;
+    constexpr int kF = D / 32;
+    const int kvh = v.c.kv_heads, group = a.in.heads / kvh;
+    const int lane = threadIdx.x & 63, l = lane & 15, q = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int steps = Steps<kRowsKeys>::count(v, a, wa, lane), share = (steps + gridDim.x - 1) / gridDim.x;
+    int at = blockIdx.x * share;
+    const int until = min(steps, at + share);
+    const uint32_t k_off = static_cast<uint32_t>((l * v.c.k_slot + (kFp8 ? 16 : 8) * q) * sizeof(C));
+    const uint32_t k_last = static_cast<uint32_t>((l * v.c.k_slot + 32 * (kF - 1) + 8 * q) * sizeof(C));  // fp8, an odd count of 32 dims
+    while (at < until) {
+        Steps<kRowsKeys> st;
+        st.find(v, a, wa, at, lane);
+        const int run = min(st.left, until - at), g = st.g;
+        at += run;
+        const Span s = span_of<Lse>(v, a, st.seq);
+        const int held = summed_rows(wa, s), n_rows = min(s.n, a.in.max_new) * group;
+        const float* from = wa.w.old_sums + st.seq * wa.w.old_batch + g * wa.w.old_head;
+        float* to = wa.w.new_sums + st.seq * wa.w.new_batch + g * wa.w.new_head;
+        // queries and their logarithms: rows past the last repeat it, and do not count
+        v8 qf[NT][kF];
+        float lse[NT];
+        int tok[NT];
+        bool counts[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = max(min(16 * nt + l, n_rows - 1), 0);
+            tok[nt] = r / group;
+            counts[nt] = 16 * nt + l < n_rows;
+            lse[nt] = 0.0f;
+            if (n_rows > 0) {
+                const int head = g * group + r % group;
+                const T* qrow = static_cast<const T*>(a.in.q) + static_cast<int64_t>(s.first + tok[nt]) * a.in.q_token + head * a.in.q_head;
+#pragma unroll
+                for (int f = 0; f < kF; ++f) {
+                    const int d = kFp8 && (f | 1) < kF ? 64 * (f >> 1) + 16 * q + 8 * (f & 1) : 32 * f + 8 * q;
+                    __builtin_memcpy(&qf[nt][f], __builtin_assume_aligned(qrow + d, 16), 16);
+                }
+                lse[nt] = a.lse[static_cast<int64_t>(s.first + tok[nt]) * a.in.heads + head];
+            }
+        }
+        const char* kbase = reinterpret_cast<const char*>(static_cast<const C*>(v.c.k) + g * v.c.k_head);
+        auto page_at = [&](int k0) { return n_rows > 0 && k0 < s.total ? page_of(v, s.seq, k0) : -1; };
+        int kb = st.step * kRowsKeys + 32 * w;
+        int id[2] = {page_at(kb), page_at(kb + 16)};
+#pragma unroll 1
+        for (int i = 0; i < run; ++i, kb += kRowsKeys) {
+            u32x4 kr[2][kFp8 ? (kF + 1) / 2 : kF];
+            bool ok[2];
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) {
+                const int k0 = kb + 16 * tt, u = __builtin_amdgcn_readfirstlane(id[tt]);
+                ok[tt] = u >= 0;
+                const char* kp = kbase + (static_cast<int64_t>(max(u, 0)) * v.c.k_page + (k0 & (v.c.page_size - 1)) * v.c.k_slot) * static_cast<int64_t>(sizeof(C));
+#pragma unroll
+                for (int f = 0; f < (kFp8 ? kF / 2 : kF); ++f) {
+                    uint32_t x[4];
+                    load_row_bytes<16, 16, true>(x, kp + 64 * f + k_off);
+                    kr[tt][f] = u32x4{x[0], x[1], x[2], x[3]};
+                }
+                if constexpr (kFp8 && kF % 2) {
+                    const u32x2 x = *reinterpret_cast<const u32x2*>(kp + k_last);
+                    kr[tt][kF / 2] = u32x4{x[0], x[1], 0, 0};
+                }
+            }
+            // lane (l < 8, q) ends up with key 16 (l / 4) + 4q + l % 4
+            const int own = kb + 16 * ((l >> 2) & 1) + 4 * q + (l & 3);
+            float old = 0.0f;
+            if (l < 8 && own < min(s.ctx, held)) old = from[own];
+            id[0] = page_at(kb + kRowsKeys);
+            id[1] = page_at(kb + kRowsKeys + 16);
+            __builtin_amdgcn_sched_barrier(0);
+            const bool full = kb + 32 <= s.ctx && ok[0] && ok[1];
+            v8 kf[2][kF];
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                for (int f = 0; f < kF; ++f) {
+                    if constexpr (kFp8) {
+                        const uint32_t x = kr[tt][f >> 1][2 * (f & 1)], y = kr[tt][f >> 1][2 * (f & 1) + 1];
+                        const u32x4 t = {F::from_fp8(x), F::from_fp8_hi(x), F::from_fp8(y), F::from_fp8_hi(y)};
+                        kf[tt][f] = __builtin_bit_cast(v8, t);
+                    } else {
+                        kf[tt][f] = __builtin_bit_cast(v8, kr[tt][f]);
+                    }
+                }
+            float sum[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e] = 0.0f;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                uint32_t vis = 0xFFFFFFFFu;
+                if (!full) {
+                    vis = visible32(a, s, tok[nt], kb);
+                    if (!ok[0]) vis &= 0xFFFF0000u;
+                    if (!ok[1]) vis &= 0x0000FFFFu;
+                }
+                vis = counts[nt] ? vis >> (4 * q) : 0;
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt) {
+                    f32x4 sc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int f = 0; f < kF; ++f) sc = F::mma16(kf[tt][f], qf[nt][f], sc);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float p = __builtin_amdgcn_exp2f(__fmaf_rn(sc[e], a.scale_log2, -lse[nt]));
+                        sum[4 * tt + e] += (vis >> (16 * tt + e)) & 1 ? p : 0.0f;
+                    }
+                }
+            }
+            float mine = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float x = row_sum(sum[e]);
+                if (l == e) mine = x;
+            }
+            if (l < 8 && own < held) to[own] = old + mine;
+        }
+    }
+}
+
+// More rows.  A workgroup takes 64 keys, held in registers as an operand of 32x32x16, and its waves the rows in turns of 32: a lane
+// has one row (lane % 32) and 16 of every 32 keys, so that a row's logarithm is the lane's and the sums of its keys gather in
+// registers; they are added up over the lanes and the waves, in order, at the end.
+constexpr int kTileKeysW = 64;
+
+template <class T, class C, int D>
+__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void weigh_tile_kernel(View v, AttnArgs a, WeighArgs wa) {
+    using F = Frag<T>;
+    using v8 = typename F::v8;
+    constexpr bool kFp8 = std::is_same_v<C, Fp8>;
+    __shared__ float part[4][kTileKeysW];
+    const int kvh = v.c.kv_heads, group = a.in.heads / kvh;
+    const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int steps = Steps<kTileKeysW>::count(v, a, wa, lane);
+    for (int at = blockIdx.x; at < steps; at += gridDim.x) {
+        Steps<kTileKeysW> st;
+        st.find(v, a, wa, at, lane);
+        const Span s = span_of<Lse>(v, a, st.seq);
+        const int g = st.g, held = summed_rows(wa, s), n_rows = min(s.n, a.in.max_new) * group, kb = st.step * kTileKeysW;
+        // keys: lane's key l32 of each 32, dims 16 db + 8 h ..
+        v8 kf[2][D / 16];
+        uint32_t have = 0;  // bit t: the page of keys 16 t .. is there
+        if (n_rows > 0) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                if (kb + 16 * t < s.total && page_of(v, s.seq, kb + 16 * t) >= 0) have |= 1u << t;
+            const C* kbase = static_cast<const C*>(v.c.k) + g * v.c.k_head;
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+                const int k = kb + 32 * hh + l32, id = k < s.total ? page_of(v, s.seq, k) : -1;
+                const C* kp = kbase + static_cast<int64_t>(max(id, 0)) * v.c.k_page + (k & (v.c.page_size - 1)) * v.c.k_slot + 8 * h;
+#pragma unroll
+                for (int db = 0; db < D / 16; ++db) {
+                    if constexpr (kFp8) {
+                        const u32x2 x = *reinterpret_cast<const u32x2*>(kp + 16 * db);
+                        const u32x4 y = {F::from_fp8(x[0]), F::from_fp8_hi(x[0]), F::from_fp8(x[1]), F::from_fp8_hi(x[1])};
+                        kf[hh][db] = __builtin_bit_cast(v8, y);
+                    } else {
+                        __builtin_memcpy(&kf[hh][db], __builtin_assume_aligned(kp + 16 * db, 16), 16);
+                    }
+                }
+            }
+        }
+        f32x16 sum[2];
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sum[hh][e] = 0.0f;
+        const bool cached = kb + kTileKeysW <= s.ctx && have == 15;
+        // a chain's rows ahead of the first key see none of them
+        const int first = a.in.mask == nullptr ? max(kb - s.ctx, 0) * group / 32 : 0;
+#pragma unroll 1
+        for (int r0 = 32 * (first + ((w - first) & 3)); r0 < n_rows; r0 += 128) {
+            const int r = min(r0 + l32, n_rows - 1), i = r / group, head = g * group + r % group;
+            const T* qrow = static_cast<const T*>(a.in.q) + static_cast<int64_t>(s.first + i) * a.in.q_token + head * a.in.q_head + 8 * h;
+            v8 qf[D / 16];
+#pragma unroll
+            for (int db = 0; db < D / 16; ++db) __builtin_memcpy(&qf[db], __builtin_assume_aligned(qrow + 16 * db, 16), 16);
+            const float lse = a.lse[static_cast<int64_t>(s.first + i) * a.in.heads + head];
+            const bool counts = r0 + l32 < n_rows;
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+                f32x16 x;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = 0.0f;
+#pragma unroll
+                for (int db = 0; db < D / 16; ++db) x = F::mma32(kf[hh][db], qf[db], x);
+                uint32_t vis = 0xFFFFFFFFu;
+                if (!cached) {
+                    vis = visible32(a, s, i, kb + 32 * hh);
+                    if (!((have >> (2 * hh)) & 1)) vis &= 0xFFFF0000u;
+                    if (!((have >> (2 * hh + 1)) & 1)) vis &= 0x0000FFFFu;
+                }
+                vis = counts ? vis >> (4 * h) : 0;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float p = __builtin_amdgcn_exp2f(__fmaf_rn(x[e], a.scale_log2, -lse));
+                    sum[hh][e] += (vis >> (8 * (e >> 2) + (e & 3))) & 1 ? p : 0.0f;
+                }
+            }
+        }
+        // register e of half hh is key 32 hh + 8 (e / 4) + 4 h + e % 4
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                float x = row_sum(sum[hh][e]);
+                x += __shfl_xor(x, 16, 64);
+                if (l32 == 0) part[w][32 * hh + 8 * (e >> 2) + 4 * h + (e & 3)] = x;
+            }
+        __syncthreads();
+        const int k = kb + static_cast<int>(threadIdx.x);
+        if (threadIdx.x < kTileKeysW && k < held) {
+            const int c = threadIdx.x;
+            const float x = ((part[0][c] + part[1][c]) + part[2][c]) + part[3][c];
+            const float* from = wa.w.old_sums + st.seq * wa.w.old_batch + g * wa.w.old_head;
+            wa.w.new_sums[st.seq * wa.w.new_batch + g * wa.w.new_head + k] = k < s.ctx ? from[k] + x : x;
+        }
+        __syncthreads();
+    }
+}
+
 struct WeighPlan {
     Plan attend;
     size_t lse, bytes;  // where the logarithms begin
@@ -75,6 +356,33 @@ int check_weights(const View& v, const qmm_paged_weights* w) {
     if (w->old_sums == w->new_sums && (w->old_batch != w->new_batch || w->old_head != w->new_head)) return bad("sums in place need the same strides.");
     if (v.c.kv_heads > 65535) return bad("too many heads.");
     return QMM_OK;
+}
+
+// Calls f with the matrix-core kernel for a call's rows and types.
+template <class T, class C, int D, class Fn>
+void with_weigh_kernel(int64_t rows, Fn f) {
+    if (rows <= 16) return f(weigh_rows_kernel<T, C, D, 1>);
+    if (rows <= 32) return f(weigh_rows_kernel<T, C, D, 2>);
+    if (D <= 128 && rows <= 64) return f(weigh_rows_kernel<T, C, D, D <= 128 ? 4 : 2>);
+    f(weigh_tile_kernel<T, C, D>);
+}
+
+template <class Fn>
+void with_weigh_kernel(const View& v, const qmm_paged_query& in, Fn f) {
+    const int64_t rows = static_cast<int64_t>(std::min(in.max_new, in.tokens)) * (in.heads / v.c.kv_heads);
+    auto types = [&](auto tc, auto cc) {
+        using T = decltype(tc);
+        using C = decltype(cc);
+        switch (v.c.head_dim) {
+            case 64: return with_weigh_kernel<T, C, 64>(rows, f);
+            case 96: return with_weigh_kernel<T, C, 96>(rows, f);
+            case 128: return with_weigh_kernel<T, C, 128>(rows, f);
+            default: return with_weigh_kernel<T, C, 256>(rows, f);
+        }
+    };
+    const bool fp8 = v.c.dtype == QMM_DTYPE_E4M3;
+    if (in.dtype == QMM_DTYPE_F16) return fp8 ? types(_Float16{}, Fp8{}) : types(_Float16{}, _Float16{});
+    return fp8 ? types(__bf16{}, Fp8{}) : types(__bf16{}, __bf16{});
 }
 
 int weighted_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, const qmm_paged_weights* weights, void* workspace,
@@ -101,9 +409,17 @@ int weighted_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, const 
         if (rc == QMM_OK && p.attend.merge) rc = launch_merge<Lse>(v, a, p.attend.kind != Kind::kLanes, p.attend.most_ranges, stream);
         if (rc != QMM_OK) return rc;
     }
-    // a row of no sequence has no sum; what the table can hold bounds the cached ones that have been given pages
     WeighArgs wa{*weights, 1};
     if (weights->rows == 0) return QMM_OK;
+    if (p.attend.kind != Kind::kLanes) {
+        with_weigh_kernel(v, *in, [&](auto kern) {
+            // workgroups that run at once, or one for each step that there can be
+            const int64_t steps = static_cast<int64_t>(v.c.batch) * v.c.kv_heads * ((weights->rows + kTileKeysW - 1) / kTileKeysW);
+            const int64_t blocks = std::min<int64_t>(kernel_slots(kern, 0), steps);
+            hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream, v, a, wa);
+        });
+        return launched(hipGetLastError(), "paged weights kernel launch");
+    }
     const int keys = 4 * (64 / (v.c.head_dim <= 64 ? 8 : v.c.head_dim <= 128 ? 16 : 32));
     wa.blocks = static_cast<int>(std::min<int64_t>((weights->rows + keys - 1) / keys, 1024));
     const dim3 grid(static_cast<unsigned>(wa.blocks), static_cast<unsigned>(v.c.kv_heads), static_cast<unsigned>(v.c.batch));
