@@ -4,12 +4,14 @@
 #include "qmm_paged.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace qmm {
 namespace paged {
 namespace {
 
 constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
+static_assert(kSelectWaves == 16, "a row of lanes adds up the waves' counts");
 constexpr int kThreads = 256;
 
 struct EvictArgs {
@@ -28,16 +30,27 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     return b >> 31 ? ~b : b | 0x80000000u;
 }
 
-// Block (x, y, z): kv head, sequence, layer.  The m-th largest weight of the rows in between is found bit by bit from the
-// top, each bit by a count of the weights at or above the number so far with the bit set; then the kept rows are
-// listed in order, those equal to it as far as there is room.
-__global__ __launch_bounds__(kSelectThreads) void select_kernel(View v, EvictArgs a) {
-    __shared__ int counts[2][kSelectWaves];
-    __shared__ int2 scan[kSelectWaves];
+// Block (x, y, z): kv head, sequence, layer.  The m-th largest weight of the rows in between is found from the top, two bits at a
+// time, by counts of the weights at or above the three numbers that the bits so far begin; where a count is m, those are
+// the rows.  Then the kept rows are listed in order, of those equal to the m-th largest the first ones.  Weights of up to
+// kHeld 1024 rows wait in registers (a count is a comparison and a scalar population count for each 64 of them, with no atomics to
+// meet on); of longer sequences (kHeld 0) they are read for each count.
+template <int kHeld>
+__global__ __launch_bounds__(kSelectThreads, kHeld <= 16 ? 8 : 4) void select_kernel(View v, EvictArgs a) {
+    __shared__ int counts[2][4][kSelectWaves];  // [turn][number][wave]
+    __shared__ int2 scan[kHeld ? kHeld : 1][kSelectWaves];
     const int g = blockIdx.x, b = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int n = table_rows(v, b), keep = a.e.keep;
+    const int keep = a.e.keep;
     const float* weights = a.e.weights + layer * a.e.w_layer + b * a.e.w_batch + g * a.e.w_head;
+    float loaded[kHeld ? kHeld : 1];  // requested ahead of the sequence's length
+    if constexpr (kHeld > 0)
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const int j = i * kSelectThreads + tid;
+            loaded[i] = j < a.e.rows ? weights[j] : -INFINITY;
+        }
+    const int n = table_rows(v, b);
     float* out = a.e.weights_out + layer * a.e.wo_layer + b * a.e.wo_batch + g * a.e.wo_head;
     if (g == 0 && layer == 0) {
         const int pages = (keep + v.c.page_size - 1) >> v.page_shift;
@@ -50,95 +63,161 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(View v, EvictArg
         for (int j = tid; j < a.e.rows; j += kSelectThreads) out[j] = j < n ? weights[j] : 0.0f;
         return;
     }
-    for (int j = keep + tid; j < a.e.rows; j += kSelectThreads) out[j] = 0.0f;
     const int first = a.e.sinks, last = n - a.e.recent, need = keep - a.e.sinks - a.e.recent;
-    auto rank = [&](int j) { return ordered(j < a.e.rows ? weights[j] : -INFINITY); };
-    uint32_t limit = 0;
-    int above = 0;  // weights above the limit
-    if (need > 0) {
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t probe = limit | (1u << bit);
-            int count = 0;
-            for (int j0 = first; j0 < last; j0 += kSelectThreads) {
-                const int j = j0 + tid;
-                count += static_cast<int>(__popcll(__ballot(j < last && rank(j) >= probe)));
-            }
-            if (lane == 0) counts[bit & 1][w] = count;
-            __syncthreads();
-            int total = 0;
-            for (int i = 0; i < kSelectWaves; ++i) total += counts[bit & 1][i];
-            if (total >= need) limit = probe;
-            else above = total;
+    // of a row in between, at least ordered(-inf); 0 of the others, which no count meets
+    auto between = [&](int j) { return j >= first && j < last; };
+    auto rank = [&](int j) { return between(j) ? ordered(j < a.e.rows ? weights[j] : -INFINITY) : 0u; };
+    uint32_t held[kHeld ? kHeld : 1];
+    if constexpr (kHeld > 0)
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) held[i] = between(i * kSelectThreads + tid) ? ordered(loaded[i]) : 0u;
+    for (int j = keep + tid; j < a.e.rows; j += kSelectThreads) out[j] = 0.0f;
+    uint32_t limit = 0;     // rows above it stay, and the first at_limit of those at it
+    int above = 0;          // rows above
+    if (need == 0) limit = 0xFFFFFFFFu;
+    for (int bit = 30; bit >= 0 && need > 0; bit -= 2) {
+        int count[3] = {0, 0, 0};
+        auto add = [&](uint32_t r) {
+#pragma unroll
+            for (int c = 0; c < 3; ++c) count[c] += static_cast<int>(__popcll(__ballot(r >= (limit | static_cast<uint32_t>(c + 1) << bit))));
+        };
+        if constexpr (kHeld > 0) {
+#pragma unroll
+            for (int i = 0; i < kHeld; i += 4)
+                if (i * kSelectThreads < last)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) add(held[i + k]);
+        } else {
+            for (int j0 = first; j0 < last; j0 += kSelectThreads) add(rank(j0 + tid));
+        }
+        if (lane < 3) counts[(bit >> 1) & 1][lane][w] = lane == 0 ? count[0] : lane == 1 ? count[1] : count[2];
+        __syncthreads();
+        // 16 lanes add up a number's counts (the last 16 read what is never written)
+        int all = counts[(bit >> 1) & 1][lane / kSelectWaves][lane % kSelectWaves];
+        auto fold = [&](auto ctrl) { all += __builtin_amdgcn_update_dpp(0, all, decltype(ctrl)::value, 0xF, 0xF, false); };
+        fold(std::integral_constant<int, 0xB1>{});   // lane ^ 1
+        fold(std::integral_constant<int, 0x4E>{});   // lane ^ 2
+        fold(std::integral_constant<int, 0x141>{});  // the mirrored lane of 8
+        fold(std::integral_constant<int, 0x140>{});  // .. and of 16
+        const int total[3] = {__builtin_amdgcn_readlane(all, 0), __builtin_amdgcn_readlane(all, 16), __builtin_amdgcn_readlane(all, 32)};
+        int most = 0;  // the largest two bits that leave enough
+#pragma unroll
+        for (int c = 0; c < 3; ++c) {
+            if (total[c] >= need) most = c + 1;
+        }
+        if (most < 3) above = total[most];
+        if (most > 0) limit |= static_cast<uint32_t>(most) << bit;
+        if (most > 0 && total[most - 1] == need) {  // these are the rows
+            --limit;
+            above = need;
+            break;
         }
     }
-    // kept rows of a step of 1024: those above the limit, and the first of those at it
-    int32_t* list = a.list + ((static_cast<int64_t>(layer) * v.c.batch + b) * v.c.kv_heads + g) * keep;
     const int at_limit = need - above;
-    int taken = 0, equal = 0;
-    for (int j0 = 0; j0 < n; j0 += kSelectThreads) {
-        const int j = j0 + tid;
-        const bool outer = j < n && (j < first || j >= last);
-        const uint32_t r = j < n && !outer ? rank(j) : 0;
-        const bool inner = j < n && !outer && need > 0;
-        const uint64_t below = (uint64_t{1} << lane) - 1;
-        const uint64_t over = __ballot(outer || (inner && r > limit)), same = __ballot(inner && r == limit);
-        if (lane == 0) scan[w] = int2{static_cast<int>(__popcll(over)), static_cast<int>(__popcll(same))};
-        __syncthreads();
-        int o = taken, e = equal;
-        for (int i = 0; i < kSelectWaves; ++i) {
-            if (i < w) {
-                o += scan[i].x;
-                e += scan[i].y;
-            }
-            taken += scan[i].x;
-            equal += scan[i].y;
-        }
-        e += static_cast<int>(__popcll(same & below));
-        o += static_cast<int>(__popcll(over & below));
-        const bool keeps = (over >> lane) & 1 || ((same >> lane) & 1 && e < at_limit);
+    int32_t* list = a.list + ((static_cast<int64_t>(layer) * v.c.batch + b) * v.c.kv_heads + g) * keep;
+    const uint64_t below = (uint64_t{1} << lane) - 1;
+    auto stays = [&](int j, uint32_t r) { return j < n && (j < first || j >= last || r > limit); };
+    auto equal = [&](int j, uint32_t r) { return at_limit > 0 && r == limit && j >= first && j < last; };
+    auto put = [&](int j, uint64_t over, uint64_t same, int2 ahead) {
+        const int o = ahead.x + static_cast<int>(__popcll(over & below)), e = ahead.y + static_cast<int>(__popcll(same & below));
+        if (!((over >> lane) & 1) && !((same >> lane) & 1 && e < at_limit)) return;
         const int place = o + min(e, at_limit);
-        if (keeps && place < keep) {
-            list[place] = j;
-            if (place < a.e.rows) out[place] = j < a.e.rows ? weights[j] : 0.0f;
+        if (place >= keep) return;
+        list[place] = j;
+        if (place < a.e.rows) out[place] = j < a.e.rows ? weights[j] : 0.0f;
+    };
+    auto number = [](uint64_t over, uint64_t same) { return int2{static_cast<int>(__popcll(over)), static_cast<int>(__popcll(same))}; };
+    if constexpr (kHeld > 0) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const int j = i * kSelectThreads + tid;
+            const uint64_t over = __ballot(stays(j, held[i])), same = __ballot(equal(j, held[i]));
+            if (lane == 0) scan[i][w] = number(over, same);
         }
         __syncthreads();
+        if (w == 0) {  // what is ahead of every 64 rows
+            int2 base{0, 0};
+            for (int i0 = 0; i0 < kHeld * kSelectWaves; i0 += 64) {
+                int2* at = &scan[0][0] + i0 + lane;
+                const int2 x = i0 + lane < kHeld * kSelectWaves ? *at : int2{0, 0};
+                int2 s = x;
+                for (int o = 1; o < 64; o <<= 1) {
+                    const int sx = __shfl_up(s.x, o, 64), sy = __shfl_up(s.y, o, 64);
+                    if (lane >= o) s = int2{s.x + sx, s.y + sy};
+                }
+                if (i0 + lane < kHeld * kSelectWaves) *at = int2{base.x + s.x - x.x, base.y + s.y - x.y};
+                base = int2{base.x + __shfl(s.x, 63, 64), base.y + __shfl(s.y, 63, 64)};
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const int j = i * kSelectThreads + tid;
+            if (i * kSelectThreads < n) put(j, __ballot(stays(j, held[i])), __ballot(equal(j, held[i])), scan[i][w]);
+        }
+    } else {
+        int2 ahead{0, 0};
+        for (int j0 = 0; j0 < n; j0 += kSelectThreads) {
+            const int j = j0 + tid;
+            const uint32_t r = rank(j);
+            const uint64_t over = __ballot(stays(j, r)), same = __ballot(equal(j, r));
+            if (lane == 0) scan[0][w] = number(over, same);
+            __syncthreads();
+            int2 mine = ahead;
+            for (int i = 0; i < kSelectWaves; ++i) {
+                const int2 x = scan[0][i];
+                if (i < w) mine = int2{mine.x + x.x, mine.y + x.y};
+                ahead = int2{ahead.x + x.x, ahead.y + x.y};
+            }
+            put(j, over, same, mine);
+            __syncthreads();
+        }
     }
 }
 
-// Copies the kept rows.  Block (x, y, z): 256 units of (row, piece) a pass, sequence and kv head, layer.
-constexpr int kRowsAtOnce = 4;  // of K and of V, per thread
+// Copies the kept rows.  Block (x, y, z): a run of rows, sequence and kv head, layer; a thread keeps its piece of a row and takes every
+// (kThreads / per_row)-th row, kRowsAtOnce of K and of V at once.
+constexpr int kRowsAtOnce = 4;
 
 template <int B>
-__global__ __launch_bounds__(kThreads) void gather_kernel(View v, Strides st, EvictArgs a) {
+__global__ __launch_bounds__(kThreads) void gather_kernel(View v, Strides st, EvictArgs a, int rows_each) {
     using U = typename Unit<B>::type;
     const int b = blockIdx.y / v.c.kv_heads, g = blockIdx.y % v.c.kv_heads, layer = blockIdx.z, keep = a.e.keep;
     if (table_rows(v, b) <= keep) return;
+    const int abreast = max(kThreads / st.per_row, 1), sub = static_cast<int>(threadIdx.x) / st.per_row;
+    if (sub >= abreast) return;
     const int32_t* list = a.list + ((static_cast<int64_t>(layer) * v.c.batch + b) * v.c.kv_heads + g) * keep;
+    const int32_t* fresh = a.e.fresh + b * a.e.fresh_stride;
     U* k = static_cast<U*>(v.c.k) + layer * st.k_layer + g * st.k_head;
     U* x = static_cast<U*>(v.c.v) + layer * st.v_layer + g * st.v_head;
-    const int64_t total = static_cast<int64_t>(keep) * st.per_row, step = static_cast<int64_t>(gridDim.x) * kThreads;
-    for (int64_t at = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; at < total; at += kRowsAtOnce * step) {
-        U rk[kRowsAtOnce], rv[kRowsAtOnce];
-        int64_t to_k[kRowsAtOnce], to_v[kRowsAtOnce];
+    const int begin = blockIdx.x * rows_each, end = begin + min(rows_each, keep - begin);
+    for (int piece = static_cast<int>(threadIdx.x) % st.per_row; piece < st.per_row; piece += kThreads) {
+        for (int row = begin + sub; row < end; row += kRowsAtOnce * abreast) {
+            U rk[kRowsAtOnce], rv[kRowsAtOnce];
+            int page[kRowsAtOnce], from[kRowsAtOnce], target[kRowsAtOnce];
 #pragma unroll
-        for (int i = 0; i < kRowsAtOnce; ++i) {
-            const int64_t u = at + i * step;
-            to_k[i] = -1;
-            if (u >= total) continue;
-            const int row = static_cast<int>(u / st.per_row), piece = static_cast<int>(u % st.per_row);
-            const int from = list[row], page = page_of(v, b, from), slot = from & (v.c.page_size - 1);
-            const int target = a.e.fresh[b * a.e.fresh_stride + (row >> v.page_shift)], to = row & (v.c.page_size - 1);
-            if (page < 0 || static_cast<uint32_t>(target) >= static_cast<uint32_t>(v.c.num_pages)) continue;
-            rk[i] = k[page * st.k_page + slot * st.k_slot + piece];
-            rv[i] = x[page * st.v_page + slot * st.v_slot + piece];
-            to_k[i] = target * st.k_page + to * st.k_slot + piece;
-            to_v[i] = target * st.v_page + to * st.v_slot + piece;
-        }
+            for (int i = 0; i < kRowsAtOnce; ++i) from[i] = list[min(row + i * abreast, keep - 1)];
 #pragma unroll
-        for (int i = 0; i < kRowsAtOnce; ++i) {
-            if (to_k[i] < 0) continue;
-            k[to_k[i]] = rk[i];
-            x[to_v[i]] = rv[i];
+            for (int i = 0; i < kRowsAtOnce; ++i) {
+                const int to = min(row + i * abreast, keep - 1);
+                page[i] = page_of(v, b, from[i]);
+                target[i] = fresh[to >> v.page_shift];
+                if (row + i * abreast >= end || static_cast<uint32_t>(target[i]) >= static_cast<uint32_t>(v.c.num_pages)) page[i] = -1;
+            }
+#pragma unroll
+            for (int i = 0; i < kRowsAtOnce; ++i) {
+                if (page[i] < 0) continue;
+                const int slot = from[i] & (v.c.page_size - 1);
+                rk[i] = k[page[i] * st.k_page + slot * st.k_slot + piece];
+                rv[i] = x[page[i] * st.v_page + slot * st.v_slot + piece];
+            }
+#pragma unroll
+            for (int i = 0; i < kRowsAtOnce; ++i) {
+                if (page[i] < 0) continue;
+                const int slot = (row + i * abreast) & (v.c.page_size - 1);
+                k[target[i] * st.k_page + slot * st.k_slot + piece] = rk[i];
+                x[target[i] * st.v_page + slot * st.v_slot + piece] = rv[i];
+            }
         }
     }
 }
@@ -179,15 +258,21 @@ int evict(const qmm_paged_kv* kv, const qmm_paged_evict_args* e, void* workspace
     }
     const EvictArgs a{*e, static_cast<int32_t*>(workspace)};
     const dim3 grid(static_cast<unsigned>(v.c.kv_heads), static_cast<unsigned>(v.c.batch), static_cast<unsigned>(v.c.num_layers));
-    hipLaunchKernelGGL(select_kernel, grid, dim3(kSelectThreads), 0, stream, v, a);
+    auto select = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kSelectThreads), 0, stream, v, a); };
+    const int64_t room = static_cast<int64_t>(v.c.table_width) * v.c.page_size;  // of a sequence
+    if (room <= 4 * kSelectThreads) select(select_kernel<4>);
+    else if (room <= 8 * kSelectThreads) select(select_kernel<8>);
+    else if (room <= 16 * kSelectThreads) select(select_kernel<16>);
+    else if (room <= 32 * kSelectThreads) select(select_kernel<32>);
+    else select(select_kernel<0>);
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return launched(err, "paged evict kernel launch");
     Strides st;
     const int unit = copy_unit(v.c, &st);
-    const int64_t units = static_cast<int64_t>(e->keep) * st.per_row, each = kThreads * kRowsAtOnce;
-    const dim3 rows(static_cast<unsigned>(std::min<int64_t>((units + each - 1) / each, 1 << 20)), static_cast<unsigned>(v.c.batch * v.c.kv_heads),
+    const int rows_each = std::max(kThreads / st.per_row, 1) * kRowsAtOnce;
+    const dim3 rows(static_cast<unsigned>((e->keep + static_cast<int64_t>(rows_each) - 1) / rows_each), static_cast<unsigned>(v.c.batch * v.c.kv_heads),
                     static_cast<unsigned>(v.c.num_layers));
-    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, rows, dim3(kThreads), 0, stream, v, st, a); };
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, rows, dim3(kThreads), 0, stream, v, st, a, rows_each); };
     unit == 16 ? go(gather_kernel<16>) : unit == 4 ? go(gather_kernel<4>) : go(gather_kernel<1>);
     return launched(hipGetLastError(), "paged evict kernel launch");
 }
