@@ -208,15 +208,15 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(View v, Strides st, Ev
             for (int i = 0; i < kRowsAtOnce; ++i) {
                 if (page[i] < 0) continue;
                 const int slot = from[i] & (v.c.page_size - 1);
-                rk[i] = k[page[i] * st.k_page + slot * st.k_slot + piece];
-                rv[i] = x[page[i] * st.v_page + slot * st.v_slot + piece];
+                rk[i] = __builtin_nontemporal_load(k + page[i] * st.k_page + slot * st.k_slot + piece);
+                rv[i] = __builtin_nontemporal_load(x + page[i] * st.v_page + slot * st.v_slot + piece);
             }
 #pragma unroll
             for (int i = 0; i < kRowsAtOnce; ++i) {
                 if (page[i] < 0) continue;
                 const int slot = (row + i * abreast) & (v.c.page_size - 1);
-                k[target[i] * st.k_page + slot * st.k_slot + piece] = rk[i];
-                x[target[i] * st.v_page + slot * st.v_slot + piece] = rv[i];
+                __builtin_nontemporal_store(rk[i], k + target[i] * st.k_page + slot * st.k_slot + piece);
+                __builtin_nontemporal_store(rv[i], x + target[i] * st.v_page + slot * st.v_slot + piece);
             }
         }
     }
