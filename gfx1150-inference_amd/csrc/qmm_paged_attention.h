@@ -52,6 +52,10 @@ struct AttnArgs {
     // product, as those beside the outputs are
     float* lse;
     float* part_sum;
+    // Lse, up to 16 rows a kv head: where there is room for them, the products of queries and keys, -inf where a row does not see the
+    // key, [sequence][kv head][score_keys / 4][score_rows][4], for a second pass that would otherwise form them again
+    float* scores;
+    int score_rows, score_keys;
 };
 
 // The new tokens of one sequence.
@@ -660,6 +664,17 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
                 for (int nt = 0; nt < NT; ++nt) {
                     o[nt][dt] = F::mma16(vf, ph[nt], o[nt][dt]);
                     if constexpr (kLo) o[nt][dt] = F::mma16(vf, pl[nt], o[nt][dt]);
+                }
+            }
+            if constexpr (M::kLse && NT == 1) {
+                // last: a wait for the values would be one for these stores too
+                if (a.scores && l < n_rows) {
+                    float* at = a.scores + (static_cast<int64_t>(cp.seq) * kvh + g) * a.score_rows * a.score_keys;
+#pragma unroll
+                    for (int tt = 0; tt < 2; ++tt)
+                        if (kb + 16 * tt + 4 * q < a.score_keys)
+                            *reinterpret_cast<f32x4*>(at + ((static_cast<int64_t>(kb) / 4 + 4 * tt + q) * a.score_rows + l) * 4) =
+                                f32x4{x[0][4 * tt], x[0][4 * tt + 1], x[0][4 * tt + 2], x[0][4 * tt + 3]};
                 }
             }
         }

@@ -232,6 +232,40 @@ __global__ __launch_bounds__(kThreads) void weigh_rows_kernel(View v, AttnArgs a
     }
 }
 
+// Up to 16 rows whose scores the attention has left: 8 bytes a row and key go to memory and back where the keys would be read again
+// (256 bytes of 128 dimensions in 16 bits).  A lane takes a key.
+constexpr int kStoredKeys = kThreads;
+
+__global__ __launch_bounds__(kThreads) void weigh_stored_kernel(View v, AttnArgs a, WeighArgs wa) {
+    const int kvh = v.c.kv_heads, group = a.in.heads / kvh, lane = threadIdx.x & 63;
+    const int steps = Steps<kStoredKeys>::count(v, a, wa, lane), share = (steps + gridDim.x - 1) / gridDim.x;
+    const float scale = fabsf(a.scale_log2);  // the attention takes a negative one into its queries
+    int at = blockIdx.x * share;
+    const int until = min(steps, at + share);
+    while (at < until) {
+        Steps<kStoredKeys> st;
+        st.find(v, a, wa, at, lane);
+        const int run = min(st.left, until - at), g = st.g;
+        at += run;
+        const Span s = span_of<Lse>(v, a, st.seq);
+        const int held = summed_rows(wa, s), n_rows = min(s.n, a.in.max_new) * group;
+        const float* from = wa.w.old_sums + st.seq * wa.w.old_batch + g * wa.w.old_head;
+        float* to = wa.w.new_sums + st.seq * wa.w.new_batch + g * wa.w.new_head;
+        const float* scores = a.scores + (static_cast<int64_t>(st.seq) * kvh + g) * a.score_rows * a.score_keys;
+        const float* lse = a.lse + static_cast<int64_t>(s.first) * a.in.heads + g * group;
+        for (int k = st.step * kStoredKeys + static_cast<int>(threadIdx.x), i = 0; i < run; ++i, k += kStoredKeys) {
+            if (k >= held) continue;
+            const float old = k < s.ctx ? from[k] : 0.0f;
+            float sum = 0.0f;
+            if (k < s.total)
+#pragma unroll 8
+                for (int r = 0; r < n_rows; ++r)
+                    sum += __builtin_amdgcn_exp2f(__fmaf_rn(__builtin_nontemporal_load(scores + (static_cast<int64_t>(k >> 2) * a.score_rows + r) * 4 + (k & 3)), scale, -lse[r / group * a.in.heads + r % group]));
+            to[k] = old + sum;
+        }
+    }
+}
+
 // More rows.  A workgroup takes 64 keys, held in registers as an operand of 32x32x16, and its waves the rows in turns of 32: a lane
 // has one row (lane % 32) and 16 of every 32 keys, so that a row's logarithm is the lane's and the sums of its keys gather in
 // registers; they are added up over the lanes and the waves, in order, at the end.
@@ -337,14 +371,30 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void weigh_tile_kernel(
 
 struct WeighPlan {
     Plan attend;
-    size_t lse, bytes;  // where the logarithms begin
+    size_t lse, scores, bytes;  // where the logarithms and the scores begin
+    int score_rows, score_keys;  // 0: the keys are read again
 };
 
-WeighPlan weigh_plan(const View& v, const qmm_paged_query& in) {
+// The scores of few rows are kept where they cost less than the keys' second reading (16 sequences of up to 16384 keys, 8 rows a kv
+// head of 128 dimensions: the attention takes 143 us with the stores, 114 without; this pass 19 us, 71 with the keys), a byte
+// written for about two read, and do not take too much memory.
+constexpr int64_t kMostScores = int64_t{1} << 29;
+
+WeighPlan weigh_plan(const View& v, const qmm_paged_query& in, const qmm_paged_weights& w) {
     WeighPlan p{};
     p.attend = plan<Lse>(v, in);
     p.lse = (p.attend.bytes + 15) / 16 * 16;
-    p.bytes = p.lse + (static_cast<size_t>(in.tokens) * in.heads * sizeof(float) + 15) / 16 * 16;
+    p.bytes = p.scores = p.lse + (static_cast<size_t>(in.tokens) * in.heads * sizeof(float) + 15) / 16 * 16;
+    const int64_t rows = static_cast<int64_t>(std::min(in.max_new, in.tokens)) * (in.heads / v.c.kv_heads);
+    if (p.attend.kind == Kind::kRows && rows > 0 && rows <= 16 && 12 * rows <= static_cast<int64_t>(v.c.head_dim) * elem_bytes(v.c.dtype)) {
+        const int64_t keys = (std::min<int64_t>(w.rows, static_cast<int64_t>(v.c.table_width) * v.c.page_size) + 3) / 4 * 4;
+        const int64_t bytes = static_cast<int64_t>(v.c.batch) * v.c.kv_heads * rows * keys * 4;
+        if (keys < INT32_MAX - 64 && bytes <= kMostScores) {
+            p.score_rows = static_cast<int>(rows);
+            p.score_keys = static_cast<int>(keys);
+            p.bytes += bytes;
+        }
+    }
     return p;
 }
 
@@ -368,7 +418,8 @@ void with_weigh_kernel(int64_t rows, Fn f) {
 }
 
 template <class Fn>
-void with_weigh_kernel(const View& v, const qmm_paged_query& in, Fn f) {
+void with_weigh_kernel(const View& v, const qmm_paged_query& in, bool stored, Fn f) {
+    if (stored) return f(weigh_stored_kernel);
     const int64_t rows = static_cast<int64_t>(std::min(in.max_new, in.tokens)) * (in.heads / v.c.kv_heads);
     auto types = [&](auto tc, auto cc) {
         using T = decltype(tc);
@@ -393,7 +444,7 @@ int weighted_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, const 
     if (rc != QMM_OK) return rc;
     if (v.c.batch == 0) return QMM_OK;
     const bool attends = in->tokens > 0 && in->max_new > 0;
-    const WeighPlan p = weigh_plan(v, *in);
+    const WeighPlan p = weigh_plan(v, *in, *weights);
     std::unique_lock<std::mutex> held;  // until the last launch is enqueued
     if (workspace) {
         if (workspace_bytes < p.bytes || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
@@ -404,6 +455,11 @@ int weighted_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, const 
     }
     AttnArgs a = attention_args(v, *in, p.attend, workspace);
     a.lse = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.lse);
+    if (p.score_rows > 0) {
+        a.scores = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.scores);
+        a.score_rows = p.score_rows;
+        a.score_keys = p.score_keys;
+    }
     if (attends) {
         rc = launch_attention<Lse>(v, a, p.attend, stream);
         if (rc == QMM_OK && p.attend.merge) rc = launch_merge<Lse>(v, a, p.attend.kind != Kind::kLanes, p.attend.most_ranges, stream);
@@ -412,7 +468,7 @@ int weighted_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, const 
     WeighArgs wa{*weights, 1};
     if (weights->rows == 0) return QMM_OK;
     if (p.attend.kind != Kind::kLanes) {
-        with_weigh_kernel(v, *in, [&](auto kern) {
+        with_weigh_kernel(v, *in, a.scores != nullptr, [&](auto kern) {
             // workgroups that run at once, or one for each step that there can be
             const int64_t steps = static_cast<int64_t>(v.c.batch) * v.c.kv_heads * ((weights->rows + kTileKeysW - 1) / kTileKeysW);
             const int64_t blocks = std::min<int64_t>(kernel_slots(kern, 0), steps);
@@ -443,7 +499,7 @@ size_t qmm_paged_weighted_workspace(const qmm_paged_kv* kv, const qmm_paged_quer
         qmm::paged::View v;
         int rc = qmm::paged::check_query(kv, in, &v);
         if (rc == QMM_OK) rc = qmm::paged::check_weights(v, weights);
-        if (rc == QMM_OK && in->tokens > 0 && v.c.batch > 0) bytes = qmm::paged::weigh_plan(v, *in).bytes;
+        if (rc == QMM_OK && in->tokens > 0 && v.c.batch > 0) bytes = qmm::paged::weigh_plan(v, *in, *weights).bytes;
         return rc;
     });
     return bytes;
