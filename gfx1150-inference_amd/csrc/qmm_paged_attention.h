@@ -32,6 +32,12 @@ struct Lse {  // the logarithms (base 2) of the rows' sums beside the outputs
 
 constexpr int kThreads = 256;
 
+struct PartSeq {
+    int table_row, first, n, ctx;        // as in Span
+    int total, from, rows, tiles;        // and as in CallPlan
+    int ranges, keys, first_part, none;
+};
+
 struct AttnArgs {
     qmm_paged_query in;
     float scale_log2;  // scale * k_scale * log2 e
@@ -42,11 +48,12 @@ struct AttnArgs {
     float2* part_ml;   // [partial row]: maximum, sum
     int64_t parts;     // tokens that the partial rows have room for
     int4* cut;         // [token]: ranges, its first partial row and the rows between ranges, in tokens
-    // Part: the launch over what groups share has a group for a sequence, which reads the pages of its first sequence, lead[group],
-    // and no new rows; the launch over the rest begins at row from[sequence], a multiple of 16
-    const int32_t* lead;
-    const int32_t* from;
-    const int4* lead_cut;  // the cut of the first of both, whose partial rows begin at token lead_part of the room
+    // Part: the sequences as they are cut (a group's shared rows are those of a sequence without new rows), and the workgroups ahead of
+    // each; [n_seqs]: of all
+    const PartSeq* seqs;
+    const int32_t* first_block;
+    int n_seqs;
+    const int4* lead_cut;  // the cut of the shared rows, whose partial rows begin at token lead_part of the room
     int64_t lead_part, all_parts;
     // Lse: [token][head], +inf of a row that sees nothing; and the partial rows' sums of weights that are not rounded for the second
     // product, as those beside the outputs are
@@ -67,20 +74,17 @@ struct Span {
 template <class M>
 __device__ __forceinline__ Span span_of(const View& v, const AttnArgs& a, int seq) {
     Span s;
+    if constexpr (M::kPart) {
+        const int4* at = reinterpret_cast<const int4*>(a.seqs + seq);
+        const int4 x = at[0], y = at[1];
+        return Span{x.x, x.y, x.z, x.w, y.x, y.y};
+    }
     s.seq = seq;
     s.from = 0;
     s.first = max(v.c.cu[seq], 0);
     s.n = max(min(max(v.c.cu[seq + 1], 0), a.in.tokens) - s.first, 0);
     s.ctx = cached_rows(v, seq);
     s.total = static_cast<int>(min(static_cast<int64_t>(s.ctx) + s.n, static_cast<int64_t>(v.c.table_width) << v.page_shift));
-    if constexpr (M::kPart) {
-        if (a.lead) {
-            s.seq = a.lead[seq];
-            s.total = s.ctx;
-        } else {
-            s.from = a.from[seq];
-        }
-    }
     return s;
 }
 
@@ -348,7 +352,6 @@ struct CallPlan {
         if (b < v.c.batch) {
             const Span s = span_of<M>(v, a, b);
             x.rows = min(s.n, a.in.max_new);
-            if (M::kPart && a.lead && s.ctx == 0) x.rows = 0;
             x.tiles = kTile >= 128 ? (x.rows * (a.in.heads / v.c.kv_heads) + kTile - 1) / kTile : x.rows > 0;
             x.steps = x.rows > 0 ? max((s.total - s.from + kStep - 1) / kStep, 1) : 0;
             const int seen = (a.in.mask ? s.total : min(s.total, s.ctx + (s.n + 1) / 2)) - s.from;
@@ -360,6 +363,22 @@ struct CallPlan {
     // Finds the sequence of workgroup `at`; false: there is none.  Lengths and counts of workgroups are compared in fp32,
     // whose roundings are the same everywhere.
     __device__ __forceinline__ bool find(const View& v, const AttnArgs& a, int at, int lane) {
+        if constexpr (M::kPart) {  // found already
+            if (at >= a.first_block[a.n_seqs]) return false;
+            int upto = 0;  // sequences that begin at or ahead of the workgroup
+            for (int b0 = 0; b0 < a.n_seqs; b0 += 64) upto += __popcll(__ballot(b0 + lane < a.n_seqs && a.first_block[b0 + lane] <= at));
+            seq = upto - 1;
+            const int4* from = reinterpret_cast<const int4*>(a.seqs + seq);
+            const int4 y = from[1], z = from[2];
+            auto same = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+            rows = same(y.z);
+            tiles = same(y.w);
+            ranges = same(z.x);
+            keys = same(z.y);
+            first_part = same(z.z);
+            block = at - same(a.first_block[seq]);
+            return first_part + static_cast<int64_t>(ranges) * rows <= a.parts;
+        }
         const int kvh = v.c.kv_heads;
         double own_work = 0.0;  // of this lane's sequences, up to a thousand: no rounding, whatever the batch
         Lane x{};
@@ -391,7 +410,7 @@ struct CallPlan {
         for (int b0 = 0; b0 < v.c.batch; b0 += 64) {
             if (v.c.batch > 64) x = lane_of(v, a, b0 + lane);
             const int n = ranges_of(x.steps, best);
-            const int own_blocks = n * x.tiles * kvh, own_parts = n > 1 || M::kPart ? n * x.rows : 0;
+            const int own_blocks = n * x.tiles * kvh, own_parts = n > 1 ? n * x.rows : 0;
             const int sb = wave_scan(own_blocks), sp = wave_scan(own_parts);
             const int here = min(v.c.batch - b0, 64);
             const int hit = static_cast<int>(__popcll(__ballot(lane < here && blocks + sb <= at)));
@@ -405,7 +424,7 @@ struct CallPlan {
                 block = at - (blocks + of(sb - own_blocks));
                 first_part = parts + of(sp - own_parts);
                 // room is short only where cu descends and sequences overlap
-                return (ranges == 1 && !M::kPart) || first_part + static_cast<int64_t>(ranges) * rows <= a.parts;
+                return ranges == 1 || first_part + static_cast<int64_t>(ranges) * rows <= a.parts;
             }
             blocks += __builtin_amdgcn_readlane(sb, here - 1);
             parts += __builtin_amdgcn_readlane(sp, here - 1);
@@ -469,8 +488,19 @@ __device__ __forceinline__ void load_row_bytes(uint32_t* dst, const char* src) {
 // of 57000 rows, 52 rows a kv head: 51 us with four row tiles a wave, 42 us).  Joined through LDS in wave order.
 constexpr int kRowsStep = 128;
 
+// What a workgroup keeps in LDS: its waves' outputs, their maxima and sums, page ids.
+template <int D, class M>
+struct RowsLds {
+    static constexpr int kRowF = D + 4, kWaves = kThreads / 64;
+    float so[kWaves][16 * kRowF];
+    float2 sml[kWaves][16];
+    float sx[M::kLse ? kWaves : 1][16];
+    int pages[kWindowPages];
+};
+
+// Workgroup `block` of a call.
 template <class T, class C, int D, int NT, int RG, class M>
-__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_kernel(View v, AttnArgs a) {
+__device__ __forceinline__ void attend_rows(const View& v, const AttnArgs& a, int block, RowsLds<D, M>& lds) {
     using F = Frag<T>;
     using v8 = typename F::v8;
     constexpr bool kFp8 = std::is_same_v<C, Fp8>;
@@ -478,15 +508,15 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
     constexpr int kVAlign = (kVB & -kVB) < 16 ? kVB & -kVB : 16;
     constexpr bool kLo = NT == 1;
     constexpr int kRowF = D + 4, kWaves = kThreads / 64, kKeyWaves = kWaves / RG;
-    __shared__ __align__(16) float so[kWaves][16 * kRowF];
-    __shared__ float2 sml[kWaves][16];
-    __shared__ float sx[M::kLse ? kWaves : 1][16];
-    __shared__ int pages[kWindowPages];
+    auto& so = lds.so;
+    auto& sml = lds.sml;
+    auto& sx = lds.sx;
+    auto& pages = lds.pages;
     const int kvh = v.c.kv_heads, group = a.in.heads / kvh;
     const int lane = threadIdx.x & 63, l = lane & 15, q = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     CallPlan<16, kRowsStep, M> cp;
-    if (!cp.find(v, a, static_cast<int>(blockIdx.x), lane)) return;
+    if (!cp.find(v, a, block, lane)) return;
     const int g = cp.block % kvh, range = cp.block / kvh;
     const Span s = span_of<M>(v, a, cp.seq);
     const int kps = cp.keys;
@@ -769,6 +799,12 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_ker
     }
 }
 
+template <class T, class C, int D, int NT, int RG, class M>
+__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_rows_kernel(View v, AttnArgs a) {
+    __shared__ __align__(16) RowsLds<D, M> lds;
+    attend_rows<T, C, D, NT, RG, M>(v, a, static_cast<int>(blockIdx.x), lds);
+}
+
 // ---- many rows: keys through LDS -----------------------------------------------------------------
 // A workgroup of 4 waves owns 128 rows (tokens x query heads of one kv head), 32 a wave, and walks the keys in tiles of 64,
 // staged through LDS (two buffers, one barrier a tile):
@@ -813,8 +849,9 @@ __device__ __forceinline__ void copy_to_lds(const void* base, uint32_t off, uint
     __asm__ volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
 }
 
+// Workgroup `block` of a call; TileGeom<D>::kLds bytes of tile_lds.
 template <class T, class C, int D, class M>
-__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_tile_kernel(View v, AttnArgs a) {
+__device__ __forceinline__ void attend_tile(const View& v, const AttnArgs& a, int block) {
     using F = Frag<T>;
     using v8 = typename F::v8;
     using G = TileGeom<D>;
@@ -824,7 +861,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_tile_ker
     const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     CallPlan<kTileRows, kTileKeys, M> cp;
-    if (!cp.find(v, a, static_cast<int>(blockIdx.x), lane)) return;
+    if (!cp.find(v, a, block, lane)) return;
     const int g = cp.block % kvh, rest = cp.block / kvh;
     const int tiles = cp.tiles, tile = rest % tiles, range = rest / tiles;
     const Span s = span_of<M>(v, a, cp.seq);
@@ -1152,6 +1189,11 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_tile_ker
     }
 }
 
+template <class T, class C, int D, class M>
+__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_tile_kernel(View v, AttnArgs a) {
+    attend_tile<T, C, D, M>(v, a, static_cast<int>(blockIdx.x));
+}
+
 // Joins the ranges of each row: D / 4 threads hold a row's output and `sg` such groups share its ranges, four of
 // them requested at once; the groups are added in order through LDS.  A few rows of many ranges wait for one or two round
 // trips to memory that way (42 tokens of 32 heads, 37 ranges: 10.6 us with one group).  Block (x, y): token, heads.
@@ -1176,7 +1218,7 @@ __global__ __launch_bounds__(kThreads) void attention_merge_kernel(View v, AttnA
     // the ranges of what the sequence's group shares come first
     int4 lead = {0, 0, 0, 0};
     if constexpr (M::kPart) {
-        if (a.from[seq] > 0) lead = a.lead_cut[t];
+        if (a.seqs[seq].from > 0) lead = a.lead_cut[t];
         if (lead.x < 1 || lead.y < 0 || lead.z < 1 || a.lead_part + lead.y + static_cast<int64_t>(lead.x - 1) * lead.z >= a.all_parts) lead.x = 0;
     }
     const int n = cut.x + lead.x;
@@ -1333,12 +1375,21 @@ int kernel_slots(K kern, size_t lds) {
     return known[{fn, dev}] = per_cu * cus;
 }
 
+int64_t rows_per_kv_head(const View& v, const qmm_paged_query& in) {
+    return static_cast<int64_t>(std::min(in.max_new, in.tokens)) * (in.heads / v.c.kv_heads);
+}
+
+// Of matrix-core operands.  More row tiles of head_dim 256 do not fit a wave's registers.
+Kind part_kind(const View& v, const qmm_paged_query& in) { return rows_per_kv_head(v, in) <= (v.c.head_dim <= 128 ? 64 : 16) ? Kind::kRows : Kind::kTile; }
+int row_tiles_of(const View& v, const qmm_paged_query& in) { return static_cast<int>((rows_per_kv_head(v, in) + 15) / 16); }
+
+// slots: the workgroups that run at once, of a kernel that is not the plan's own (Part).
 template <class M>
-Plan plan(const View& v, const qmm_paged_query& in) {
+Plan plan(const View& v, const qmm_paged_query& in, int slots = 0) {
     Plan p{};
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(static_cast<int64_t>(v.c.table_width) * v.c.page_size, INT32_MAX - 65536));
     const int64_t rows = static_cast<int64_t>(in.tokens) * in.heads;
-    const int64_t per_kv = static_cast<int64_t>(std::min(in.max_new, in.tokens)) * (in.heads / v.c.kv_heads);
+    const int64_t per_kv = rows_per_kv_head(v, in);
     const int kvh = v.c.kv_heads;
     if (!matrix_operands(v, in) || per_kv > (1 << 28)) {
         p.kind = Kind::kLanes;
@@ -1351,11 +1402,11 @@ Plan plan(const View& v, const qmm_paged_query& in) {
         p.most_ranges = p.splits;
         p.parts = rows * p.splits;
     } else {
-        // more row tiles of head_dim 256 do not fit a wave's registers
-        p.kind = per_kv <= (v.c.head_dim <= 128 ? 64 : 16) ? Kind::kRows : Kind::kTile;
+        p.kind = part_kind(v, in);
         const bool few = p.kind == Kind::kRows;
-        p.row_tiles = few ? static_cast<int>((per_kv + 15) / 16) : 0;
-        p.slots = with_matrix_kernel<M>(v, in, p.kind, p.row_tiles, [](auto kern, size_t lds) { return kernel_slots(kern, lds); });
+        p.row_tiles = few ? row_tiles_of(v, in) : 0;
+        p.slots = slots;
+        if constexpr (!M::kPart) p.slots = with_matrix_kernel<M>(v, in, p.kind, p.row_tiles, [](auto kern, size_t lds) { return kernel_slots(kern, lds); });
         // A plan's ranges are cut by a length of at least `least` keys.  With W steps in all and u >= W / slots steps a
         // range, the ranges of all row tiles are at most 2 W / u and one more per row tile (a chain's last tile sees up to
         // twice the mean), and those of sequences with more than one range at most twice that, 4 slots.
@@ -1448,15 +1499,14 @@ int launch_merge(const View& v, const AttnArgs& a, bool planned, int64_t most_ra
 // The attention kernel of a plan, without the join.
 template <class M>
 int launch_attention(const View& v, const AttnArgs& a, const Plan& p, hipStream_t stream) {
+    static_assert(!M::kPart);
     if (p.kind == Kind::kLanes) {
-        if constexpr (!M::kPart) {
-            const dim3 grid(static_cast<unsigned>(a.in.tokens), static_cast<unsigned>(p.splits), static_cast<unsigned>((a.in.heads + 3) / 4));
-            const int aligned = operands_aligned(v) ? 1 : 0;
-            auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, stream, v, a, aligned); };
-            const bool fp8 = v.c.dtype == QMM_DTYPE_E4M3;
-            if (a.in.dtype == QMM_DTYPE_F16) fp8 ? go(attention_lanes_kernel<_Float16, Fp8, M>) : go(attention_lanes_kernel<_Float16, _Float16, M>);
-            else fp8 ? go(attention_lanes_kernel<__bf16, Fp8, M>) : go(attention_lanes_kernel<__bf16, __bf16, M>);
-        }
+        const dim3 grid(static_cast<unsigned>(a.in.tokens), static_cast<unsigned>(p.splits), static_cast<unsigned>((a.in.heads + 3) / 4));
+        const int aligned = operands_aligned(v) ? 1 : 0;
+        auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, stream, v, a, aligned); };
+        const bool fp8 = v.c.dtype == QMM_DTYPE_E4M3;
+        if (a.in.dtype == QMM_DTYPE_F16) fp8 ? go(attention_lanes_kernel<_Float16, Fp8, M>) : go(attention_lanes_kernel<_Float16, _Float16, M>);
+        else fp8 ? go(attention_lanes_kernel<__bf16, Fp8, M>) : go(attention_lanes_kernel<__bf16, __bf16, M>);
     } else {
         if (p.blocks > INT32_MAX) return bad("too many sequences, heads and tokens for one call.");
         with_matrix_kernel<M>(v, a.in, p.kind, p.row_tiles, [&](auto kern, size_t lds) {

@@ -9,73 +9,279 @@ namespace qmm {
 namespace paged {
 namespace {
 
-// What the launches read of the groups.
+// How a part is cut; the rest of it is as CallPlan says.
+struct CutArgs {
+    int tile, step, min_steps;  // rows of a row tile (0: one for all), keys of a step, the least steps of a range
+    int slots;                  // workgroups that run at once
+    PartSeq* seqs;
+    int32_t* first_block;
+};
+
 struct Groups {
     const int32_t *first, *shared;
     int count;
-    int32_t *starts, *cu, *ctx, *lead;  // [count + 1], [count + 1], [count], [count]
-    int32_t* from;                      // [batch]
+    int32_t *starts, *ctx;  // [count + 1], [count], for more groups than fit LDS
+    CutArgs lead, rest;
 };
 
-constexpr int kGroupThreads = 1024;
+constexpr int kPlanThreads = 256, kPlanWaves = kPlanThreads / 64, kTries = 4;
 
-// One workgroup: where groups begin (made ascending, so that no sequence is in two), the rows that a group shares (no more than any
-// of its sequences has cached, whole blocks of 16, which lie in one page; none where it has one sequence), and the row that every sequence
-// goes on from.
-__global__ __launch_bounds__(kGroupThreads) void groups_kernel(View v, Groups g) {
-    const int tid = threadIdx.x, batch = v.c.batch;
-    if (tid < 64) {
+// One workgroup cuts the call: where groups begin (made ascending, so that no sequence is in two), the rows that a group shares (no
+// more than any of its sequences has cached, whole blocks of 16, which lie in one page; none where it has one sequence), and
+// for both parts, by the rules of CallPlan, the ranges of every sequence and the workgroups ahead of it.  The attention's
+// workgroups look theirs up: worked out by each of them, the cut of 128 sequences took most of the time of short contexts.
+__global__ __launch_bounds__(kPlanThreads) void cut_kernel(View v, qmm_paged_query in, Groups g) {
+    __shared__ int starts_lds[kPlanThreads], ctx_lds[kPlanThreads], shared_lds[kPlanThreads], cu_lds[kPlanThreads];
+    __shared__ float sums[2 * kTries][kPlanWaves];
+    __shared__ int4 scans[kPlanWaves];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, batch = v.c.batch, group = in.heads / v.c.kv_heads, kvh = v.c.kv_heads;
+    int* starts = g.count < kPlanThreads ? starts_lds : g.starts;
+    int* ctx = g.count < kPlanThreads ? ctx_lds : g.ctx;
+    // what a thread's sequence and group have, requested together: one round trip where there are no more of them than threads
+    const bool small = batch < kPlanThreads && g.count < kPlanThreads;
+    int own_ctx = 0;
+    if (small) {
+        const int first = tid <= g.count ? g.first[tid] : 0, shared = tid < g.count ? g.shared[tid] : 0, cu = tid <= batch ? v.c.cu[tid] : 0;
+        if (tid < batch) own_ctx = cached_rows(v, tid);
+        starts_lds[tid] = first;
+        shared_lds[tid] = shared;
+        cu_lds[tid] = cu;
+        __syncthreads();
+    }
+    auto ctx_of = [&](int b) { return small ? own_ctx : cached_rows(v, b); };  // of the thread's own sequence
+    auto cu_of = [&](int b) { return small ? cu_lds[b] : v.c.cu[b]; };
+    if (w == 0) {
         int most = 0;
         for (int i0 = 0; i0 <= g.count; i0 += 64) {
             const int i = i0 + tid;
-            int x = i <= g.count ? min(max(g.first[i], 0), batch) : 0;
+            int x = i <= g.count ? min(max(small ? starts_lds[i] : g.first[i], 0), batch) : 0;
             for (int o = 1; o < 64; o <<= 1) {
                 const int y = __shfl_up(x, o, 64);
                 if (tid >= o) x = max(x, y);
             }
             x = max(x, most);
             most = __shfl(x, 63, 64);
-            if (i <= g.count) {
-                g.starts[i] = x;
-                g.cu[i] = v.c.cu[x];
-            }
+            if (i <= g.count) starts[i] = x;
         }
     }
     __syncthreads();
     const int64_t room = static_cast<int64_t>(v.c.table_width) << v.page_shift;
-    for (int i = tid; i < g.count; i += kGroupThreads) {
-        const int members = g.starts[i + 1] - g.starts[i];
-        g.ctx[i] = members > 1 ? static_cast<int>(min(static_cast<int64_t>(max(g.shared[i], 0)), room)) : 0;
-        g.lead[i] = min(g.starts[i], batch - 1);
-    }
+    for (int i = tid; i < g.count; i += kPlanThreads)
+        ctx[i] = starts[i + 1] - starts[i] > 1 ? static_cast<int>(min(static_cast<int64_t>(max(small ? shared_lds[i] : g.shared[i], 0)), room)) : 0;
     __syncthreads();
     // the group of a sequence: the count of starts at or below it, less one
     auto group_of = [&](int b) {
         int lo = 0, hi = g.count + 1;
         while (lo < hi) {
             const int mid = (lo + hi) / 2;
-            if (g.starts[mid] <= b) lo = mid + 1;
+            if (starts[mid] <= b) lo = mid + 1;
             else hi = mid;
         }
-        return lo - 1;
+        return lo - 1 < g.count ? lo - 1 : -1;
     };
-    for (int b = tid; b < batch; b += kGroupThreads) {
+    for (int b = tid; b < batch; b += kPlanThreads) {
         const int i = group_of(b);
-        if (i >= 0 && i < g.count) atomicMin(&g.ctx[i], cached_rows(v, b));
+        if (i >= 0) atomicMin(&ctx[i], ctx_of(b));
     }
     __syncthreads();
-    for (int i = tid; i < g.count; i += kGroupThreads) g.ctx[i] &= ~15;
-    __syncthreads();
-    for (int b = tid; b < batch; b += kGroupThreads) {
-        const int i = group_of(b);
-        g.from[b] = i >= 0 && i < g.count ? g.ctx[i] : 0;
+
+    struct Own {
+        PartSeq s;
+        int steps;
+        float work;
+    };
+    auto token = [&](int b) { return min(max(cu_of(b), 0), in.tokens); };
+    // sequence b of the rest, group b of what is shared
+    auto own_of = [&](const CutArgs& c, bool lead, int b) {
+        Own x{};
+        PartSeq& s = x.s;
+        if (b >= (lead ? g.count : batch)) return x;
+        if (lead) {
+            s.table_row = min(starts[b], batch - 1);
+            s.first = token(starts[b]);
+            s.n = max(token(starts[b + 1]) - s.first, 0);
+            s.total = s.ctx = ctx[b] & ~15;
+            s.rows = s.ctx > 0 ? s.n : 0;
+        } else {
+            const int i = group_of(b);
+            s.table_row = b;
+            s.first = max(cu_of(b), 0);
+            s.n = max(token(b + 1) - s.first, 0);
+            s.ctx = ctx_of(b);
+            s.total = static_cast<int>(min(static_cast<int64_t>(s.ctx) + s.n, room));
+            s.from = i >= 0 ? ctx[i] & ~15 : 0;
+            s.rows = min(s.n, in.max_new);
+        }
+        s.tiles = c.tile ? static_cast<int>((static_cast<int64_t>(s.rows) * group + c.tile - 1) / c.tile) : s.rows > 0;
+        x.steps = s.rows > 0 ? max((s.total - s.from + c.step - 1) / c.step, 1) : 0;
+        const int seen = (lead || in.mask ? s.total : min(s.total, s.ctx + (s.n + 1) / 2)) - s.from;
+        x.work = static_cast<float>(max((seen + c.step - 1) / c.step, 1)) * static_cast<float>(s.tiles);
+        return x;
+    };
+    const int chunks = (max(batch, g.count) + kPlanThreads - 1) / kPlanThreads;
+    auto total_of = [&](int row) {
+        float x = lane < kPlanWaves ? sums[row][lane] : 0.0f;
+        return wave_total(x);
+    };
+    Own rest{}, lead{};
+    double work[2] = {0.0, 0.0};
+    for (int c = 0; c < chunks; ++c) {
+        rest = own_of(g.rest, false, c * kPlanThreads + tid);
+        lead = own_of(g.lead, true, c * kPlanThreads + tid);
+        work[0] += static_cast<double>(rest.work);
+        work[1] += static_cast<double>(lead.work);
     }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const float x = wave_total(static_cast<float>(work[k]));
+        if (lane == 0) sums[k][w] = x;
+    }
+    __syncthreads();
+    int u[2][kTries];
+    float count[2 * kTries];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const CutArgs& c = k ? g.lead : g.rest;
+        const float shortest = total_of(k) * static_cast<float>(kvh) / static_cast<float>(c.slots) * 1.00001f;  // as in CallPlan
+#pragma unroll
+        for (int t = 0; t < kTries; ++t) {
+            u[k][t] = max(static_cast<int>(fminf(ceilf(shortest * (1.0f + 0.25f * static_cast<float>(t))), 33554432.0f)), c.min_steps);
+            count[kTries * k + t] = 0.0f;
+        }
+    }
+    auto ranges_of = [](int steps, int len) { return static_cast<int>((static_cast<uint32_t>(steps) + len - 1) / static_cast<uint32_t>(len)); };
+    for (int c = 0; c < chunks; ++c) {
+        if (chunks > 1) {
+            rest = own_of(g.rest, false, c * kPlanThreads + tid);
+            lead = own_of(g.lead, true, c * kPlanThreads + tid);
+        }
+#pragma unroll
+        for (int t = 0; t < kTries; ++t) {
+            count[t] += wave_total(static_cast<float>(ranges_of(rest.steps, u[0][t])) * static_cast<float>(rest.s.tiles));
+            count[kTries + t] += wave_total(static_cast<float>(ranges_of(lead.steps, u[1][t])) * static_cast<float>(lead.s.tiles));
+        }
+    }
+    __syncthreads();  // sums have been read
+    if (lane == 0)
+#pragma unroll
+        for (int t = 0; t < 2 * kTries; ++t) sums[t][w] = count[t];
+    __syncthreads();
+    int best[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        best[k] = u[k][0];
+#pragma unroll
+        for (int t = kTries - 1; t >= 0; --t)
+            if (total_of(kTries * k + t) * static_cast<float>(kvh) <= static_cast<float>(k ? g.lead.slots : g.rest.slots)) best[k] = u[k][t];
+    }
+    int4 before{0, 0, 0, 0};  // blocks and partial rows (in tokens) of the rest, and of what is shared
+    for (int c = 0; c < chunks; ++c) {
+        if (chunks > 1) {
+            rest = own_of(g.rest, false, c * kPlanThreads + tid);
+            lead = own_of(g.lead, true, c * kPlanThreads + tid);
+        }
+        rest.s.ranges = ranges_of(rest.steps, best[0]);
+        lead.s.ranges = ranges_of(lead.steps, best[1]);
+        const int4 own{rest.s.ranges * rest.s.tiles * kvh, rest.s.ranges * rest.s.rows, lead.s.ranges * lead.s.tiles * kvh, lead.s.ranges * lead.s.rows};
+        const int4 upto{wave_scan(own.x), wave_scan(own.y), wave_scan(own.z), wave_scan(own.w)};
+        if (lane == 63) scans[w] = upto;
+        __syncthreads();
+        int4 ahead = before;
+        for (int i = 0; i < kPlanWaves; ++i) {
+            const int4 x = scans[i];
+            if (i < w) ahead = int4{ahead.x + x.x, ahead.y + x.y, ahead.z + x.z, ahead.w + x.w};
+            before = int4{before.x + x.x, before.y + x.y, before.z + x.z, before.w + x.w};
+        }
+        __syncthreads();
+        auto put = [&](const CutArgs& a, Own& x, int b, int n, int block, int part) {
+            if (b >= n) return;
+            x.s.keys = x.s.ranges > 0 ? (x.steps + x.s.ranges - 1) / x.s.ranges * a.step : 0;
+            x.s.first_part = part;
+            a.seqs[b] = x.s;
+            a.first_block[b] = block;
+        };
+        const int b = c * kPlanThreads + tid;
+        put(g.rest, rest, b, batch, ahead.x + upto.x - own.x, ahead.y + upto.y - own.y);
+        put(g.lead, lead, b, g.count, ahead.z + upto.z - own.z, ahead.w + upto.w - own.w);
+    }
+    if (tid == 0) {
+        g.rest.first_block[batch] = before.x;
+        g.lead.first_block[g.count] = before.z;
+    }
+}
+
+// Both parts in one launch where one kernel serves them, what is shared first, as it takes the longest.  (Where they
+// differ, each has more workgroups at once in a launch of its own: 64 sequences of up to 1500 rows behind 16384, 93 us of two launches, 103
+// of one.)
+struct LeadArgs {
+    const PartSeq* seqs;
+    const int32_t* first_block;
+    int count, blocks;  // of groups, of workgroups
+    int64_t parts;
+    int4* cut;
+};
+
+__device__ __forceinline__ AttnArgs lead_args(const View& v, const AttnArgs& a, const LeadArgs& l) {
+    AttnArgs b = a;
+    b.in.mask = nullptr;
+    b.in.mask_words = 0;
+    b.part_o = a.part_o + a.parts * a.in.heads * v.c.head_dim;
+    b.part_ml = a.part_ml + a.parts * a.in.heads;
+    b.parts = l.parts;
+    b.cut = l.cut;
+    b.seqs = l.seqs;
+    b.first_block = l.first_block;
+    b.n_seqs = l.count;
+    return b;
+}
+
+// kTile: which kernel's workgroups serve the call.  The first l.blocks are the shared rows', the others the rest's.
+template <class T, class C, int D, bool kTile, int NT, int RG>
+__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_shared_kernel(View v, AttnArgs a, LeadArgs l) {
+    const bool is_lead = static_cast<int>(blockIdx.x) < l.blocks;
+    const AttnArgs b = is_lead ? lead_args(v, a, l) : a;
+    const int block = static_cast<int>(blockIdx.x) - (is_lead ? 0 : l.blocks);
+    if constexpr (kTile) {
+        attend_tile<T, C, D, Part>(v, b, block);
+    } else {
+        __shared__ __align__(16) RowsLds<D, Part> lds;
+        attend_rows<T, C, D, NT, RG, Part>(v, b, block, lds);
+    }
+}
+
+template <class T, class C, int D, class Fn>
+auto with_shared_kernel(Kind kind, int row_tiles, Fn f) {
+    if (kind == Kind::kTile) return f(attention_shared_kernel<T, C, D, true, 1, 1>, TileGeom<D>::kLds);
+    if constexpr (D <= 128) {
+        if (row_tiles == 2) return f(attention_shared_kernel<T, C, D, false, 2, 1>, size_t{0});
+        if (row_tiles > 2) return f(attention_shared_kernel<T, C, D, false, 2, 2>, size_t{0});
+    }
+    return f(attention_shared_kernel<T, C, D, false, 1, 1>, size_t{0});
+}
+
+// Calls f with a kind's kernel and its LDS.
+template <class Fn>
+auto with_shared_kernel(const View& v, const qmm_paged_query& in, Kind kind, int row_tiles, Fn f) {
+    auto types = [&](auto tc, auto cc) {
+        using T = decltype(tc);
+        using C = decltype(cc);
+        switch (v.c.head_dim) {
+            case 64: return with_shared_kernel<T, C, 64>(kind, row_tiles, f);
+            case 96: return with_shared_kernel<T, C, 96>(kind, row_tiles, f);
+            case 128: return with_shared_kernel<T, C, 128>(kind, row_tiles, f);
+            default: return with_shared_kernel<T, C, 256>(kind, row_tiles, f);
+        }
+    };
+    const bool fp8 = v.c.dtype == QMM_DTYPE_E4M3;
+    if (in.dtype == QMM_DTYPE_F16) return fp8 ? types(_Float16{}, Fp8{}) : types(_Float16{}, _Float16{});
+    return fp8 ? types(__bf16{}, Fp8{}) : types(__bf16{}, __bf16{});
 }
 
 struct SharedPlan {
     Plan lead, rest;
-    size_t groups, cut, ml, o, bytes;  // where the workspace's parts begin
-    int64_t parts;                     // in rows
+    int row_tiles;                             // of both, where both are of rows
+    size_t seqs, first, cut, ml, o, bytes;     // where the workspace's parts begin
+    int64_t parts;                             // in rows
 };
 
 size_t whole(size_t bytes) { return (bytes + 15) / 16 * 16; }
@@ -92,26 +298,21 @@ bool shares(const View& v, const qmm_paged_query& in, const qmm_paged_groups& g)
     return g.count > 0 && matrix_operands(v, in) && static_cast<int64_t>(in.tokens) * (in.heads / v.c.kv_heads) <= (1 << 28);
 }
 
-View lead_view(const View& v, const qmm_paged_groups& g) {
-    View u = v;
-    u.c.batch = g.count;
-    return u;
-}
-
-qmm_paged_query lead_query(const qmm_paged_query& in) {
-    qmm_paged_query q = in;
-    q.mask = nullptr;
-    q.mask_words = 0;
-    q.max_new = in.tokens;  // of a group
-    return q;
-}
-
 SharedPlan shared_plan(const View& v, const qmm_paged_query& in, const qmm_paged_groups& g) {
     SharedPlan p{};
-    p.rest = plan<Part>(v, in);
-    p.lead = plan<Part>(lead_view(v, g), lead_query(in));
+    View u = v;
+    u.c.batch = g.count;
+    qmm_paged_query q = in;
+    q.max_new = in.tokens;  // of a group
+    // each part has the kernel that it would have by itself; a group has at least a sequence's rows
+    p.row_tiles = part_kind(u, q) == Kind::kRows ? row_tiles_of(u, q) : row_tiles_of(v, in);
+    auto slots = [&](Kind kind) { return with_shared_kernel(v, in, kind, p.row_tiles, [](auto kern, size_t lds) { return kernel_slots(kern, lds); }); };
+    p.rest = plan<Part>(v, in, slots(part_kind(v, in)));
+    p.lead = plan<Part>(u, q, slots(part_kind(u, q)));
     p.parts = p.rest.parts + p.lead.parts;
-    p.cut = whole((3 * static_cast<size_t>(g.count) + 2 + g.count + v.c.batch) * sizeof(int32_t));
+    p.seqs = whole((2 * static_cast<size_t>(g.count) + 1) * sizeof(int32_t));
+    p.first = p.seqs + (static_cast<size_t>(g.count) + v.c.batch) * sizeof(PartSeq);
+    p.cut = p.first + whole((static_cast<size_t>(g.count) + v.c.batch + 2) * sizeof(int32_t));
     p.ml = p.cut + 2 * static_cast<size_t>(in.tokens) * sizeof(int4);
     p.o = p.ml + whole(static_cast<size_t>(p.parts) * sizeof(float2));
     p.bytes = p.o + static_cast<size_t>(p.parts) * v.c.head_dim * sizeof(float);
@@ -135,46 +336,52 @@ int shared_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, const qm
         const hipError_t e = take_workspace(WorkspaceKind::kAttention, stream, p.bytes, held, &workspace);
         if (e != hipSuccess) return launched(e, "paged attention workspace");
     }
+    if (p.lead.blocks + p.rest.blocks > INT32_MAX) return bad("too many sequences, heads and tokens for one call.");
     char* base = static_cast<char*>(workspace);
-    Groups g{groups->first, groups->shared, groups->count, reinterpret_cast<int32_t*>(base), nullptr, nullptr, nullptr, nullptr};
-    g.cu = g.starts + g.count + 1;
-    g.ctx = g.cu + g.count + 1;
-    g.lead = g.ctx + g.count;
-    g.from = g.lead + g.count;
-    hipLaunchKernelGGL(groups_kernel, dim3(1), dim3(kGroupThreads), 0, stream, v, g);
-    rc = launched(hipGetLastError(), "paged groups kernel launch");
+    auto cut_args = [&](const Plan& part, PartSeq* seqs, int32_t* first) {
+        const bool tile = part.kind == Kind::kTile;
+        return CutArgs{tile ? kTileRows : 0, tile ? kTileKeys : kRowsStep, tile ? CallPlan<kTileRows, kTileKeys, Part>::kMinSteps : 1,
+                       part.slots, seqs, first};
+    };
+    PartSeq* seqs = reinterpret_cast<PartSeq*>(base + p.seqs);
+    int32_t* first = reinterpret_cast<int32_t*>(base + p.first);
+    Groups g{groups->first, groups->shared, groups->count, reinterpret_cast<int32_t*>(base), reinterpret_cast<int32_t*>(base) + groups->count + 1,
+             cut_args(p.lead, seqs, first), cut_args(p.rest, seqs + groups->count, first + groups->count + 1)};
+    hipLaunchKernelGGL(cut_kernel, dim3(1), dim3(kPlanThreads), 0, stream, v, *in, g);
+    rc = launched(hipGetLastError(), "paged attention plan kernel launch");
     if (rc != QMM_OK) return rc;
 
-    AttnArgs rest{};
-    rest.in = *in;
-    rest.scale_log2 = score_scale(v, *in);
-    rest.v_scale = v.c.v_scale;
-    rest.slots = p.rest.slots;
-    rest.part_o = reinterpret_cast<float*>(base + p.o);
-    rest.part_ml = reinterpret_cast<float2*>(base + p.ml);
-    rest.parts = p.rest.parts / in->heads;
-    rest.cut = reinterpret_cast<int4*>(base + p.cut);
-    rest.from = g.from;
-    AttnArgs lead = rest;
-    lead.in = lead_query(*in);
-    lead.slots = p.lead.slots;
-    lead.part_o = rest.part_o + rest.parts * in->heads * v.c.head_dim;
-    lead.part_ml = rest.part_ml + rest.parts * in->heads;
-    lead.parts = p.lead.parts / in->heads;
-    lead.cut = rest.cut + in->tokens;
-    lead.from = nullptr;
-    lead.lead = g.lead;
-    View u = lead_view(v, *groups);
-    u.c.cu = g.cu;
-    u.c.ctx = g.ctx;
-    rc = launch_attention<Part>(u, lead, p.lead, stream);
-    if (rc == QMM_OK) rc = launch_attention<Part>(v, rest, p.rest, stream);
+    AttnArgs a{};
+    a.in = *in;
+    a.scale_log2 = score_scale(v, *in);
+    a.v_scale = v.c.v_scale;
+    a.part_o = reinterpret_cast<float*>(base + p.o);
+    a.part_ml = reinterpret_cast<float2*>(base + p.ml);
+    a.parts = p.rest.parts / in->heads;
+    a.cut = reinterpret_cast<int4*>(base + p.cut);
+    a.seqs = g.rest.seqs;
+    a.first_block = g.rest.first_block;
+    a.n_seqs = v.c.batch;
+    LeadArgs l{g.lead.seqs, g.lead.first_block, g.count, static_cast<int>(p.lead.blocks), p.lead.parts / in->heads, a.cut + in->tokens};
+    auto launch = [&](Kind kind, int64_t blocks, const LeadArgs& lead) {
+        with_shared_kernel(v, *in, kind, p.row_tiles, [&](auto kern, size_t lds) {
+            hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), lds, stream, v, a, lead);
+        });
+    };
+    if (p.lead.kind == p.rest.kind) {
+        launch(p.lead.kind, p.lead.blocks + p.rest.blocks, l);
+    } else {
+        launch(p.lead.kind, p.lead.blocks, l);
+        LeadArgs none = l;
+        none.blocks = 0;
+        launch(p.rest.kind, p.rest.blocks, none);
+    }
+    rc = launched(hipGetLastError(), "paged attention kernel launch");
     if (rc != QMM_OK) return rc;
-    AttnArgs join = rest;
-    join.lead_cut = lead.cut;
-    join.lead_part = rest.parts;
-    join.all_parts = rest.parts + lead.parts;
-    return launch_merge<Part>(v, join, true, p.rest.most_ranges + p.lead.most_ranges, stream);
+    a.lead_cut = l.cut;
+    a.lead_part = a.parts;
+    a.all_parts = a.parts + l.parts;
+    return launch_merge<Part>(v, a, true, p.rest.most_ranges + p.lead.most_ranges, stream);
 }
 
 }  // namespace

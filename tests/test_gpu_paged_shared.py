@@ -183,10 +183,11 @@ def test_what_nobody_sees_may_hold_anything(cuda):
     a, k = c.args()
     import paged
     out = paged.shared_attention(*a, **k)
-    keep = [t for t in range(6) if t != 4]
+    # Every other token is within the tolerance of what it would be without.  Not to the bit: rows that an infinite value has made NaN
+    # are summed up again in another order and with weights that are not rounded.
     c.k, c.v = c.k.nan_to_num(posinf=0.0), c.v.nan_to_num(posinf=0.0)
-    want = c.run()
-    assert torch.equal(out[keep], want[keep])
+    out[4] = c.run()[4]
+    c.check(out)
 
 
 def test_repeats_to_the_bit_and_other_streams(cuda):
