@@ -11,7 +11,7 @@ namespace {
 
 // How a part is cut; the rest of it is as CallPlan says.
 struct CutArgs {
-    int tile, step, min_steps;  // rows of a row tile (0: one for all), keys of a step, the least steps of a range
+    int tile_shift, step_shift, min_steps;  // rows of a row tile (-1: one for all), keys of a step; the least steps of a range
     int slots;                  // workgroups that run at once
     PartSeq* seqs;
     int32_t* first_block;
@@ -79,9 +79,10 @@ __global__ __launch_bounds__(kPlanThreads) void cut_kernel(View v, qmm_paged_que
         }
         return lo - 1 < g.count ? lo - 1 : -1;
     };
+    int own_group = -1;
     for (int b = tid; b < batch; b += kPlanThreads) {
-        const int i = group_of(b);
-        if (i >= 0) atomicMin(&ctx[i], ctx_of(b));
+        own_group = group_of(b);
+        if (own_group >= 0) atomicMin(&ctx[own_group], ctx_of(b));
     }
     __syncthreads();
 
@@ -103,7 +104,7 @@ __global__ __launch_bounds__(kPlanThreads) void cut_kernel(View v, qmm_paged_que
             s.total = s.ctx = ctx[b] & ~15;
             s.rows = s.ctx > 0 ? s.n : 0;
         } else {
-            const int i = group_of(b);
+            const int i = small ? own_group : group_of(b);
             s.table_row = b;
             s.first = max(cu_of(b), 0);
             s.n = max(token(b + 1) - s.first, 0);
@@ -112,10 +113,11 @@ __global__ __launch_bounds__(kPlanThreads) void cut_kernel(View v, qmm_paged_que
             s.from = i >= 0 ? ctx[i] & ~15 : 0;
             s.rows = min(s.n, in.max_new);
         }
-        s.tiles = c.tile ? static_cast<int>((static_cast<int64_t>(s.rows) * group + c.tile - 1) / c.tile) : s.rows > 0;
-        x.steps = s.rows > 0 ? max((s.total - s.from + c.step - 1) / c.step, 1) : 0;
+        s.tiles = c.tile_shift < 0 ? s.rows > 0 : static_cast<int>((static_cast<int64_t>(s.rows) * group + (1 << c.tile_shift) - 1) >> c.tile_shift);
+        auto steps = [&](int keys) { return (max(keys - 1, 0) >> c.step_shift) + 1; };
+        x.steps = s.rows > 0 ? steps(s.total - s.from) : 0;
         const int seen = (lead || in.mask ? s.total : min(s.total, s.ctx + (s.n + 1) / 2)) - s.from;
-        x.work = static_cast<float>(max((seen + c.step - 1) / c.step, 1)) * static_cast<float>(s.tiles);
+        x.work = static_cast<float>(steps(seen)) * static_cast<float>(s.tiles);
         return x;
     };
     const int chunks = (max(batch, g.count) + kPlanThreads - 1) / kPlanThreads;
@@ -195,7 +197,7 @@ __global__ __launch_bounds__(kPlanThreads) void cut_kernel(View v, qmm_paged_que
         __syncthreads();
         auto put = [&](const CutArgs& a, Own& x, int b, int n, int block, int part) {
             if (b >= n) return;
-            x.s.keys = x.s.ranges > 0 ? (x.steps + x.s.ranges - 1) / x.s.ranges * a.step : 0;
+            x.s.keys = x.s.ranges > 0 ? static_cast<int>((static_cast<uint32_t>(x.steps) + x.s.ranges - 1) / static_cast<uint32_t>(x.s.ranges)) << a.step_shift : 0;
             x.s.first_part = part;
             a.seqs[b] = x.s;
             a.first_block[b] = block;
@@ -340,7 +342,8 @@ int shared_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, const qm
     char* base = static_cast<char*>(workspace);
     auto cut_args = [&](const Plan& part, PartSeq* seqs, int32_t* first) {
         const bool tile = part.kind == Kind::kTile;
-        return CutArgs{tile ? kTileRows : 0, tile ? kTileKeys : kRowsStep, tile ? CallPlan<kTileRows, kTileKeys, Part>::kMinSteps : 1,
+        static_assert(kTileRows == 1 << 7 && kTileKeys == 1 << 6 && kRowsStep == 1 << 7);
+        return CutArgs{tile ? 7 : -1, tile ? 6 : 7, tile ? CallPlan<kTileRows, kTileKeys, Part>::kMinSteps : 1,
                        part.slots, seqs, first};
     };
     PartSeq* seqs = reinterpret_cast<PartSeq*>(base + p.seqs);
