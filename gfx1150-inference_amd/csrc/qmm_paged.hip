@@ -324,6 +324,9 @@ __global__ __launch_bounds__(kThreads) void append_normed_kernel(View v, AppendA
         n = decode(u);
         request(n);
     }
+    // the angles' and the norms' operands too, ahead of the chain to the token's row
+    const uint64_t turn = tid < half ? fr.turn[tid] : 0;
+    int pos = tid < half && a.in.positions ? a.in.positions[nm.axis[tid] * nm.axis_stride + t] : 0;
     for (int d = tid; d < D; d += kThreads) {
         weights[0][d] = nm.qw ? norm_weight<T>(nm, nm.qw, d) : 1.0f;
         weights[1][d] = nm.kw ? norm_weight<T>(nm, nm.kw, d) : 1.0f;
@@ -332,7 +335,8 @@ __global__ __launch_bounds__(kThreads) void append_normed_kernel(View v, AppendA
     if (seq >= v.c.batch || t < v.c.cu[seq]) return;  // a token of no sequence (the same in every wave)
     const int row = row_behind(cached_rows(v, seq), t - max(v.c.cu[seq], 0));
     const int page = page_of(v, seq, row), slot = row & (v.c.page_size - 1);
-    if (tid < half) cs[tid] = cos_sin(fr.turn[tid], a.in.positions ? a.in.positions[nm.axis[tid] * nm.axis_stride + t] : row);
+    if (!a.in.positions) pos = row;
+    if (tid < half) cs[tid] = cos_sin(turn, pos);
     __syncthreads();
     const int64_t k_at = page * v.c.k_page + slot * v.c.k_slot, v_at = page * v.c.v_page + slot * v.c.v_slot;
     const float mean = 1.0f / static_cast<float>(D);

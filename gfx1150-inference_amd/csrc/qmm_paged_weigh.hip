@@ -318,15 +318,30 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void weigh_tile_kernel(
         const bool cached = kb + kTileKeysW <= s.ctx && have == 15;
         // a chain's rows ahead of the first key see none of them
         const int first = a.in.mask == nullptr ? max(kb - s.ctx, 0) * group / 32 : 0;
+        v8 next[D / 16];  // the next rows are on the way while these are multiplied
+        float next_lse = 0.0f;
+        int next_i = 0;
+        auto request = [&](int r0) {
+            const int r = max(min(r0 + l32, n_rows - 1), 0), head = g * group + r % group;
+            next_i = r / group;
+            const T* qrow = static_cast<const T*>(a.in.q) + static_cast<int64_t>(s.first + next_i) * a.in.q_token + head * a.in.q_head + 8 * h;
+#pragma unroll
+            for (int db = 0; db < D / 16; ++db) __builtin_memcpy(&next[db], __builtin_assume_aligned(qrow + 16 * db, 16), 16);
+            next_lse = a.lse[static_cast<int64_t>(s.first + next_i) * a.in.heads + head];
+        };
+        const int begin = 32 * (first + ((w - first) & 3));
+        if (begin < n_rows) request(begin);
 #pragma unroll 1
-        for (int r0 = 32 * (first + ((w - first) & 3)); r0 < n_rows; r0 += 128) {
-            const int r = min(r0 + l32, n_rows - 1), i = r / group, head = g * group + r % group;
-            const T* qrow = static_cast<const T*>(a.in.q) + static_cast<int64_t>(s.first + i) * a.in.q_token + head * a.in.q_head + 8 * h;
+        for (int r0 = begin; r0 < n_rows; r0 += 128) {
             v8 qf[D / 16];
 #pragma unroll
-            for (int db = 0; db < D / 16; ++db) __builtin_memcpy(&qf[db], __builtin_assume_aligned(qrow + 16 * db, 16), 16);
-            const float lse = a.lse[static_cast<int64_t>(s.first + i) * a.in.heads + head];
+            for (int db = 0; db < D / 16; ++db) qf[db] = next[db];
+            const float lse = next_lse;
+            const int i = next_i;
             const bool counts = r0 + l32 < n_rows;
+            if (D <= 128) {
+                if (r0 + 128 < n_rows) request(r0 + 128);
+            }
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
                 f32x16 x;
@@ -347,6 +362,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void weigh_tile_kernel(
                     sum[hh][e] += (vis >> (8 * (e >> 2) + (e & 3))) & 1 ? p : 0.0f;
                 }
             }
+            if (D > 128 && r0 + 128 < n_rows) request(r0 + 128);  // no registers for both
         }
         // register e of half hh is key 32 hh + 8 (e / 4) + 4 h + e % 4
 #pragma unroll
