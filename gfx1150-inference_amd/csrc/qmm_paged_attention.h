@@ -1198,11 +1198,11 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_tile_ker
 // them requested at once; the groups are added in order through LDS.  A few rows of many ranges wait for one or two round
 // trips to memory that way (42 tokens of 32 heads, 37 ranges: 10.6 us with one group).  Block (x, y): token, heads.
 template <class T, bool kPlanned, class M>
-__global__ __launch_bounds__(kThreads) void attention_merge_kernel(View v, AttnArgs a, int sg) {
+__device__ __forceinline__ void join_ranges(const View& v, const AttnArgs& a, int sg, int t, int part) {
     __shared__ f32x4 so[kThreads];
     __shared__ float2 sml[kThreads];
     __shared__ float sx[M::kLse ? kThreads : 1];
-    const int t = blockIdx.x, D = v.c.head_dim, per = D / 4, rows = kThreads / per / sg, lane = threadIdx.x & 63;
+    const int D = v.c.head_dim, per = D / 4, rows = kThreads / per / sg, lane = threadIdx.x & 63;
     int4 cut = {0, 0, 0, 0};
     if constexpr (kPlanned) cut = a.cut[t];  // not written for a token of no sequence, or past max_new
     const int seq = sequence_of(v, t, lane);
@@ -1225,7 +1225,7 @@ __global__ __launch_bounds__(kThreads) void attention_merge_kernel(View v, AttnA
     int64_t row = static_cast<int64_t>(cut.y) * a.in.heads, lead_row = (a.lead_part + lead.y) * a.in.heads;
     const int64_t step = static_cast<int64_t>(cut.z) * a.in.heads, lead_step = static_cast<int64_t>(lead.z) * a.in.heads;  // between ranges
     auto row_of = [&](int c) { return M::kPart && c < lead.x ? lead_row + c * lead_step : row + (c - lead.x) * step; };
-    const int slot = threadIdx.x / per, d0 = 4 * (threadIdx.x % per), gi = slot % sg, head = blockIdx.y * rows + slot / sg;
+    const int slot = threadIdx.x / per, d0 = 4 * (threadIdx.x % per), gi = slot % sg, head = part * rows + slot / sg;
     const bool live = slot < rows * sg && head < a.in.heads;
     row += live ? head : 0;
     lead_row += live ? head : 0;
@@ -1291,6 +1291,11 @@ __global__ __launch_bounds__(kThreads) void attention_merge_kernel(View v, AttnA
     else
 #pragma unroll
         for (int i = 0; i < 4; ++i) out[i] = h[i];
+}
+
+template <class T, bool kPlanned, class M>
+__global__ __launch_bounds__(kThreads) void attention_merge_kernel(View v, AttnArgs a, int sg) {
+    join_ranges<T, kPlanned, M>(v, a, sg, static_cast<int>(blockIdx.x), static_cast<int>(blockIdx.y));
 }
 
 // ---- host side -------------------------------------------------------------------------------
@@ -1474,14 +1479,24 @@ AttnArgs attention_args(const View& v, const qmm_paged_query& in, const Plan& p,
     return a;
 }
 
-// Joins the ranges; planned: of the kernels with a plan.
-template <class M>
-int launch_merge(const View& v, const AttnArgs& a, bool planned, int64_t most_ranges, hipStream_t stream) {
+// Thread groups that share a row's ranges in the join, and the workgroups for a token's heads.
+struct JoinShape {
+    int sg, per_token;
+};
+JoinShape join_shape(const View& v, const AttnArgs& a, int64_t most_ranges) {
     const int groups = kThreads / (v.c.head_dim / 4);
     int sg = 1;
     while (2 * sg <= groups && 4 * sg < most_ranges && static_cast<int64_t>(a.in.tokens) * a.in.heads * sg < 8192) sg *= 2;
     const int rows = groups / sg;
-    const dim3 grid(static_cast<unsigned>(a.in.tokens), static_cast<unsigned>((a.in.heads + rows - 1) / rows));
+    return {sg, (a.in.heads + rows - 1) / rows};
+}
+
+// Joins the ranges; planned: of the kernels with a plan.
+template <class M>
+int launch_merge(const View& v, const AttnArgs& a, bool planned, int64_t most_ranges, hipStream_t stream) {
+    const JoinShape shape = join_shape(v, a, most_ranges);
+    const int sg = shape.sg;
+    const dim3 grid(static_cast<unsigned>(a.in.tokens), static_cast<unsigned>(shape.per_token));
     auto merge = [&](auto tc) {
         using T = decltype(tc);
         auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, stream, v, a, sg); };
