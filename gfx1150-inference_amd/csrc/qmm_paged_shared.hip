@@ -86,6 +86,8 @@ __global__ __launch_bounds__(kPlanThreads) void cut_kernel(View v, qmm_paged_que
     }
     __syncthreads();
 
+    // rows that group i shares; past the caches, which may hold what an entry was before the minima
+    auto shared_of = [&](int i) { return __hip_atomic_load(&ctx[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) & ~15; };
     struct Own {
         PartSeq s;
         int steps;
@@ -101,7 +103,7 @@ __global__ __launch_bounds__(kPlanThreads) void cut_kernel(View v, qmm_paged_que
             s.table_row = min(starts[b], batch - 1);
             s.first = token(starts[b]);
             s.n = max(token(starts[b + 1]) - s.first, 0);
-            s.total = s.ctx = ctx[b] & ~15;
+            s.total = s.ctx = shared_of(b);
             s.rows = s.ctx > 0 ? s.n : 0;
         } else {
             const int i = small ? own_group : group_of(b);
@@ -110,7 +112,7 @@ __global__ __launch_bounds__(kPlanThreads) void cut_kernel(View v, qmm_paged_que
             s.n = max(token(b + 1) - s.first, 0);
             s.ctx = ctx_of(b);
             s.total = static_cast<int>(min(static_cast<int64_t>(s.ctx) + s.n, room));
-            s.from = i >= 0 ? ctx[i] & ~15 : 0;
+            s.from = i >= 0 ? shared_of(i) : 0;
             s.rows = min(s.n, in.max_new);
         }
         s.tiles = c.tile_shift < 0 ? s.rows > 0 : static_cast<int>((static_cast<int64_t>(s.rows) * group + (1 << c.tile_shift) - 1) >> c.tile_shift);

@@ -110,6 +110,15 @@ def test_sizes_of_groups(cuda, members):
     Case(members, 8, 2, 64, 16, [members, 2], [161, 40], [rng.randrange(40) for _ in range(members + 2)], [1] * (members + 2)).check()
 
 
+@pytest.mark.parametrize("groups", [1, 60, 299])
+def test_more_sequences_than_the_plan_has_threads(cuda, groups):
+    rng = random.Random(groups)
+    sizes = [600 // groups // 2 if groups < 299 else 2] * groups
+    n = sum(sizes)
+    Case(groups, 4, 2, 64, 16, sizes, [rng.randrange(16, 80) for _ in sizes], [rng.randrange(20) for _ in range(n)],
+         [1 if i % 7 else 0 for i in range(n)]).check()
+
+
 def test_chunks_of_prompts(cuda):
     """A chain of many new tokens: tiles of 128 rows over the shared rows and over the rest."""
     Case(3, 8, 2, 128, 16, [3], [333], [20, 0, 150], [130, 64, 40], BF16).check()

@@ -101,6 +101,14 @@ def test_sums_refusals(bad):
     assert L.qmm_paged_weighted_workspace(_kv(), _query(), _weights(**bad)) == 0
 
 
+@pytest.mark.parametrize("strides", [dict(new_batch=0), dict(new_head=0), dict(new_head=63), dict(new_batch=100), dict(new_batch=-128)], ids=lambda b: str(b))
+def test_sums_that_overlap_are_refused(strides):
+    """Sums of several heads or sequences in one place, as of an expanded tensor; as an input they are fine."""
+    _refused(L.qmm_paged_weighted_attention(_kv(), _query(), _weights(old_sums=2 * P, **strides), None, 0, None), "overlap")
+    assert L.qmm_paged_weighted_workspace(_kv(), _query(), _weights(old_sums=2 * P, old_batch=0, old_head=0)) > 0
+    assert L.qmm_paged_weighted_workspace(_kv(), _query(), _weights(old_sums=2 * P, new_batch=64, new_head=128)) > 0
+
+
 @pytest.mark.parametrize("bad", [dict(dtype=qmm.DTYPE_E4M3), dict(heads=3), dict(q=None), dict(scale=float("nan"))], ids=lambda b: str(b))
 def test_query_refusals(bad):
     _refused(L.qmm_paged_shared_attention(_kv(), _query(**bad), _groups(), None, 0, None))
