@@ -34,7 +34,8 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 // time, by counts of the weights at or above the three numbers that the bits so far begin; where a count is m, those are
 // the rows.  Then the kept rows are listed in order, of those equal to the m-th largest the first ones.  Weights of up to
 // kHeld 1024 rows wait in registers (a count is a comparison and a scalar population count for each 64 of them, with no atomics to
-// meet on); of longer sequences (kHeld 0) they are read for each count.
+// meet on); of longer sequences (kHeld 0) they are read for each count.  Bound by the chain of counts: 256 workgroups of 3000 rows 13 us;
+// 768 of up to 8192, of which two thirds choose, 43.
 template <int kHeld>
 __global__ __launch_bounds__(kSelectThreads, kHeld <= 16 ? 8 : 4) void select_kernel(View v, EvictArgs a) {
     __shared__ int counts[2][4][kSelectWaves];  // [turn][number][wave]
@@ -176,7 +177,8 @@ __global__ __launch_bounds__(kSelectThreads, kHeld <= 16 ? 8 : 4) void select_ke
 }
 
 // Copies the kept rows.  Block (x, y, z): a run of rows, sequence and kv head, layer; a thread keeps its piece of a row and takes every
-// (kThreads / per_row)-th row, kRowsAtOnce of K and of V at once.
+// (kThreads / per_row)-th row, kRowsAtOnce of K and of V at once.  At the rate of a copy: 1.45 GB read and written in 289 us, 5.0 TB/s (297 where the rows stay in the
+// caches).
 constexpr int kRowsAtOnce = 4;
 
 template <int B>

@@ -104,7 +104,7 @@ struct Steps {
 
 // Up to 16 NT rows (tokens x query heads of one kv head): decoding, small trees.  As in the attention over them a wave takes 32 keys
 // at a time, straight into registers, and lane (l, q) = (lane % 16, lane / 16) receives the scores of row l with keys 4q ..
-// 4q + 3 of each 16; their weights are added up over the 16 lanes.
+// 4q + 3 of each 16; their weights are added up over the 16 lanes.  Bound by reading K: 308 MB in 71 us, 4.3 TB/s.
 constexpr int kRowsKeys = 128;
 
 template <class T, class C, int D, int NT>
@@ -300,7 +300,8 @@ __global__ __launch_bounds__(kThreads) void weigh_stored_kernel(View v, AttnArgs
 
 // More rows.  A workgroup takes 64 keys, held in registers as an operand of 32x32x16, and its waves the rows in turns of 32: a lane
 // has one row (lane % 32) and 16 of every 32 keys, so that a row's logarithm is the lane's and the sums of its keys gather in
-// registers; they are added up over the lanes and the waves, in order, at the end.
+// registers; they are added up over the lanes and the waves, in order, at the end.  Two chunks of up to 600 tokens, 32 heads of 128 over
+// up to 2100 keys (14 GFLOP): 50 us, bound by the waits of two waves a SIMD (matrix cores busy for 14 % of the cycles, vector ALUs 33 %).
 constexpr int kTileKeysW = 64;
 
 template <class T, class C, int D>
