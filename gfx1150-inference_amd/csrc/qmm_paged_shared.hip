@@ -216,9 +216,9 @@ __global__ __launch_bounds__(kPlanThreads) void cut_kernel(View v, qmm_paged_que
     }
 }
 
-// Both parts in one launch where one kernel serves them, what is shared first, as it takes the longest.  (Where they
-// differ, each has more workgroups at once in a launch of its own: 64 sequences of up to 1500 rows behind 16384, 93 us of two launches, 103
-// of one.)
+// Both parts in one launch, what is shared first, as it takes the longest.  Where tiles of 128 rows serve it and few rows each the
+// others, these have fewer workgroups at once in it than in a launch of their own, so large calls of that kind have two
+// (kOneLaunch).
 struct LeadArgs {
     const PartSeq* seqs;
     const int32_t* first_block;
@@ -241,41 +241,49 @@ __device__ __forceinline__ AttnArgs lead_args(const View& v, const AttnArgs& a, 
     return b;
 }
 
-// kTile: which kernel's workgroups serve the call.  The first l.blocks are the shared rows', the others the rest's.
-template <class T, class C, int D, bool kTile, int NT, int RG>
+// kLeadTile, kRestTile: which kernel's workgroups serve the parts.  The first l.blocks are the shared rows', the others the rest's.
+template <class T, class C, int D, bool kLeadTile, bool kRestTile, int NT, int RG>
 __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_shared_kernel(View v, AttnArgs a, LeadArgs l) {
     const bool is_lead = static_cast<int>(blockIdx.x) < l.blocks;
     const AttnArgs b = is_lead ? lead_args(v, a, l) : a;
     const int block = static_cast<int>(blockIdx.x) - (is_lead ? 0 : l.blocks);
-    if constexpr (kTile) {
+    auto& rows_lds = *reinterpret_cast<RowsLds<D, Part>*>(tile_lds);
+    if constexpr (kLeadTile && kRestTile) {
         attend_tile<T, C, D, Part>(v, b, block);
+    } else if constexpr (!kLeadTile) {
+        attend_rows<T, C, D, NT, RG, Part>(v, b, block, rows_lds);
     } else {
-        __shared__ __align__(16) RowsLds<D, Part> lds;
-        attend_rows<T, C, D, NT, RG, Part>(v, b, block, lds);
+        if (is_lead) attend_tile<T, C, D, Part>(v, b, block);
+        else attend_rows<T, C, D, NT, RG, Part>(v, b, block, rows_lds);
     }
 }
 
 template <class T, class C, int D, class Fn>
-auto with_shared_kernel(Kind kind, int row_tiles, Fn f) {
-    if (kind == Kind::kTile) return f(attention_shared_kernel<T, C, D, true, 1, 1>, TileGeom<D>::kLds);
-    if constexpr (D <= 128) {
-        if (row_tiles == 2) return f(attention_shared_kernel<T, C, D, false, 2, 1>, size_t{0});
-        if (row_tiles > 2) return f(attention_shared_kernel<T, C, D, false, 2, 2>, size_t{0});
-    }
-    return f(attention_shared_kernel<T, C, D, false, 1, 1>, size_t{0});
+auto with_shared_kernel(Kind lead, Kind rest, int row_tiles, Fn f) {
+    constexpr size_t rows = sizeof(RowsLds<D, Part>), tile = TileGeom<D>::kLds, both = rows > tile ? rows : tile;
+    if (rest == Kind::kTile) return f(attention_shared_kernel<T, C, D, true, true, 1, 1>, tile);
+    auto few = [&](auto lead_tile, size_t lds) {
+        constexpr bool L = decltype(lead_tile)::value;
+        if constexpr (D <= 128) {
+            if (row_tiles == 2) return f(attention_shared_kernel<T, C, D, L, false, 2, 1>, lds);
+            if (row_tiles > 2) return f(attention_shared_kernel<T, C, D, L, false, 2, 2>, lds);
+        }
+        return f(attention_shared_kernel<T, C, D, L, false, 1, 1>, lds);
+    };
+    return lead == Kind::kTile ? few(std::true_type{}, both) : few(std::false_type{}, rows);
 }
 
-// Calls f with a kind's kernel and its LDS.
+// Calls f with the kernel of both parts' kinds and its LDS.
 template <class Fn>
-auto with_shared_kernel(const View& v, const qmm_paged_query& in, Kind kind, int row_tiles, Fn f) {
+auto with_shared_kernel(const View& v, const qmm_paged_query& in, Kind lead, Kind rest, int row_tiles, Fn f) {
     auto types = [&](auto tc, auto cc) {
         using T = decltype(tc);
         using C = decltype(cc);
         switch (v.c.head_dim) {
-            case 64: return with_shared_kernel<T, C, 64>(kind, row_tiles, f);
-            case 96: return with_shared_kernel<T, C, 96>(kind, row_tiles, f);
-            case 128: return with_shared_kernel<T, C, 128>(kind, row_tiles, f);
-            default: return with_shared_kernel<T, C, 256>(kind, row_tiles, f);
+            case 64: return with_shared_kernel<T, C, 64>(lead, rest, row_tiles, f);
+            case 96: return with_shared_kernel<T, C, 96>(lead, rest, row_tiles, f);
+            case 128: return with_shared_kernel<T, C, 128>(lead, rest, row_tiles, f);
+            default: return with_shared_kernel<T, C, 256>(lead, rest, row_tiles, f);
         }
     };
     const bool fp8 = v.c.dtype == QMM_DTYPE_E4M3;
@@ -283,8 +291,14 @@ auto with_shared_kernel(const View& v, const qmm_paged_query& in, Kind kind, int
     return fp8 ? types(__bf16{}, Fp8{}) : types(__bf16{}, __bf16{});
 }
 
+// Products of queries and keys, by the table's width, up to which parts of different kinds go in one launch (16 x 8 beams behind
+// 1000 rows of 32 heads, 4e6: 46 us with two launches, 42 with one; 45 sequences behind 585 rows of 16 heads, 6e5: 34 and 26; the
+// attention alone of 64 sequences of 64 heads behind 16384, 7e7: 93 and 103).
+constexpr int64_t kOneLaunch = int64_t{3} << 23;
+
 struct SharedPlan {
     Plan lead, rest;
+    bool one;                                  // launch
     int row_tiles;                             // of both, where both are of rows
     size_t seqs, first, cut, ml, o, bytes;     // where the workspace's parts begin
     int64_t parts;                             // in rows
@@ -312,9 +326,11 @@ SharedPlan shared_plan(const View& v, const qmm_paged_query& in, const qmm_paged
     q.max_new = in.tokens;  // of a group
     // each part has the kernel that it would have by itself; a group has at least a sequence's rows
     p.row_tiles = part_kind(u, q) == Kind::kRows ? row_tiles_of(u, q) : row_tiles_of(v, in);
-    auto slots = [&](Kind kind) { return with_shared_kernel(v, in, kind, p.row_tiles, [](auto kern, size_t lds) { return kernel_slots(kern, lds); }); };
-    p.rest = plan<Part>(v, in, slots(part_kind(v, in)));
-    p.lead = plan<Part>(u, q, slots(part_kind(u, q)));
+    const Kind lead = part_kind(u, q), rest = part_kind(v, in);
+    p.one = lead == rest || static_cast<int64_t>(in.tokens) * in.heads * v.c.table_width <= kOneLaunch / v.c.page_size;
+    auto slots = [&](Kind l, Kind r) { return with_shared_kernel(v, in, l, r, p.row_tiles, [](auto kern, size_t lds) { return kernel_slots(kern, lds); }); };
+    p.rest = plan<Part>(v, in, p.one ? slots(lead, rest) : slots(rest, rest));
+    p.lead = plan<Part>(u, q, p.one ? slots(lead, rest) : slots(lead, lead));
     p.parts = p.rest.parts + p.lead.parts;
     p.seqs = whole((2 * static_cast<size_t>(g.count) + 1) * sizeof(int32_t));
     p.first = p.seqs + (static_cast<size_t>(g.count) + v.c.batch) * sizeof(PartSeq);
@@ -370,18 +386,18 @@ int shared_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, const qm
     a.first_block = g.rest.first_block;
     a.n_seqs = v.c.batch;
     LeadArgs l{g.lead.seqs, g.lead.first_block, g.count, static_cast<int>(p.lead.blocks), p.lead.parts / in->heads, a.cut + in->tokens};
-    auto launch = [&](Kind kind, int64_t blocks, const LeadArgs& lead) {
-        with_shared_kernel(v, *in, kind, p.row_tiles, [&](auto kern, size_t lds) {
-            hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), lds, stream, v, a, lead);
+    auto launch = [&](Kind lead, Kind rest, int64_t blocks, const LeadArgs& args) {
+        with_shared_kernel(v, *in, lead, rest, p.row_tiles, [&](auto kern, size_t lds) {
+            hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), lds, stream, v, a, args);
         });
     };
-    if (p.lead.kind == p.rest.kind) {
-        launch(p.lead.kind, p.lead.blocks + p.rest.blocks, l);
+    if (p.one) {
+        launch(p.lead.kind, p.rest.kind, p.lead.blocks + p.rest.blocks, l);
     } else {
-        launch(p.lead.kind, p.lead.blocks, l);
+        launch(p.lead.kind, p.lead.kind, p.lead.blocks, l);
         LeadArgs none = l;
         none.blocks = 0;
-        launch(p.rest.kind, p.rest.blocks, none);
+        launch(p.rest.kind, p.rest.kind, p.rest.blocks, none);
     }
     rc = launched(hipGetLastError(), "paged attention kernel launch");
     if (rc != QMM_OK) return rc;
