@@ -50,8 +50,10 @@ def append(k, v, k_cache, v_cache, table, cu, ctx, q=None, q_out=None, positions
     ``rotary_dim / 2`` ints, pair i turns by ``positions[axes[i], token]`` of ``positions`` ``[axes, tokens]``: time, height and
     width of an image's or a video's tokens, in runs of pairs or in turn (a text's token has the same position on
     all)."""
-    return _on(stream, _ops.append, k, v, k_cache, v_cache, table, cu, ctx, q, q_out, positions, freq_base, rotary_dim, neox, k_scale,
-               v_scale, q_norm, k_norm, norm_eps, axes)
+    args = (k, v, k_cache, v_cache, table, cu, ctx, q, q_out, positions, freq_base, rotary_dim, neox, k_scale, v_scale)
+    if q_norm is None and k_norm is None and axes is None:
+        return _on(stream, _ops.append, *args)
+    return _on(stream, _ops.append_normed, *args, q_norm, k_norm, norm_eps, axes)
 
 
 def tree_attention(q, k_cache, v_cache, table, cu, ctx, mask=None, max_new=None, scale=None, k_scale: float = 1.0,

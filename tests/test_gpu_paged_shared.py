@@ -138,6 +138,19 @@ def test_long_prefix(cuda):
     Case(7, 16, 2, 128, 16, [6], [9000], [2500, 0, 1, 700, 64, 8], [1, 1, 2, 1, 3, 1]).check()
 
 
+@pytest.mark.parametrize("dtype,cache,D", [(F16, F16, 128), (BF16, E4, 64), (F16, F16, 256)])
+def test_wide_tables(cuda, dtype, cache, D):
+    """By the table's width the call may be a large one: each part has a launch of its own where their kernels differ."""
+    import paged
+    c = Case(20, 16, 2, D, 16, [9, 4], [700, 90], [50, 0, 1, 70, 64, 8, 3, 16, 31, 2, 0, 40, 5], [1] * 13, dtype, cache)
+    a, k = c.args()
+    wide = torch.full((13, 12000), -1, dtype=torch.int32, device="cuda")
+    wide[:, :a[3].shape[1]] = a[3]
+    assert 13 * 16 * 12000 * 16 > 3 << 23
+    c.check(paged.shared_attention(*a[:3], wide, *a[4:], **k))
+    c.check()
+
+
 def test_sequences_outside_groups_and_empty_groups(cuda):
     import paged
     c = Case(8, 8, 2, 64, 16, [2, 3, 2], [100, 50, 200], [4, 0, 7, 9, 60, 33, 2], [1, 2, 1, 1, 3, 1, 1])
