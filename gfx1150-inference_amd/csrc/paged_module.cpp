@@ -207,7 +207,7 @@ OptTensor append_normed(const Tensor& k, const Tensor& v, const Tensor& k_cache,
     return q_out;
 }
 
-// Without the last four: pybind takes 0.1 us an argument, of the 5 that a decoding step's call takes.
+// Without norms and axes, whose arguments such a call need not pass.
 OptTensor append(const Tensor& k, const Tensor& v, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& cu,
                  const Tensor& ctx, const OptTensor& q, const OptTensor& q_out, const OptTensor& positions, double freq_base,
                  std::optional<int64_t> rotary_dim, bool neox, double k_scale, double v_scale) {
