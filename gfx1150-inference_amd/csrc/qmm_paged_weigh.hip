@@ -197,18 +197,25 @@ __global__ __launch_bounds__(kThreads) void weigh_rows_kernel(View v, AttnArgs a
                         kf[tt][f] = __builtin_bit_cast(v8, kr[tt][f]);
                     }
                 }
+            // what every row sees, ahead of the first product: round a branch between a product and its use the compiler has
+            // left out the wait for the result (tests/test_matrix_waits.py)
+            uint32_t vis[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) vis[nt] = 0xFFFFFFFFu;
+            if (!full)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    vis[nt] = visible32(a, s, tok[nt], kb);
+                    if (!ok[0]) vis[nt] &= 0xFFFF0000u;
+                    if (!ok[1]) vis[nt] &= 0x0000FFFFu;
+                }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) vis[nt] = counts[nt] ? vis[nt] >> (4 * q) : 0;
             float sum[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[e] = 0.0f;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                uint32_t vis = 0xFFFFFFFFu;
-                if (!full) {
-                    vis = visible32(a, s, tok[nt], kb);
-                    if (!ok[0]) vis &= 0xFFFF0000u;
-                    if (!ok[1]) vis &= 0x0000FFFFu;
-                }
-                vis = counts[nt] ? vis >> (4 * q) : 0;
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int tt = 0; tt < 2; ++tt) {
                     f32x4 sc = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -217,10 +224,9 @@ __global__ __launch_bounds__(kThreads) void weigh_rows_kernel(View v, AttnArgs a
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float p = __builtin_amdgcn_exp2f(__fmaf_rn(sc[e], a.scale_log2, -lse[nt]));
-                        sum[4 * tt + e] += (vis >> (16 * tt + e)) & 1 ? p : 0.0f;
+                        sum[4 * tt + e] += (vis[nt] >> (16 * tt + e)) & 1 ? p : 0.0f;
                     }
                 }
-            }
             float mine = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
