@@ -297,8 +297,12 @@ __global__ __launch_bounds__(kThreads) void weigh_stored_kernel(View v, AttnArgs
             float sum = 0.0f;
             if (k < s.total)
 #pragma unroll 8
-                for (int r = 0; r < n_rows; ++r)
-                    sum += __builtin_amdgcn_exp2f(__fmaf_rn(__builtin_nontemporal_load(scores + (static_cast<int64_t>(k >> 2) * a.score_rows + r) * 4 + (k & 3)), scale, -lse[r]));
+                for (int r = 0; r < n_rows; ++r) {
+                    // of a key that the row does not see nothing, also where the row's logarithm is NaN
+                    const float x = __builtin_nontemporal_load(scores + (static_cast<int64_t>(k >> 2) * a.score_rows + r) * 4 + (k & 3));
+                    const float p = __builtin_amdgcn_exp2f(__fmaf_rn(x, scale, -lse[r]));
+                    sum += x == -INFINITY ? 0.0f : p;
+                }
             to[k] = old + sum;
         }
     }
