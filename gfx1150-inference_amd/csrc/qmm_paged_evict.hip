@@ -36,10 +36,14 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 // kHeld 1024 rows wait in registers (a count is a comparison and a scalar population count for each 64 of them, with no atomics to
 // meet on); of longer sequences (kHeld 0) they are read for each count.  Bound by the chain of counts: 256 workgroups of 3000 rows 13 us;
 // 768 of up to 8192, of which two thirds choose, 43.
+// A row without a page is no row: nothing of it could be copied, and its place in a fresh page would show what the page held before.
+// Where fewer rows than `keep` have pages the sequence ends with them; past them only places without a fresh page, which show
+// nothing either, count for rows without one.
 template <int kHeld>
 __global__ __launch_bounds__(kSelectThreads, kHeld <= 16 ? 8 : 4) void select_kernel(View v, EvictArgs a) {
     __shared__ int counts[2][4][kSelectWaves];  // [turn][number][wave]
     __shared__ int2 scan[kHeld ? kHeld : 1][kSelectWaves];
+    __shared__ int none[2];  // rows without a page: of the first and last ones, of those in between
     const int g = blockIdx.x, b = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int keep = a.e.keep;
@@ -53,26 +57,59 @@ __global__ __launch_bounds__(kSelectThreads, kHeld <= 16 ? 8 : 4) void select_ke
         }
     const int n = table_rows(v, b);
     float* out = a.e.weights_out + layer * a.e.wo_layer + b * a.e.wo_batch + g * a.e.wo_head;
-    if (g == 0 && layer == 0) {
-        const int pages = (keep + v.c.page_size - 1) >> v.page_shift;
+    const int32_t* fresh = a.e.fresh + b * a.e.fresh_stride;
+    auto put_table = [&](int length) {
+        if (g != 0 || layer != 0) return;
+        const int pages = (length + v.c.page_size - 1) >> v.page_shift;
         for (int p = tid; p < v.c.table_width; p += kSelectThreads)
-            a.e.table_out[static_cast<int64_t>(b) * v.c.table_width + p] = n <= keep ? v.c.table[b * v.c.table_stride + p]
-                                                                           : p < pages ? a.e.fresh[b * a.e.fresh_stride + p] : -1;
-        if (tid == 0) a.e.lens_out[b] = min(n, keep);
-    }
+            a.e.table_out[static_cast<int64_t>(b) * v.c.table_width + p] = n <= keep ? v.c.table[b * v.c.table_stride + p] : p < pages ? fresh[p] : -1;
+        if (tid == 0) a.e.lens_out[b] = length;
+    };
     if (n <= keep) {
+        put_table(n);
         for (int j = tid; j < a.e.rows; j += kSelectThreads) out[j] = j < n ? weights[j] : 0.0f;
         return;
     }
-    const int first = a.e.sinks, last = n - a.e.recent, need = keep - a.e.sinks - a.e.recent;
-    // of a row in between, at least ordered(-inf); 0 of the others, which no count meets
+    const int first = a.e.sinks, last = n - a.e.recent, pages = ((n - 1) >> v.page_shift) + 1;
+    bool misses = false;
+    for (int p = tid; p < pages; p += kSelectThreads) misses |= page_of(v, b, p << v.page_shift) < 0;
+    if (tid < 2) none[tid] = 0;
+    const bool gap = __syncthreads_or(misses);
+    int need = keep - a.e.sinks - a.e.recent, kept = keep, length = keep;  // rows to choose, rows that stay, the new length
+    if (gap) {
+        for (int p = tid; p < pages; p += kSelectThreads) {
+            if (page_of(v, b, p << v.page_shift) >= 0) continue;
+            const int from = p << v.page_shift, to = min(from + v.c.page_size, n), inner = max(min(to, last) - max(from, first), 0);
+            atomicAdd(&none[0], to - from - inner);
+            atomicAdd(&none[1], inner);
+        }
+        __syncthreads();
+        const int ends = a.e.sinks + a.e.recent - none[0];
+        need = min(keep - ends, last - first - none[1]);
+        kept = ends + need;
+        for (int p = kept >> v.page_shift; kept < keep && p <= (keep - 1) >> v.page_shift; ++p) {
+            if (static_cast<uint32_t>(fresh[p]) >= static_cast<uint32_t>(v.c.num_pages)) continue;
+            length = max(kept, p << v.page_shift);
+            break;
+        }
+    }
+    put_table(length);
+    // Of a row in between its weight's, at least ordered(-inf).  Of the others, which no count meets, kAway where there is no page and
+    // the row does not stay in any case, else 0.
+    constexpr uint32_t kAway = 1;
     auto between = [&](int j) { return j >= first && j < last; };
-    auto rank = [&](int j) { return between(j) ? ordered(j < a.e.rows ? weights[j] : -INFINITY) : 0u; };
+    auto away = [&](int j) { return gap && j < n && page_of(v, b, j) < 0; };
+    auto rank = [&](int j) { return away(j) ? (between(j) ? 0u : kAway) : between(j) ? ordered(j < a.e.rows ? weights[j] : -INFINITY) : 0u; };
     uint32_t held[kHeld ? kHeld : 1];
-    if constexpr (kHeld > 0)
+    if constexpr (kHeld > 0) {
 #pragma unroll
         for (int i = 0; i < kHeld; ++i) held[i] = between(i * kSelectThreads + tid) ? ordered(loaded[i]) : 0u;
-    for (int j = keep + tid; j < a.e.rows; j += kSelectThreads) out[j] = 0.0f;
+        if (gap)
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i)
+                if (const int j = i * kSelectThreads + tid; away(j)) held[i] = between(j) ? 0u : kAway;
+    }
+    for (int j = length + tid; j < a.e.rows; j += kSelectThreads) out[j] = 0.0f;
     uint32_t limit = 0;     // rows above it stay, and the first at_limit of those at it
     int above = 0;          // rows above
     if (need == 0) limit = 0xFFFFFFFFu;
@@ -117,15 +154,17 @@ __global__ __launch_bounds__(kSelectThreads, kHeld <= 16 ? 8 : 4) void select_ke
     const int at_limit = need - above;
     int32_t* list = a.list + ((static_cast<int64_t>(layer) * v.c.batch + b) * v.c.kv_heads + g) * keep;
     const uint64_t below = (uint64_t{1} << lane) - 1;
-    auto stays = [&](int j, uint32_t r) { return j < n && (j < first || j >= last || r > limit); };
-    auto equal = [&](int j, uint32_t r) { return at_limit > 0 && r == limit && j >= first && j < last; };
+    auto stays = [&](int j, uint32_t r) { return j < n && (between(j) ? r > limit : r != kAway); };
+    auto equal = [&](int j, uint32_t r) { return at_limit > 0 && r == limit && between(j); };
+    auto put_at = [&](int place, int j) {
+        list[place] = j;
+        if (place < a.e.rows) out[place] = j < a.e.rows ? weights[j] : 0.0f;
+    };
     auto put = [&](int j, uint64_t over, uint64_t same, int2 ahead) {
         const int o = ahead.x + static_cast<int>(__popcll(over & below)), e = ahead.y + static_cast<int>(__popcll(same & below));
         if (!((over >> lane) & 1) && !((same >> lane) & 1 && e < at_limit)) return;
         const int place = o + min(e, at_limit);
-        if (place >= keep) return;
-        list[place] = j;
-        if (place < a.e.rows) out[place] = j < a.e.rows ? weights[j] : 0.0f;
+        if (place < kept) put_at(place, j);
     };
     auto number = [](uint64_t over, uint64_t same) { return int2{static_cast<int>(__popcll(over)), static_cast<int>(__popcll(same))}; };
     if constexpr (kHeld > 0) {
@@ -174,6 +213,13 @@ __global__ __launch_bounds__(kSelectThreads, kHeld <= 16 ? 8 : 4) void select_ke
             __syncthreads();
         }
     }
+    if (length == kept) return;
+    for (int j = tid; j < n; j += kSelectThreads) {
+        if (!away(j)) continue;
+        int place = kept + (j & (v.c.page_size - 1));
+        for (int p = 0; p < j >> v.page_shift; ++p) place += page_of(v, b, p << v.page_shift) < 0 ? v.c.page_size : 0;
+        if (place < length) put_at(place, j);
+    }
 }
 
 // Copies the kept rows.  Block (x, y, z): a run of rows, sequence and kv head, layer; a thread keeps its piece of a row and takes every
@@ -185,6 +231,7 @@ template <int B>
 __global__ __launch_bounds__(kThreads) void gather_kernel(View v, Strides st, EvictArgs a, int rows_each) {
     using U = typename Unit<B>::type;
     const int b = blockIdx.y / v.c.kv_heads, g = blockIdx.y % v.c.kv_heads, layer = blockIdx.z, keep = a.e.keep;
+    const int length = a.e.lens_out[b];  // `keep`, or less where rows have no page
     if (table_rows(v, b) <= keep) return;
     const int abreast = max(kThreads / st.per_row, 1), sub = static_cast<int>(threadIdx.x) / st.per_row;
     if (sub >= abreast) return;
@@ -192,16 +239,17 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(View v, Strides st, Ev
     const int32_t* fresh = a.e.fresh + b * a.e.fresh_stride;
     U* k = static_cast<U*>(v.c.k) + layer * st.k_layer + g * st.k_head;
     U* x = static_cast<U*>(v.c.v) + layer * st.v_layer + g * st.v_head;
-    const int begin = blockIdx.x * rows_each, end = begin + min(rows_each, keep - begin);
+    const int begin = blockIdx.x * rows_each, end = min(begin + min(rows_each, keep - begin), length);
+    if (begin >= end) return;
     for (int piece = static_cast<int>(threadIdx.x) % st.per_row; piece < st.per_row; piece += kThreads) {
         for (int row = begin + sub; row < end; row += kRowsAtOnce * abreast) {
             U rk[kRowsAtOnce], rv[kRowsAtOnce];
             int page[kRowsAtOnce], from[kRowsAtOnce], target[kRowsAtOnce];
 #pragma unroll
-            for (int i = 0; i < kRowsAtOnce; ++i) from[i] = list[min(row + i * abreast, keep - 1)];
+            for (int i = 0; i < kRowsAtOnce; ++i) from[i] = list[min(row + i * abreast, end - 1)];
 #pragma unroll
             for (int i = 0; i < kRowsAtOnce; ++i) {
-                const int to = min(row + i * abreast, keep - 1);
+                const int to = min(row + i * abreast, end - 1);
                 page[i] = page_of(v, b, from[i]);
                 target[i] = fresh[to >> v.page_shift];
                 if (row + i * abreast >= end || static_cast<uint32_t>(target[i]) >= static_cast<uint32_t>(v.c.num_pages)) page[i] = -1;

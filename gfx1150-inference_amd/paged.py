@@ -105,6 +105,8 @@ def evict(k_cache, v_cache, table, ctx, weights, fresh, keep: int, recent: int =
     The kept rows are copied, in their order, from ``k_cache`` and ``v_cache`` ``[layers, pages, kv_heads, page_size, head_dim]``
     to the sequence's pages ``fresh`` ``[batch, ceil(keep / page_size)]`` int32, which no sequence may use; the old pages are free
     afterwards unless another sequence shares them.  A sequence of up to ``keep`` rows stays as it is, its fresh pages unused.
+    Rows without a page (``-1`` in the table) are not kept: others take their places, and where there are too few of them the
+    sequence gets shorter than ``keep``.
     The new table is as wide as ``table``, -1 behind a cut sequence's pages; the new weights are 0 behind its rows.  Keys keep the
     positions that they were rotated by: give ``append`` the tokens' ``positions`` from then on."""
     return _on(stream, _ops.evict, k_cache, v_cache, table, ctx, weights, fresh, keep, recent, sinks)

@@ -465,7 +465,8 @@ int qmm_paged_weighted_attention(const qmm_paged_kv* kv, const qmm_paged_query* 
  * of the largest weights [num_layers][batch][kv_heads][rows] (fp32; equal ones go to the lower row; NaN, and a row that
  * `rows` has no place for, count as -inf), `keep` rows in all.  A sequence of at most `keep` rows (that its table has
  * places for) stays as it is.  Of the others the kept rows are copied in their order to rows 0 .. keep - 1 of the pages
- * fresh[b][0 .. fresh_width - 1], which no sequence of the table uses. */
+ * fresh[b][0 .. fresh_width - 1], which no sequence of the table uses.  Rows whose page is outside the table or the pool are
+ * not kept, the first and last ones neither: others take their places, and a sequence with fewer such others ends with them. */
 typedef struct qmm_paged_evict_args {
     const float* weights;
     float* weights_out;   /* alike, not overlapping: the kept rows' weights, 0 behind them */
