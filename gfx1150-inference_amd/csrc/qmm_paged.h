@@ -5,8 +5,10 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <exception>
 #include <string>
+#include <utility>
 
 #include "qmm_internal.h"
 
@@ -106,6 +108,19 @@ inline int bad(const std::string& msg) { return set_last_error(QMM_ERR_INVALID_A
 inline int launched(hipError_t e, const char* what) {
     if (e == hipSuccess) return QMM_OK;
     return set_last_error(QMM_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
+}
+
+// Have the runs of `size` elements of an array of `axes` (count and stride each) a place of their own each?  They have where every axis,
+// by ascending strides, steps over all of the ones before; others are not told apart.
+template <size_t N>
+bool apart(std::pair<int64_t, int64_t> (&&axes)[N], int64_t size) {
+    std::sort(axes, axes + N, [](const auto& x, const auto& y) { return x.second < y.second; });
+    for (const auto& [count, stride] : axes) {
+        if (count <= 1) continue;
+        if (stride < size) return false;
+        size += (count - 1) * stride;
+    }
+    return true;
 }
 
 // Checks a cache description; fills `out`.  need_cu: the call reads cu.

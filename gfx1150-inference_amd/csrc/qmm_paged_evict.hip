@@ -289,6 +289,8 @@ int check_evict(const qmm_paged_kv* kv, const qmm_paged_evict_args* e, View* v) 
     if ((reinterpret_cast<uintptr_t>(e->weights) | reinterpret_cast<uintptr_t>(e->weights_out)) % 4 != 0) return bad("weights must be aligned to their elements.");
     if (v->c.batch > 0 && (e->weights_out == e->weights && e->rows > 0)) return bad("weights_out must not be weights.");
     if (v->c.batch > 0 && (e->table_out == v->c.table || e->lens_out == v->c.ctx)) return bad("table_out and lens_out must not be the inputs.");
+    if (e->rows > 0 && !apart({{v->c.kv_heads, e->wo_head}, {v->c.batch, e->wo_batch}, {v->c.num_layers, e->wo_layer}}, e->rows))
+        return bad("weights_out must not overlap itself.");
     if (v->c.kv_heads > 65535 || v->c.num_layers > 65535 || static_cast<int64_t>(v->c.batch) * v->c.kv_heads > 65535) return bad("too many layers, sequences and heads.");
     return QMM_OK;
 }

@@ -464,11 +464,7 @@ int check_weights(const View& v, const qmm_paged_weights* w) {
     if ((reinterpret_cast<uintptr_t>(w->old_sums) | reinterpret_cast<uintptr_t>(w->new_sums)) % 4 != 0) return bad("old_sums and new_sums must be aligned to their elements.");
     if (w->old_sums == w->new_sums && (w->old_batch != w->new_batch || w->old_head != w->new_head)) return bad("sums in place need the same strides.");
     if (v.c.kv_heads > 65535) return bad("too many heads.");
-    // two sums must not have one place: of the heads within a sequence and of the sequences, or the other way round
-    const int64_t B = v.c.batch, H = v.c.kv_heads, R = w->rows;
-    auto apart = [](int64_t n, int64_t stride, int64_t size) { return n <= 1 || stride >= size; };
-    auto nested = [&](int64_t n1, int64_t s1, int64_t n2, int64_t s2) { return apart(n1, s1, R) && apart(n2, s2, (n1 > 1 ? (n1 - 1) * s1 : 0) + R); };
-    if (R > 0 && !nested(H, w->new_head, B, w->new_batch) && !nested(B, w->new_batch, H, w->new_head)) return bad("new_sums must not overlap itself.");
+    if (w->rows > 0 && !apart({{v.c.kv_heads, w->new_head}, {v.c.batch, w->new_batch}}, w->rows)) return bad("new_sums must not overlap itself.");
     return QMM_OK;
 }
 
