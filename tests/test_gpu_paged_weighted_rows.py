@@ -1,11 +1,12 @@
 """GPU tests of paged.weighted_attention with 17 to 64 rows (tokens x query heads) a kv head: drafted trees and a few tokens of a
-chain behind contexts of several fully cached blocks and several ranges.  Limits as in test_gpu_paged_weighted.py."""
+chain behind contexts of several fully cached blocks and several ranges.  Limits as in test_gpu_paged_weighted.py and, for the
+outputs, test_gpu_paged_attention.py."""
 
 import pytest
 import torch
 
-from test_gpu_paged_attention import Case
-from test_gpu_paged_weighted import _check
+from test_gpu_paged_attention import HALF, Case
+from test_gpu_paged_weighted import _check as _check_sums
 
 pytestmark = pytest.mark.gpu
 
@@ -15,6 +16,13 @@ F16, BF16, E4 = torch.float16, torch.bfloat16, torch.float8_e4m3fn
 def _case(seed, heads, kv, D, page, ctx, new, dtype, cache, mask):
     e4 = cache == E4
     return Case(seed, heads, kv, D, page, ctx, new, dtype, cache, mask, ks=0.0625 if e4 else 1.0, vs=0.3 if e4 else 1.0)
+
+
+def _check(c):
+    out, _ = _check_sums(c)
+    want, spread = c.want()
+    lim = HALF[c.dtype] * (want.abs() + spread) + 4e-5 * spread + 1e-7
+    assert ((out.double().cpu() - want).abs() <= lim).all()
 
 
 @pytest.mark.parametrize("dtype,cache", [(F16, F16), (BF16, BF16), (F16, E4), (BF16, E4)])
