@@ -7,7 +7,7 @@
 // range's maximum (base 2), sum and unnormalised output are joined by a second kernel in the order of the ranges,
 // so a call repeats itself to the bit.  Its bits go by what chooses the kernel and the cut: all sequences' lengths,
 // max_new, alignment, the workgroups that the device runs at once, and, on the vector ALUs, the table's width.  How long a range is, every workgroup works out from all
-// sequences' lengths, which only the device knows (plan_call): the host sees no more than the width of the table.
+// sequences' lengths, which only the device knows (CallPlan in qmm_paged_attention.h): the host sees no more than the width of the table.
 #include "qmm_paged_attention.h"
 
 namespace qmm {

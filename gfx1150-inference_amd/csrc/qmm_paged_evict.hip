@@ -34,8 +34,8 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 // time, by counts of the weights at or above the three numbers that the bits so far begin; where a count is m, those are
 // the rows.  Then the kept rows are listed in order, of those equal to the m-th largest the first ones.  Weights of up to
 // kHeld 1024 rows wait in registers (a count is a comparison and a scalar population count for each 64 of them, with no atomics to
-// meet on); of longer sequences (kHeld 0) they are read for each count.  Bound by the chain of counts: 256 workgroups of 3000 rows 13 us;
-// 768 of up to 8192, of which two thirds choose, 43.
+// meet on); of longer sequences (kHeld 0) they are read for each count.  Bound by the chain of counts: 256 workgroups of 3000 rows 14 us;
+// 768 of up to 8192, of which two thirds choose, 44.
 // A row without a page is no row: nothing of it could be copied, and its place in a fresh page would show what the page held before.
 // Where fewer rows than `keep` have pages the sequence ends with them; past them only places without a fresh page, which show
 // nothing either, count for rows without one.

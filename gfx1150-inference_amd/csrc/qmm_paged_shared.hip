@@ -3,7 +3,7 @@
 // these rows, and every token to the rest of its own sequence's; the partial rows of both, each with its maximum and sum,
 // are joined as those of any two ranges are,
 //   m = max(m1, m2),  out = (2^(m1 - m) o1 + 2^(m2 - m) o2) / (2^(m1 - m) l1 + 2^(m2 - m) l2).
-// Shared rows meet many queries and are bound by the matrix cores (64 tokens of 64 heads behind 16384 rows, 34 GFLOP: 50 us), a
+// Shared rows meet many queries and are bound by the matrix cores (64 tokens of 64 heads behind 16384 rows, 34 GFLOP: 47 us), a
 // sequence's own by their reading (197 MB: 40 us).
 #include "qmm_paged_attention.h"
 

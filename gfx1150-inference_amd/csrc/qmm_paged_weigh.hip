@@ -311,7 +311,7 @@ __global__ __launch_bounds__(kThreads) void weigh_stored_kernel(View v, AttnArgs
 // More rows.  A workgroup takes 64 keys, held in registers as an operand of 32x32x16, and its waves the rows in turns of 32: a lane
 // has one row (lane % 32) and 16 of every 32 keys, so that a row's logarithm is the lane's and the sums of its keys gather in
 // registers; they are added up over the lanes and the waves, in order, at the end.  Two chunks of up to 600 tokens, 32 heads of 128 over
-// up to 2100 keys (14 GFLOP): 50 us, bound by the waits of two waves a SIMD (matrix cores busy for 14 % of the cycles, vector ALUs 33 %).
+// up to 2100 keys (14 GFLOP): 44 us, bound by the waits of two waves a SIMD (matrix cores busy for 14 % of the cycles, vector ALUs 33 %).
 constexpr int kTileKeysW = 64;
 
 template <class T, class C, int D>
@@ -435,7 +435,7 @@ struct WeighPlan {
 };
 
 // The scores of few rows are kept where they cost less than the keys' second reading (16 sequences of up to 16384 keys, 8 rows a kv
-// head of 128 dimensions: the attention takes 143 us with the stores, 114 without; this pass 19 us, 71 with the keys), a byte
+// head of 128 dimensions: the attention takes 143 us with the stores, 114 without; this pass 22 us, 71 with the keys), a byte
 // written for about two read, and do not take too much memory.
 constexpr int64_t kMostScores = int64_t{1} << 29;
 
