@@ -457,8 +457,8 @@ typedef struct qmm_paged_weights {
 } qmm_paged_weights;
 
 /* qmm_paged_tree_attention, and the weights' sums.  Up to 16 rows (tokens x query heads) a kv head the workspace also holds the
- * scores, 4 bytes for each row and each of the sequences' keys that `rows` and the table's width have places for, where
- * that is at most 2^29 bytes; of more the keys are read a second time instead, which takes longer. */
+ * scores where they are less to move than the keys: 4 bytes for each row and each of the sequences' keys that `rows` and the
+ * table's width have places for, 2^29 bytes at most; where they would be more the keys are read a second time, which takes longer. */
 size_t qmm_paged_weighted_workspace(const qmm_paged_kv* kv, const qmm_paged_query* in, const qmm_paged_weights* weights);
 int qmm_paged_weighted_attention(const qmm_paged_kv* kv, const qmm_paged_query* in, const qmm_paged_weights* weights, void* workspace,
                                  size_t workspace_bytes, void* stream);
